@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <string>
 #include <vector>
 
 #include "common/host.h"
@@ -14,6 +15,7 @@
 #include "misc/rowops.h"
 #include "comm/peer.h"
 #include "optim/optim_api.h"
+#include "misc/layer_norm.h"
 #include "misc/norm_variants.h"
 #include "misc/spectral.h"
 
@@ -234,6 +236,72 @@ void bilinear_grad(const Tensor& dy, const Tensor& wd, const Tensor& l, const Te
                           dl.stride(0), static_cast<int>(mode), cur_stream());
 }
 
+
+// ------------------------------------------------------------------ layer norm
+ttb::ScalarType scalar_type(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return ttb::ScalarType::kF32;
+    case torch::kBFloat16: return ttb::ScalarType::kBF16;
+    case torch::kFloat16: return ttb::ScalarType::kF16;
+    default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16");
+  }
+}
+
+void check_rows(const Tensor& t, const char* name, const Tensor& like) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.device() == like.device(), name, " must be on the device of the input");
+  TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), name, " must be 2-D with a unit column stride");
+}
+
+// Numbers enter the messages as std::to_string text: with libstdc++ linked statically into this library,
+// torch's own stream formatting of a number crashes while the error is being raised.
+void check_f32_vector(const Tensor& t, const char* name, int64_t n, const Tensor& like) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.device() == like.device(), name, " must be on the device of the input");
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.numel() == n, name,
+              " must be a contiguous float32 vector of " + std::to_string(n) + " elements");
+}
+
+// x [N, d] -> (y [N, d], mean [N], rstd [N]); the statistics are empty unless asked for.
+std::vector<Tensor> layer_norm_fwd(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& b, double eps,
+                                   torch::ScalarType out, bool stats) {
+  check_rows(x, "x", x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t N = x.size(0), d = x.size(1);
+  TORCH_CHECK(d >= 1 && d <= ttb::kLayerNormMaxDim, "layer norm: the last dimension must be between 1 and " +
+              std::to_string(ttb::kLayerNormMaxDim) + ", not " + std::to_string(d));
+  check_f32_vector(w, "weight", d, x);
+  if (b.has_value()) check_f32_vector(*b, "bias", d, x);
+  auto y = torch::empty({N, d}, x.options().dtype(out));
+  auto stat = torch::empty({2, stats ? N : 0}, x.options().dtype(torch::kFloat32));
+  float* sp = stats && N > 0 ? stat.data_ptr<float>() : nullptr;
+  ttb::layer_norm_fwd({N, static_cast<int>(d), scalar_type(x, "x"), scalar_type(y, "the output")}, x.data_ptr(),
+                      x.stride(0), w.data_ptr<float>(), b.has_value() ? b->data_ptr<float>() : nullptr, y.data_ptr(),
+                      sp, sp == nullptr ? nullptr : sp + N, static_cast<float>(eps), cur_stream());
+  return {y, stat};
+}
+
+// stat: the forward's [2, N] (mean, rstd).  Returns (dx, dw, db).
+std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& stat) {
+  check_rows(x, "x", x);
+  check_rows(dy, "dy", x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t N = x.size(0), d = x.size(1);
+  TORCH_CHECK(dy.size(0) == N && dy.size(1) == d, "dy must have x's shape");
+  check_f32_vector(w, "weight", d, x);
+  check_f32_vector(stat, "stat", 2 * N, x);
+  auto dx = torch::empty({N, d}, x.options());
+  auto dwb = N > 0 ? torch::empty({2, d}, w.options()) : torch::zeros({2, d}, w.options());
+  if (N > 0) {
+    const ttb::LayerNormShape s{N, static_cast<int>(d), scalar_type(x, "x"), scalar_type(dy, "dy")};
+    auto part = torch::empty({ttb::layer_norm_bwd_partials(s), 2 * d}, w.options());
+    const float* sp = stat.data_ptr<float>();
+    ttb::layer_norm_bwd(s, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), w.data_ptr<float>(), sp, sp + N,
+                        dx.data_ptr(), dwb.data_ptr<float>(), dwb.data_ptr<float>() + d, part.data_ptr<float>(),
+                        cur_stream());
+  }
+  return {dx, dwb.select(0, 0), dwb.select(0, 1)};
+}
 
 // ------------------------------------------------------------------ row ops
 std::vector<Tensor> rmsnorm_fwd(const Tensor& x, const Tensor& w, int64_t groups, double eps) {
@@ -751,6 +819,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_bwd", &rmsnorm_bwd, "(group) RMSNorm backward; adds dx into the residual grad, returns dw",
         py::arg("dy"), py::arg("x"), py::arg("w"), py::arg("rstd"), py::arg("dres"), py::arg("accumulate"),
         py::arg("groups"), py::arg("out16") = py::none(), py::arg("scale16") = 1.0);
+  m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm: y and, on request, the rows' mean and 1/std", py::arg("x"),
+        py::arg("w"), py::arg("b"), py::arg("eps"), py::arg("out"), py::arg("stats"));
+  m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward: dx, dw, db", py::arg("dy"), py::arg("x"),
+        py::arg("w"), py::arg("stat"));
   m.def("rope_", &rope_, "in-place rotary embedding (or its inverse) on a bf16 [N, ld] buffer");
   m.def("embed_fwd", &embed_fwd, "fp32 embedding gather");
   m.def("embed_bwd", &embed_bwd, "deterministic embedding backward (accumulates into dW)");

@@ -1,0 +1,116 @@
+// Vector loads and stores of fp32, bf16 and fp16 rows as fp32 registers, the choice of a kernel instance by
+// element type, and small warp reductions.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include <stdexcept>
+#include <type_traits>
+
+#include "dtype.h"
+
+namespace ttb {
+
+// Calls f with a null pointer of the element type that `t` names.
+template <typename F>
+void with_type(ScalarType t, F&& f) {
+  switch (t) {
+    case ScalarType::kF32: return f(static_cast<float*>(nullptr));
+    case ScalarType::kBF16: return f(static_cast<__nv_bfloat16*>(nullptr));
+    case ScalarType::kF16: return f(static_cast<__half*>(nullptr));
+  }
+  throw std::invalid_argument("tensor_train_ing_b200: unknown scalar type");
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+  else return __float2half_rn(v);
+}
+
+// Two 16-bit elements of type T held in one 32-bit word.
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t u, float& lo, float& hi) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    lo = __uint_as_float(u << 16);
+    hi = __uint_as_float(u & 0xFFFF0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    lo = f.x;
+    hi = f.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// V consecutive elements (V = 1, 4 or 8; p aligned to V elements, at most 16 bytes per access).
+template <int V, typename T>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const float4 u = reinterpret_cast<const float4*>(p)[i];
+      v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+    }
+  } else if constexpr (V == 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    unpack2<T>(u.x, v[0], v[1]);
+    unpack2<T>(u.y, v[2], v[3]);
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    unpack2<T>(u.x, v[0], v[1]);
+    unpack2<T>(u.y, v[2], v[3]);
+    unpack2<T>(u.z, v[4], v[5]);
+    unpack2<T>(u.w, v[6], v[7]);
+  }
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else if constexpr (V == 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+  } else {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Barrier `id` (1..15) among the `threads` threads of a group of warps of the block.
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+}  // namespace ttb

@@ -1,0 +1,66 @@
+"""Layer norm on the sm_100a kernels (csrc/misc/layer_norm.cu), forward and backward:
+
+    mu = mean_j x,  rstd = 1 / sqrt(mean_j (x - mu)^2 + eps),  xhat = (x - mu) rstd,  y = xhat * weight + bias
+    g = dy * weight,  dx = rstd (g - mean_j g - xhat mean_j (g xhat)),  dweight = sum_n dy xhat,  dbias = sum_n dy
+
+``models.normalization.LayerNorm`` is the module that uses it and, in plain PyTorch, its definition.
+"""
+from __future__ import annotations
+
+import torch
+
+from ._ext import lib
+
+MAX_DIM = 16384
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class LayerNormFn(torch.autograd.Function):
+    """x: [N, d] rows.  The backward reads x again with the forward's per-row mean and rstd; weight and
+    bias gradients are summed in a fixed order (the same inputs give the same bits)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, out_dtype):
+        y, stat = lib().layer_norm_fwd(x, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(x, weight, stat)
+        ctx.has_bias = bias is not None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stat = ctx.saved_tensors
+        if dy.stride(-1) != 1:
+            dy = dy.contiguous()
+        dx, dw, db = lib().layer_norm_bwd(dy, x, weight, stat)
+        return dx, dw, db if ctx.has_bias else None, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Normalise ``x`` (..., d) over its last dimension.
+
+    ``x``: fp32, bf16 or fp16 on CUDA, any strides (rows with a unit column stride are read in place),
+    1 <= d <= 16384.  ``weight`` and the optional ``bias``: fp32 [d].  The result is ``out_dtype`` (default
+    x's), dense.  Statistics and sums are fp32; the result is rounded once.  Runs on the current stream."""
+    if not x.is_cuda:
+        raise ValueError("layer_norm: x must be a CUDA tensor (models.normalization.LayerNorm has the CPU form)")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if x.dtype not in _FLOATS or out_dtype not in _FLOATS:
+        raise TypeError(f"layer_norm: x and the result must be float32, bfloat16 or float16, not {x.dtype} -> {out_dtype}")
+    d = x.shape[-1] if x.dim() else 0
+    if not 1 <= d <= MAX_DIM:
+        raise ValueError(f"layer_norm: the last dimension must be between 1 and {MAX_DIM}, not {d}")
+    if not eps >= 0:
+        raise ValueError(f"layer_norm: eps must not be negative ({eps})")
+    rows = x if x.dim() == 2 else x.reshape(-1, d)
+    if rows.stride(1) != 1 and d > 1:
+        rows = rows.contiguous()
+    weight = weight.contiguous()
+    bias = bias.contiguous() if bias is not None else None
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        y = LayerNormFn.apply(rows, weight, bias, float(eps), out_dtype)
+    else:
+        y = lib().layer_norm_fwd(rows, weight, bias, float(eps), out_dtype, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
