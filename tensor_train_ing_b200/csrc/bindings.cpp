@@ -10,6 +10,7 @@
 
 #include "common/host.h"
 #include "attn/attn_api.h"
+#include "distill/distill_api.h"
 #include "gemm/api.h"
 #include "gemm/ce_api.h"
 #include "misc/rowops.h"
@@ -301,6 +302,104 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x, const Tens
                         cur_stream());
   }
   return {dx, dwb.select(0, 0), dwb.select(0, 1)};
+}
+
+// ------------------------------------------------------------------ distillation
+// z [N, V] -> (values [N, k], ids int32 [N, k], lse [N])
+std::vector<Tensor> top_logits(const Tensor& z, int64_t k, double tau) {
+  check_rows(z, "logits", z);
+  const c10::cuda::CUDAGuard guard(z.device());
+  const int64_t N = z.size(0), V = z.size(1);
+  TORCH_CHECK(V >= 1 && V < (1LL << 31) && k >= 1 && k <= V && k <= ttb::kTopLogitsMaxK,
+              "top_logits: k must be between 1 and min(" + std::to_string(ttb::kTopLogitsMaxK) + ", columns), not " +
+                  std::to_string(k));
+  auto values = torch::empty({N, k}, z.options());
+  auto ids = torch::empty({N, k}, z.options().dtype(torch::kInt32));
+  auto lse = torch::empty({N}, z.options().dtype(torch::kFloat32));
+  ttb::TopLogitsArgs a{};
+  a.z = z.data_ptr();
+  a.ldz = z.stride(0);
+  a.type = scalar_type(z, "logits");
+  a.rows = N;
+  a.vocab = static_cast<int>(V);
+  a.k = static_cast<int>(k);
+  a.inv_tau = static_cast<float>(1.0 / tau);
+  a.values = values.data_ptr();
+  a.ids = ids.data_ptr<int>();
+  a.lse = lse.data_ptr<float>();
+  ttb::top_logits(a, cur_stream());
+  return {values, ids, lse};
+}
+
+// (loss [N] fp32, dz or an undefined tensor).  dz is given (its columns past V are zeroed) or not wanted.
+Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c10::optional<Tensor>& teacher_lse,
+                    const c10::optional<Tensor>& targets, double tau, double kd, double ce,
+                    const c10::optional<Tensor>& scale, const c10::optional<Tensor>& dz) {
+  check_rows(z, "logits", z);
+  const c10::cuda::CUDAGuard guard(z.device());
+  const int64_t N = z.size(0), V = z.size(1), K = ids.size(-1);
+  TORCH_CHECK(V >= 1 && V < (1LL << 31), "the logits have no columns");
+  for (const Tensor* q : {&ids, &t}) {
+    check_cuda(*q, "the teacher's list");
+    TORCH_CHECK(q->device() == z.device() && q->dim() == 2 && q->is_contiguous() && q->size(0) == N && q->size(1) == K,
+                "teacher_ids and teacher_logits must be dense [rows, k] on the logits' device");
+  }
+  TORCH_CHECK(ids.scalar_type() == torch::kInt32 || ids.scalar_type() == torch::kInt64, "teacher_ids: int32 or int64");
+  TORCH_CHECK(K >= 1 && K <= ttb::kDistillMaxList, "the teacher's list must have between 1 and " +
+              std::to_string(ttb::kDistillMaxList) + " entries, not " + std::to_string(K));
+  if (teacher_lse.has_value()) check_f32_vector(*teacher_lse, "teacher_lse", N, z);
+  if (targets.has_value())
+    TORCH_CHECK(targets->device() == z.device() && targets->scalar_type() == torch::kInt64 &&
+                    targets->is_contiguous() && targets->numel() == N,
+                "targets must be dense int64 [rows] on the logits' device");
+  TORCH_CHECK(ce == 0.0 || targets.has_value(), "the cross-entropy term needs targets");
+  if (scale.has_value()) check_f32_vector(*scale, "scale", 1, z);
+  auto loss = torch::empty({N}, z.options().dtype(torch::kFloat32));
+  ttb::DistillArgs a{};
+  a.z = z.data_ptr();
+  a.ldz = z.stride(0);
+  a.z_type = scalar_type(z, "logits");
+  a.rows = N;
+  a.vocab = static_cast<int>(V);
+  a.ids = ids.data_ptr();
+  a.ids64 = ids.scalar_type() == torch::kInt64;
+  a.t = t.data_ptr();
+  a.t_type = scalar_type(t, "teacher_logits");
+  a.k = static_cast<int>(K);
+  a.teacher_lse = teacher_lse.has_value() ? teacher_lse->data_ptr<float>() : nullptr;
+  a.targets = targets.has_value() ? reinterpret_cast<const long long*>(targets->data_ptr<int64_t>()) : nullptr;
+  a.tau = static_cast<float>(tau);
+  a.kd = static_cast<float>(kd);
+  a.ce = static_cast<float>(ce);
+  a.scale = scale.has_value() ? scale->data_ptr<float>() : nullptr;
+  a.loss = loss.data_ptr<float>();
+  if (dz.has_value()) {
+    check_rows(*dz, "dz", z);
+    TORCH_CHECK(dz->size(0) == N && dz->size(1) >= V, "dz must have the logits' rows and at least their columns");
+    a.dz = dz->data_ptr();
+    a.lddz = dz->stride(0);
+    a.dz_cols = static_cast<int>(dz->size(1));
+    a.dz_type = scalar_type(*dz, "dz");
+  }
+  a.status = ttb::status_ptr();
+  ttb::distill_loss(a, cur_stream());
+  return loss;
+}
+
+// Rows of dz times g (one factor, or one per row), in place; a factor of 1 leaves its row untouched.
+void scale_rows_(Tensor& dz, const Tensor& g) {
+  check_rows(dz, "dz", dz);
+  const c10::cuda::CUDAGuard guard(dz.device());
+  const int64_t N = dz.size(0);
+  check_f32_vector(g, "g", g.numel() == 1 ? 1 : N, dz);
+  ttb::scale_in_place(dz.data_ptr(), scalar_type(dz, "dz"), N, static_cast<int>(dz.size(1)), dz.stride(0),
+                      g.data_ptr<float>(), g.numel() == 1 ? 0 : 1, cur_stream());
+}
+
+bool logits_row_fits(int64_t columns, torch::ScalarType type) {
+  return columns < (1LL << 31) && ttb::logits_row_fits(static_cast<int>(columns), type == torch::kFloat32
+                                                                                      ? ttb::ScalarType::kF32
+                                                                                      : ttb::ScalarType::kBF16);
 }
 
 // ------------------------------------------------------------------ row ops
@@ -823,6 +922,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("w"), py::arg("b"), py::arg("eps"), py::arg("out"), py::arg("stats"));
   m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward: dx, dw, db", py::arg("dy"), py::arg("x"),
         py::arg("w"), py::arg("stat"));
+  m.def("top_logits", &top_logits, "the k largest logits of each row, their columns and the row's log-sum-exp",
+        py::arg("z"), py::arg("k"), py::arg("tau"));
+  m.def("distill_loss", &distill_loss, "distillation loss of each row and, into dz, its gradient", py::arg("z"),
+        py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),
+        py::arg("ce"), py::arg("scale"), py::arg("dz"));
+  m.def("scale_rows_", &scale_rows_, "rows of dz times their factor, in place", py::arg("dz"), py::arg("g"));
+  m.def("logits_row_fits", &logits_row_fits, "whether rows of this many logits fit the distillation kernels");
   m.def("rope_", &rope_, "in-place rotary embedding (or its inverse) on a bf16 [N, ld] buffer");
   m.def("embed_fwd", &embed_fwd, "fp32 embedding gather");
   m.def("embed_bwd", &embed_bwd, "deterministic embedding backward (accumulates into dW)");

@@ -1,0 +1,164 @@
+"""Distillation from a teacher's top logits, on the sm_100a kernels of csrc/distill:
+
+  top_logits          the k largest logits of each row, their columns, and the row's log-sum-exp
+  distillation_loss   the loss of a student's logits against such a list, differentiable
+
+With a_i = t_i / tau over the teacher's listed columns c_i, q = softmax(z / tau) of the student's logits z and
+q_rest the student's mass on all columns that are not listed:
+
+  p_i  = exp(a_i - L),  L = teacher_lse (then m = 1 - sum p_i is the teacher's mass on the rest), or the
+         log-sum-exp of the list itself (then m = 0: the teacher is renormalised over its list)
+  KL   = sum_i p_i (log p_i - log q_{c_i}) + m (log m - log q_rest)
+  loss = scale (kd_weight tau^2 KL + ce_weight (log sum_j exp z_j - z_target))
+
+tau^2 keeps the gradient's size independent of the temperature (Hinton, Vinyals, Dean 2015, section 2.1).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from ._ext import lib
+
+MAX_TOP = 256
+MAX_LIST = 1024
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class TopLogits(NamedTuple):
+    """``values`` (..., k) of the logits' type in descending order, ``ids`` int32 (..., k) their columns,
+    ``lse`` fp32 (...) the log-sum-exp of the whole row over the temperature."""
+    values: torch.Tensor
+    ids: torch.Tensor
+    lse: torch.Tensor
+
+
+def _rows(logits: torch.Tensor, what: str) -> torch.Tensor:
+    """The logits as [N, V] rows with a unit column stride (a view where there is one)."""
+    if not logits.is_cuda:
+        raise ValueError(f"{what}: the logits must be a CUDA tensor")
+    if logits.dtype not in _FLOATS:
+        raise TypeError(f"{what}: the logits must be float32, bfloat16 or float16, not {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: the logits need at least one column, not {tuple(logits.shape)}")
+    if not lib().logits_row_fits(logits.shape[-1], logits.dtype):
+        raise ValueError(f"{what}: rows of {logits.shape[-1]} logits exceed the shared memory of a cluster")
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    return rows if rows.stride(1) == 1 or rows.shape[1] == 1 else rows.contiguous()
+
+
+@torch.no_grad()
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The ``k`` largest logits of each row (1 <= k <= 256), in descending order; equal logits by
+    the lower column first; NaN counts as the largest value.  Not differentiable: it prepares a
+    teacher's list.  ``lse`` is that of ``logits / temperature``, as ``distillation_loss`` takes it."""
+    if not temperature > 0:
+        raise ValueError(f"top_logits: the temperature must be positive, not {temperature}")
+    rows = _rows(logits, "top_logits")
+    if not 1 <= k <= min(MAX_TOP, rows.shape[1]):
+        raise ValueError(f"top_logits: k must be between 1 and {min(MAX_TOP, rows.shape[1])}, not {k}")
+    values, ids, lse = lib().top_logits(rows, int(k), float(temperature))
+    if logits.dim() == 2:
+        return TopLogits(values, ids, lse)
+    lead = logits.shape[:-1]
+    return TopLogits(values.view(*lead, k), ids.view(*lead, k), lse.view(lead))
+
+
+def _gradient_like(rows: torch.Tensor) -> torch.Tensor:
+    """An uninitialised gradient with the rows' stride where that wastes little: its rows then have
+    the alignment of the logits' rows, and the kernel stores whole vectors."""
+    n, v = rows.shape
+    ld = rows.stride(0) if n > 1 else v
+    return torch.empty_strided((n, v), (ld if v <= ld < v + 64 else v, 1), dtype=rows.dtype, device=rows.device)
+
+
+class DistillationFn(torch.autograd.Function):
+    """The forward forms the gradient in the same pass over the logits and keeps it instead of them; the
+    backward multiplies it by the incoming factor in place (nothing to do when that is 1, which ``scale``
+    makes the usual case).  It can therefore run once."""
+
+    @staticmethod
+    def forward(ctx, rows, ids, t, teacher_lse, targets, tau, kd, ce, scale, reduction):
+        dz = _gradient_like(rows)
+        loss = lib().distill_loss(rows, ids, t, teacher_lse, targets, tau, kd, ce, scale, dz)
+        ctx.dz = dz
+        return loss.sum() if reduction == "sum" else loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        dz, ctx.dz = ctx.dz, None
+        if dz is None:
+            raise RuntimeError("distillation_loss: the gradient was handed out by an earlier backward")
+        lib().scale_rows_(dz, g.contiguous())
+        return (dz,) + (None,) * 9
+
+
+def _list_arguments(rows, teacher_ids, teacher_logits, teacher_lse, targets, ce_weight, scale):
+    n = rows.shape[0]
+    if teacher_ids.shape != teacher_logits.shape or teacher_ids.dim() < 1:
+        raise ValueError(f"distillation_loss: teacher_ids {tuple(teacher_ids.shape)} and teacher_logits "
+                         f"{tuple(teacher_logits.shape)} must have the same shape")
+    k = teacher_ids.shape[-1]
+    if not 1 <= k <= MAX_LIST:
+        raise ValueError(f"distillation_loss: the list must have between 1 and {MAX_LIST} entries, not {k}")
+    if teacher_ids.numel() != n * k:
+        raise ValueError(f"distillation_loss: {teacher_ids.numel() // k} lists for {n} rows of logits")
+    if teacher_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"distillation_loss: teacher_ids must be int32 or int64, not {teacher_ids.dtype}")
+    if teacher_logits.dtype not in _FLOATS:
+        raise TypeError(f"distillation_loss: teacher_logits must be float32, bfloat16 or float16, not "
+                        f"{teacher_logits.dtype}")
+    if ce_weight != 0 and targets is None:
+        raise ValueError("distillation_loss: the cross-entropy term needs targets")
+    for name, value in (("teacher_lse", teacher_lse), ("targets", targets)):
+        if value is not None and value.numel() != n:
+            raise ValueError(f"distillation_loss: {name} has {value.numel()} elements for {n} rows")
+    if teacher_lse is not None:
+        teacher_lse = teacher_lse.detach().reshape(-1).float().contiguous()
+    if targets is not None:
+        targets = targets.reshape(-1).contiguous()
+    if scale is not None:
+        if not isinstance(scale, torch.Tensor):
+            scale = torch.full((1,), float(scale), device=rows.device)
+        if scale.numel() != 1:
+            raise ValueError(f"distillation_loss: scale must be one number, not {tuple(scale.shape)}")
+        scale = scale.detach().reshape(1).float()
+    return (teacher_ids.reshape(n, k).contiguous(), teacher_logits.detach().reshape(n, k).contiguous(), teacher_lse,
+            targets, scale)
+
+
+def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                      teacher_lse: torch.Tensor | None = None, targets: torch.Tensor | None = None,
+                      temperature: float = 1.0, kd_weight: float = 1.0, ce_weight: float = 0.0,
+                      scale: torch.Tensor | float | None = None, reduction: str = "sum") -> torch.Tensor:
+    """Loss of ``logits`` (..., V) against a teacher's lists, summed over rows or (``reduction="none"``) per row.
+
+    ``teacher_ids`` / ``teacher_logits`` (..., k), 1 <= k <= 1024: columns (int32 or int64) and logits of the
+    teacher, distinct columns in any order; an entry with a negative id is absent, and a row without entries
+    has no divergence.  An id past the vocabulary is recorded in the status word (``ops._ext.check_status``)
+    and counts as absent.  ``teacher_lse`` (...): the log-sum-exp of the teacher's whole row over the same
+    temperature (``top_logits(...).lse``); without it the teacher is renormalised over its list.
+    ``targets`` (...) int64: rows with a negative target (-100) are left out entirely, loss and gradient zero;
+    they are required when ``ce_weight`` is not 0.  ``scale`` (a number or a one-element tensor, e.g. one over
+    the update's target count) multiplies loss and gradient inside the kernel, before the gradient is rounded
+    to the logits' type, so that ``backward()`` has nothing left to do.
+
+    Differentiable with respect to ``logits`` alone, once.  A teacher's mass outside its list at or below
+    2^-20 counts as none (that is what rounding leaves of 1 - sum p)."""
+    if not temperature > 0:
+        raise ValueError(f"distillation_loss: the temperature must be positive, not {temperature}")
+    if reduction not in ("sum", "none"):
+        raise ValueError(f"distillation_loss: reduction must be 'sum' or 'none', not {reduction!r}")
+    rows = _rows(logits, "distillation_loss")
+    ids, t, teacher_lse, targets, scale = _list_arguments(rows, teacher_ids, teacher_logits, teacher_lse, targets,
+                                                          ce_weight, scale)
+    args = (ids, t, teacher_lse, targets, float(temperature), float(kd_weight), float(ce_weight), scale)
+    if torch.is_grad_enabled() and rows.requires_grad:
+        loss = DistillationFn.apply(rows, *args, reduction)
+    else:
+        loss = lib().distill_loss(rows, *args, None)
+        if reduction == "sum":
+            loss = loss.sum()
+    return loss if reduction == "sum" or logits.dim() == 2 else loss.view(logits.shape[:-1])
