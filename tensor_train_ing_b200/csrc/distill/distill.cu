@@ -1,14 +1,22 @@
 // Distillation from a teacher's top logits: the loss of every row and, in the same pass over the logits, its
 // gradient (formulas in distill_api.h).
 //
-// A row sits in the shared memory of a cluster (row_slice.cuh), so the gradient needs no second read of
-// it.  The listed columns are taken out of the slice first (replaced by -inf): what the passes over the slice
-// then sum is the rest of the row, whose mass q_rest is thereby never the difference of two nearly equal
-// numbers.  With M the largest unlisted logit, every unlisted column's gradient is
-//     exp((z_j - M) / tau) A + exp(z_j - M) B,
-//     A = scale kd tau ((P + m) exp(M / tau - lse_tau) - m / S),  S = sum over the rest of exp((z - M) / tau)
-//     B = scale ce exp(M - lse_1)
-// which overflows nowhere; the few listed columns and the target are written after the others.
+// A row sits in the shared memory of a cluster, usually of one CTA (row_slice.cuh), so the gradient needs no second
+// read of it.  While it arrives, every thread takes the maximum of its elements and the first warp reads the
+// teacher's list with the student's logits at it.  The listed columns are then taken out of the slice
+// (replaced by -inf): what the passes over the slice sum is the rest of the row, whose mass q_rest is thereby never the
+// difference of two nearly equal numbers.  With R the row's reference (its largest logit), every unlisted
+// column's gradient is
+//     exp((z_j - R) / tau) A + exp(z_j - R) B,
+//     A = scale kd tau ((P + m) / T - m / S),  S, T = sums of exp((z - R) / tau) over the rest and the row
+//     B = scale ce / T1,                       T1 = sum of exp(z - R) over the row
+// and the few listed columns and the target are written after the others.  Should S vanish in fp32 because the rest lies
+// far below the list, it is summed again relative to the rest's own largest logit.
+//
+// POW: how exp(z - R) of the cross-entropy follows from e = exp((z - R) / tau) of the divergence: not needed or the
+// same (0), e^2 or e^4 for the temperatures 2 and 4 (a product is cheaper than a second exponential: the
+// special-function unit gives 16 a cycle and SM, and two more per element would bound 16-bit logits), else (1) by
+// another exponential.
 #include "../common/host.h"
 #include "distill_api.h"
 #include "row_slice.cuh"
@@ -19,24 +27,26 @@ namespace {
 using rows::Slice;
 namespace cg = cooperative_groups;
 
-struct Part {  // what one CTA knows of its slice; sums are relative to the maxima
-  float rest_max, rest_sum, rest_sum1;  // unlisted columns, at tau and at 1
-  float list_max, list_sum, list_sum1;  // listed columns (each counted once)
+struct Part {  // what one CTA knows of its slice; sums are relative to ref
+  float ref;
+  float rest, rest1;  // unlisted columns, at tau and at 1
+  float list, list1;  // listed columns (each counted once)
   int listed;
 };
 
 struct Shared {
-  Part part[rows::kMaxParts];
-  float red[32][4];
+  Part part[rows::kMaxParts], again_part[rows::kMaxParts];
+  float red[rows::kMaxThreads / 32][4];
+  float red_max[rows::kMaxThreads / 32];
   float target_logit;
   float mass, rest;  // P and m
-  int entries;       // present entries of the list
-  // the row's scalars for the gradient: q_j = exp((z_j - top) / tau) inv_sum
+  // the row's scalars for the gradient: q_j = exp((z_j - top) / tau) inv_sum, the passes over the slice use ref
   float ref, A, B, top, inv_sum, inv_sum1, all_mass;
+  int again, repeats, target_listed, listed;
 };
 
 struct Params {
-  int vocab, k, per, dz_cols;
+  int vocab, k, per, parts, dz_cols;
   bool ids64;
   float inv_tau, tau, kd, ce;
   const void* ids;
@@ -47,37 +57,6 @@ struct Params {
   long long ldz, lddz;
   uint32_t* status;
 };
-
-template <int N>
-__device__ __forceinline__ void block_reduce_max(float (&v)[N], float (*red)[4]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_max(v[i]);
-  if ((threadIdx.x & 31) == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) red[threadIdx.x >> 5][i] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = red[0][i];
-    for (int w = 1; w < blockDim.x / 32; ++w) v[i] = fmaxf(v[i], red[w][i]);
-  }
-  __syncthreads();
-}
-template <int N>
-__device__ __forceinline__ void block_reduce_sum(float (&v)[N], float (*red)[4]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if ((threadIdx.x & 31) == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) red[threadIdx.x >> 5][i] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = red[0][i];
-    for (int w = 1; w < blockDim.x / 32; ++w) v[i] += red[w][i];
-  }
-  __syncthreads();
-}
 
 // Entry i of the shared-memory copy of the teacher's list.
 struct Entry {
@@ -99,60 +78,80 @@ __device__ __forceinline__ int get_mark(const T* p) {
   else return *reinterpret_cast<const unsigned short*>(p);
 }
 
-// TWO: cross-entropy at another temperature than the divergence's, which needs a second exponential.
-template <typename TZ, typename TT, typename TG, bool GRAD, bool TWO>
-__global__ void __launch_bounds__(512) distill_kernel(const TZ* __restrict__ z, const TT* __restrict__ t,
-                                                      TG* __restrict__ dz, const __grid_constant__ Params p) {
+// Threads first, first + step, ... write the row's zeros: 16 bytes each between the ragged ends.
+template <typename T>
+__device__ __forceinline__ void zero_row(T* row, int cols, int first, int step) {
+  constexpr int E = 16 / static_cast<int>(sizeof(T));
+  const int head = min(cols, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(T)));
+  const int vecs = (cols - head) / E;
+  for (int i = first; i < head; i += step) row[i] = from_f32<T>(0.f);
+  for (int i = first; i < vecs; i += step) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = head + vecs * E + first; i < cols; i += step) row[i] = from_f32<T>(0.f);
+}
+
+template <int POW>
+__device__ __forceinline__ float2 at_one(float2 e, float2 x) {  // exp(z - R) from e and x = (z - R) log2(e) / tau
+  if constexpr (POW == 2) {
+    return rows::mul2(e, e);
+  } else if constexpr (POW == 4) {
+    const float2 sq = rows::mul2(e, e);
+    return rows::mul2(sq, sq);
+  } else {
+    return make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
+  }
+}
+
+template <typename TZ, typename TT, typename TG, bool GRAD, int POW>
+__global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __restrict__ z,
+                                                                   const TT* __restrict__ t, TG* __restrict__ dz,
+                                                                   const __grid_constant__ Params p) {
   constexpr int E = Slice<TZ>::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = cluster.num_blocks(), rank = cluster.block_rank();
+  const int parts = p.parts, rank = parts > 1 ? cluster.block_rank() : 0;
   const long long row = blockIdx.x / parts;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   auto* list = reinterpret_cast<Entry*>(smem + static_cast<size_t>(p.per) * 16);
   const TZ* zrow = z + row * p.ldz;
   TG* drow = GRAD ? dz + row * p.lddz : nullptr;
 
   long long target = -1;
-  bool live = true;
   if (p.targets != nullptr) {
     target = p.targets[row];
-    if (target >= p.vocab) {
-      if (rank == 0 && tid == 0) record_error(p.status, kErrBadIndex);
-      target = -1;
+    if (target >= p.vocab && rank == 0 && tid == 0) record_error(p.status, kErrBadIndex);
+    if (target < 0 || target >= p.vocab) {  // the same for the whole cluster
+      if (rank == 0 && tid == 0) p.loss[row] = 0.f;
+      if (GRAD) zero_row(drow, p.dz_cols, rank * blockDim.x + tid, parts * blockDim.x);
+      return;
     }
-    live = target >= 0;
-  }
-  if (!live) {  // the same for the whole cluster
-    if (rank == 0 && tid == 0) p.loss[row] = 0.f;
-    if (GRAD)
-      for (int c = rank * blockDim.x + tid; c < p.dz_cols; c += parts * blockDim.x) drow[c] = from_f32<TG>(0.f);
-    return;
   }
 
   const Slice<TZ> s = rows::start_load(reinterpret_cast<TZ*>(smem), zrow, p.vocab, rank, p.per);
-
-  // the teacher's list, by the first warp of every CTA, while the row arrives
   if (warp == 0) {
+    // The teacher's list and the student's logits at it, by every CTA for itself.
     float top = -CUDART_INF_F;
     int present = 0;
+    bool has_target = false;
     for (int i = lane; i < p.k; i += 32) {
       long long c = p.ids64 ? static_cast<const long long*>(p.ids)[row * p.k + i]
                             : static_cast<const int*>(p.ids)[row * p.k + i];
+      const float raw = to_f32(t[row * p.k + i]) * p.inv_tau;
       if (c >= p.vocab) {
         if (rank == 0) record_error(p.status, kErrBadIndex);
         c = -1;
       }
-      const float a = c < 0 ? -CUDART_INF_F : to_f32(t[row * p.k + i]) * p.inv_tau;
+      const float a = c < 0 ? -CUDART_INF_F : raw;
       list[i].col = c < 0 ? -1 : static_cast<int>(c);
       list[i].logp = a;
-      list[i].z = 0.f;
-      list[i].owner = 0;
+      list[i].z = c < 0 ? 0.f : to_f32(zrow[c]);
       top = fmaxf(top, a);
       present += c >= 0;
+      has_target |= c >= 0 && c == target;
     }
+    const float target_logit = p.ce != 0.f ? to_f32(zrow[target]) : 0.f;
     present = __reduce_add_sync(0xffffffffu, present);
+    has_target = __any_sync(0xffffffffu, has_target);
     top = warp_max(top);
     // p_i = exp(a_i - base) / sum
     float base = 0.f, inv = 1.f, log_sum = 0.f;
@@ -178,196 +177,235 @@ __global__ void __launch_bounds__(512) distill_kernel(const TZ* __restrict__ z, 
       const float rest = p.teacher_lse != nullptr && present > 0 ? 1.f - mass : 0.f;
       sh.mass = mass;
       sh.rest = rest > kDistillLeastRest ? rest : 0.f;
-      sh.entries = present;
+      sh.target_logit = target_logit;
+      sh.target_listed = has_target;
+      sh.again = sh.repeats = sh.listed = 0;
     }
   }
-  rows::finish_load();
-  if (parts > 1) cluster.sync();  // every CTA of the row runs: its shared memory may be written
-
-  // Take the listed logits out of the slice: read them, let the entries that share a column agree on one (the
-  // slot holds the number of the last writer), then put -inf.  The first CTA gets a copy of all of them.
-  Entry* first_list = cluster.map_shared_rank(list, 0);
-  for (int i = tid; i < p.k; i += blockDim.x) {
-    const int c = list[i].col;
-    if (c >= 0 && s.holds(c)) {
-      const float v = to_f32(s.sm[c - s.first]);
-      list[i].z = v;
-      if (rank != 0) first_list[i].z = v;
-    }
-  }
-  if (tid == 0 && target >= 0 && s.holds(static_cast<int>(target)))
-    cluster.map_shared_rank(&sh, 0)->target_logit = to_f32(s.sm[target - s.first]);
+  float mx = warp_max(rows::max_while_loading(s));
+  if (lane == 0) sh.red_max[warp] = mx;
   __syncthreads();
+  if (parts > 1) cluster.barrier_arrive();  // this CTA runs: its shared memory may be written
+  mx = warp_max(lane < warps ? sh.red_max[lane] : -CUDART_INF_F);
+  float ref = isfinite(mx) ? mx : 0.f;
+
+  // Take the listed logits out of the slice.  Entries that share a column agree on one: the slot holds the number
+  // of its last writer until that one puts -inf there (no number has -inf's bits).
   for (int i = tid; i < p.k; i += blockDim.x)
     if (list[i].col >= 0 && s.holds(list[i].col)) put_mark(s.sm + (list[i].col - s.first), i);
   __syncthreads();
-  bool shared_column = false;
-  bool target_listed = false;
   for (int i = tid; i < p.k; i += blockDim.x) {
     const int c = list[i].col;
+    bool owner = false;
     if (c >= 0 && s.holds(c)) {
-      list[i].owner = get_mark(s.sm + (c - s.first)) == i;
-      shared_column |= !list[i].owner;
+      owner = get_mark(s.sm + (c - s.first)) == i;
+      if (!owner) sh.repeats = 1;
+      if (owner) s.sm[c - s.first] = rows::neg_inf<TZ>();
     }
-    target_listed |= c >= 0 && c == target;
-  }
-  const bool repeats = __syncthreads_or(shared_column);
-  target_listed = __syncthreads_or(target_listed);
-  float list_max = -CUDART_INF_F;
-  int listed = 0;
-  for (int i = tid; i < p.k; i += blockDim.x) {
-    if (list[i].owner) {
-      s.sm[list[i].col - s.first] = rows::neg_inf<TZ>();
-      list_max = fmaxf(list_max, list[i].z);
-      ++listed;
-    }
+    list[i].owner = owner;
+    if (owner && p.k >= p.vocab) atomicAdd(&sh.listed, 1);  // only such a list can name every column
   }
   __syncthreads();
+  if (parts > 1) cluster.barrier_wait();
 
-  // the slice's maxima and sums
-  float mx[2] = {-CUDART_INF_F, list_max};
-  for (int v = tid; v < s.nv; v += blockDim.x) {
-    float e[E];
-    load_vec<E>(s.sm + v * E, e);
+  // sums over the slice and its listed columns, relative to the slice's largest logit
+  const float2 c2 = rows::both(p.inv_tau * CUDART_L2E_F), l2 = rows::both(CUDART_L2E_F);
+  {
+    const float2 r2 = rows::both(-ref);
+    float2 acc[2] = {rows::both(0.f), rows::both(0.f)}, acc1[2] = {rows::both(0.f), rows::both(0.f)};
+    for (int v = tid; v < s.nv; v += blockDim.x) {
+      float2 q[E / 2];
+      rows::load_pairs(s, v, q);
 #pragma unroll
-    for (int i = 0; i < E; ++i) mx[0] = fmaxf(mx[0], e[i]);
-  }
-  block_reduce_max(mx, sh.red);
-  const float c2 = p.inv_tau * CUDART_L2E_F;
-  float ref = isfinite(mx[0]) ? mx[0] : 0.f;
-  const float list_ref = isfinite(mx[1]) ? mx[1] : 0.f;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int v = tid; v < s.nv; v += blockDim.x) {
-    float e[E];
-    load_vec<E>(s.sm + v * E, e);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float x = e[i] - ref;
-      sum[0] += rows::fast_exp2(x * c2);
-      if (TWO) sum[1] += rows::fast_exp2(x * CUDART_L2E_F);
-    }
-  }
-  for (int i = tid; i < p.k; i += blockDim.x) {
-    if (list[i].owner) {
-      const float x = list[i].z - list_ref;
-      sum[2] += expf(x * p.inv_tau);
-      if (TWO) sum[3] += expf(x);
-    }
-  }
-  block_reduce_sum(sum, sh.red);
-  int owned = 0;  // only a list as long as the row can name every column
-  if (p.k >= p.vocab) {
-    float n[1] = {static_cast<float>(listed)};
-    block_reduce_sum(n, sh.red);
-    owned = static_cast<int>(n[0]);
-  }
-  if (tid < parts) {
-    Part* q = &cluster.map_shared_rank(&sh, tid)->part[rank];
-    *q = Part{mx[0], sum[0], sum[1], mx[1], sum[2], sum[3], owned};
-  }
-  if (parts > 1)
-    cluster.sync();
-  else
-    __syncthreads();
-
-  if (warp == 0) {
-    // every CTA combines the parts in the same order
-    float rest_max = -CUDART_INF_F, lmax = -CUDART_INF_F;
-    int all_listed = 0;
-    for (int c = 0; c < parts; ++c) {
-      rest_max = fmaxf(rest_max, sh.part[c].rest_max);
-      lmax = fmaxf(lmax, sh.part[c].list_max);
-      all_listed += sh.part[c].listed;
-    }
-    const float row_ref = isfinite(rest_max) ? rest_max : 0.f;
-    const float lref = isfinite(lmax) ? lmax : 0.f;
-    float S = 0.f, S1 = 0.f, L = 0.f, L1 = 0.f;
-    for (int c = 0; c < parts; ++c) {
-      const Part& q = sh.part[c];
-      const float dr = (isfinite(q.rest_max) ? q.rest_max : 0.f) - row_ref;
-      const float dl = (isfinite(q.list_max) ? q.list_max : 0.f) - lref;
-      if (q.rest_sum != 0.f) S += q.rest_sum * expf(dr * p.inv_tau);
-      if (q.list_sum != 0.f) L += q.list_sum * expf(dl * p.inv_tau);
-      if (TWO) {
-        if (q.rest_sum1 != 0.f) S1 += q.rest_sum1 * expf(dr);
-        if (q.list_sum1 != 0.f) L1 += q.list_sum1 * expf(dl);
+      for (int i = 0; i < E / 2; ++i) {
+        const float2 d = rows::add2(q[i], r2);
+        const float2 x = rows::mul2(d, c2);
+        const float2 e = make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
+        acc[i & 1] = rows::add2(acc[i & 1], e);
+        if constexpr (POW == 2) acc1[i & 1] = rows::fma2(e, e, acc1[i & 1]);
+        if constexpr (POW == 1 || POW == 4) acc1[i & 1] = rows::add2(acc1[i & 1], at_one<POW>(e, rows::mul2(d, l2)));
       }
     }
-    // The row's sums relative to its largest logit: probabilities come from these, not from a log-sum-exp,
-    // whose rounding (half an ulp of a number around 10) would enter every one of them.
-    const float hi = fmaxf(rest_max, lmax);
-    const float top = isfinite(hi) ? hi : 0.f;
-    const float fr = S != 0.f ? expf((row_ref - top) * p.inv_tau) : 0.f;
-    const float total = S * fr + (L != 0.f ? L * expf((lref - top) * p.inv_tau) : 0.f);
-    float fr1 = fr, total1 = total;
-    if (TWO) {
-      fr1 = S1 != 0.f ? expf(row_ref - top) : 0.f;
-      total1 = S1 * fr1 + (L1 != 0.f ? L1 * expf(lref - top) : 0.f);
+    float sum[4] = {(acc[0].x + acc[0].y) + (acc[1].x + acc[1].y), (acc1[0].x + acc1[0].y) + (acc1[1].x + acc1[1].y),
+                    0.f, 0.f};
+    for (int i = tid; i < p.k; i += blockDim.x) {
+      if (list[i].owner) {
+        const float x = list[i].z - ref;
+        sum[2] += expf(x * p.inv_tau);
+        if (POW != 0) sum[3] += expf(x);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (POW == 0 && (i & 1)) continue;
+      sum[i] = warp_sum(sum[i]);
+      if (lane == 0) sh.red[warp][i] = sum[i];
+    }
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (POW != 0 || !(i & 1)) sum[i] = warp_sum(lane < warps ? sh.red[lane][i] : 0.f);
+      if (lane < parts) {
+        Part* to = &(parts > 1 ? cluster.map_shared_rank(&sh, lane) : &sh)->part[rank];
+        *to = Part{ref, sum[0], sum[1], sum[2], sum[3], sh.listed};
+      }
+      __syncwarp();
+    }
+  }
+  if (parts > 1) cluster.sync();
+
+  // The row's scalars, by the first warp of every CTA, the parts in the same order.
+  float top = 0.f, S = 0.f, total = 0.f, total1 = 0.f, m = 0.f;
+  // With the rest's sum S relative to `at` and the logarithm of its probability: what the gradient needs, and the loss.
+  auto finish = [&](float at, float rest_sum, float log_rest) {
     const float scale = p.scale != nullptr ? *p.scale : 1.f;
-    // a list that names every column leaves no rest, whatever rounding says
-    const float m = p.k >= p.vocab && all_listed >= p.vocab ? 0.f : sh.rest;
     const float mass = sh.mass + m;
+    const float f = at == top ? 1.f : expf((at - top) * p.inv_tau), f1 = at == top ? 1.f : expf(at - top);
     if (lane == 0) {
-      sh.ref = row_ref;
+      float A = mass != 0.f ? mass * f / total : 0.f;
+      if (m > 0.f && rest_sum > 0.f) A -= m / rest_sum;
+      A *= scale * p.kd * p.tau;
+      float B = p.ce != 0.f ? scale * p.ce * f1 / total1 : 0.f;
+      if (POW == 0) {  // one exponential serves both terms
+        A += B;
+        B = 0.f;
+      }
+      sh.ref = at;
+      sh.A = A;
+      sh.B = B;
       sh.top = top;
       sh.inv_sum = 1.f / total;
       sh.inv_sum1 = 1.f / total1;
       sh.all_mass = mass;
-      float A = mass != 0.f ? mass * fr / total : 0.f;
-      if (m > 0.f && S > 0.f) A -= m / S;
-      A *= scale * p.kd * p.tau;
-      float B = p.ce != 0.f ? scale * p.ce * fr1 / total1 : 0.f;
-      if (!TWO) {
-        A += B;
-        B = 0.f;
-      }
-      sh.A = A;
-      sh.B = B;
     }
     if (rank == 0) {
+      const float log_total = logf(total);
       float kl = 0.f;
       for (int i = lane; i < p.k; i += 32) {
-        const float logq = (list[i].z - top) * p.inv_tau - logf(total);
+        const float logq = (list[i].z - top) * p.inv_tau - log_total;
         if (list[i].p != 0.f) kl += list[i].p * (list[i].logp - logq);
       }
       kl = warp_sum(kl);
       if (lane == 0) {
-        if (m > 0.f)  // log q_rest from its parts where the probability itself leaves fp32's range
-          kl += m * (fr > 1e-30f ? logf(m / (S * fr / total))
-                                 : logf(m) - (logf(S) + (row_ref - top) * p.inv_tau - logf(total)));
+        if (m > 0.f) kl += m * (logf(m) - log_rest);
         float loss = p.kd != 0.f ? p.kd * p.tau * p.tau * kl : 0.f;
         if (p.ce != 0.f) loss += p.ce * (logf(total1) - (sh.target_logit - top));
         p.loss[row] = scale * loss;
       }
     }
+  };
+  if (warp == 0) {
+    top = -CUDART_INF_F;
+    int all_listed = 0;
+    for (int c = 0; c < parts; ++c) {
+      const Part& q = sh.part[c];
+      if (q.rest != 0.f || q.list != 0.f) top = fmaxf(top, q.ref);
+      all_listed += q.listed;
+    }
+    if (top == -CUDART_INF_F) top = 0.f;
+    float L = 0.f, S1 = 0.f, L1 = 0.f;
+    for (int c = 0; c < parts; ++c) {
+      const Part& q = sh.part[c];
+      if (q.rest == 0.f && q.list == 0.f) continue;
+      const float f = expf((q.ref - top) * p.inv_tau);
+      S += q.rest * f;
+      L += q.list * f;
+      if (POW != 0) {
+        const float f1 = expf(q.ref - top);
+        S1 += q.rest1 * f1;
+        L1 += q.list1 * f1;
+      }
+    }
+    total = S + L;
+    total1 = POW != 0 ? S1 + L1 : total;
+    // a list that names every column leaves no rest, whatever rounding says
+    m = p.k >= p.vocab && all_listed >= p.vocab ? 0.f : sh.rest;
+    const bool again = m > 0.f && S < 1e-30f;
+    if (lane == 0) sh.again = again;
+    if (!again) finish(top, S, logf(S / total));
+  }
+  __syncthreads();
+  if (sh.again) {  // the same for the whole cluster: the rest's sum, relative to the rest's own largest logit
+    float rest_max = -CUDART_INF_F;
+    for (int v = tid; v < s.nv; v += blockDim.x) {
+      float e[E];
+      load_vec<E>(s.sm + v * E, e);
+#pragma unroll
+      for (int i = 0; i < E; ++i) rest_max = fmaxf(rest_max, e[i]);
+    }
+    rest_max = warp_max(rest_max);
+    if (lane == 0) sh.red_max[warp] = rest_max;
+    __syncthreads();
+    rest_max = warp_max(lane < warps ? sh.red_max[lane] : -CUDART_INF_F);
+    const float at = isfinite(rest_max) ? rest_max : 0.f;
+    float sum = 0.f;
+    for (int v = tid; v < s.nv; v += blockDim.x) {
+      float e[E];
+      load_vec<E>(s.sm + v * E, e);
+#pragma unroll
+      for (int i = 0; i < E; ++i) sum += rows::fast_exp2((e[i] - at) * c2.x);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) sh.red[warp][0] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      sum = warp_sum(lane < warps ? sh.red[lane][0] : 0.f);
+      if (lane < parts) {
+        Part* to = &(parts > 1 ? cluster.map_shared_rank(&sh, lane) : &sh)->again_part[rank];
+        *to = Part{at, sum, 0.f, 0.f, 0.f, 0};
+      }
+      __syncwarp();
+    }
+    if (parts > 1) cluster.sync();
+    if (warp == 0) {
+      float own_top = -CUDART_INF_F;
+      for (int c = 0; c < parts; ++c)
+        if (sh.again_part[c].rest != 0.f) own_top = fmaxf(own_top, sh.again_part[c].ref);
+      S = 0.f;
+      if (own_top == -CUDART_INF_F) own_top = top;  // nothing finite outside the list
+      for (int c = 0; c < parts; ++c)
+        if (sh.again_part[c].rest != 0.f)
+          S += sh.again_part[c].rest * expf((sh.again_part[c].ref - own_top) * p.inv_tau);
+      finish(own_top, S, logf(S) + (own_top - top) * p.inv_tau - logf(total));
+    }
+    __syncthreads();
   }
   if (!GRAD) return;
-  __syncthreads();
 
   // gradient of the slice, then of the listed columns and the target
-  ref = sh.ref;
   const float A = sh.A, B = sh.B;
   const bool same_vectors =
       sizeof(TG) == sizeof(TZ)
           ? (reinterpret_cast<uintptr_t>(drow) & 15) / sizeof(TG) == static_cast<uintptr_t>(s.off)
           : s.off == 0 && (reinterpret_cast<uintptr_t>(drow) & (E * sizeof(TG) - 1)) == 0;
+  const float2 r2 = rows::both(-sh.ref), A2 = rows::both(A), B2 = rows::both(B);
   for (int v = tid; v < s.nv; v += blockDim.x) {
-    float e[E];
-    load_vec<E>(s.sm + v * E, e);
-    const int col = s.first + v * E;
+    float2 q[E / 2];
+    rows::load_pairs(s, v, q);
+    float g[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float x = e[i] - ref;
-      e[i] = rows::fast_exp2(x * c2) * A;
-      if (TWO) e[i] += rows::fast_exp2(x * CUDART_L2E_F) * B;
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 d = rows::add2(q[i], r2);
+      const float2 x = rows::mul2(d, c2);
+      const float2 e = make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
+      float2 r;
+      if constexpr (POW == 0)
+        r = rows::mul2(e, A2);
+      else if constexpr (POW == 2)
+        r = rows::mul2(e, rows::fma2(e, B2, A2));
+      else
+        r = rows::fma2(at_one<POW>(e, rows::mul2(d, l2)), B2, rows::mul2(e, A2));
+      g[2 * i] = r.x;
+      g[2 * i + 1] = r.y;
     }
+    const int col = s.first + v * E;
     if (same_vectors && col >= 0 && col + E <= p.vocab) {
-      store_vec<E>(drow + col, e);
+      store_vec<E>(drow + col, g);
     } else {
 #pragma unroll
       for (int i = 0; i < E; ++i)
-        if (col + i >= 0 && col + i < p.vocab) drow[col + i] = from_f32<TG>(e[i]);
+        if (col + i >= 0 && col + i < p.vocab) drow[col + i] = from_f32<TG>(g[i]);
     }
   }
   if (rank == parts - 1)
@@ -379,19 +417,22 @@ __global__ void __launch_bounds__(512) distill_kernel(const TZ* __restrict__ z, 
     if (!list[i].owner) continue;
     const int c = list[i].col;
     float share = list[i].p;
-    if (repeats) {
+    if (sh.repeats) {
       share = 0.f;
       for (int j = 0; j < p.k; ++j)
         if (list[j].col == c) share += list[j].p;
     }
-    float g = kd != 0.f ? kd * (expf((list[i].z - sh.top) * p.inv_tau) * sh.inv_sum * sh.all_mass - share) : 0.f;
-    if (ce != 0.f) g += ce * (expf(list[i].z - sh.top) * sh.inv_sum1 - (c == target ? 1.f : 0.f));
+    const float d = list[i].z - sh.top;
+    float g = kd != 0.f ? kd * (expf(d * p.inv_tau) * sh.inv_sum * sh.all_mass - share) : 0.f;
+    if (ce != 0.f) g += ce * (expf(d) * sh.inv_sum1 - (c == target ? 1.f : 0.f));
     drow[c] = from_f32<TG>(g);
   }
-  if (tid == 0 && ce != 0.f && target >= 0 && !target_listed && s.holds(static_cast<int>(target))) {
-    const float x = to_f32(s.sm[target - s.first]) - ref;
-    float g = rows::fast_exp2(x * c2) * A - ce;
-    if (TWO) g += rows::fast_exp2(x * CUDART_L2E_F) * B;
+  if (tid == 0 && ce != 0.f && !sh.target_listed && s.holds(static_cast<int>(target))) {
+    const float2 d = rows::add2(rows::both(to_f32(s.sm[target - s.first])), r2);
+    const float2 x = rows::mul2(d, c2);
+    const float2 e = rows::both(rows::fast_exp2(x.x));
+    float g = e.x * A - ce;
+    if constexpr (POW != 0) g += at_one<POW>(e, rows::mul2(d, l2)).x * B;
     drow[target] = from_f32<TG>(g);
   }
 }
@@ -427,6 +468,7 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   p.vocab = a.vocab;
   p.k = a.k;
   p.per = plan.per;
+  p.parts = plan.parts;
   p.dz_cols = a.dz_cols;
   p.ids64 = a.ids64;
   p.inv_tau = 1.f / a.tau;
@@ -441,7 +483,7 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   p.ldz = a.ldz;
   p.lddz = a.lddz;
   p.status = a.status;
-  const bool two = a.ce != 0.f && a.tau != 1.f;
+  const int pow = a.ce == 0.f || a.tau == 1.f ? 0 : a.tau == 2.f ? 2 : a.tau == 4.f ? 4 : 1;
   const size_t smem = plan.slice_bytes + a.k * sizeof(Entry);
   auto launch = [&](auto kernel, auto* z, auto* t, auto* dz) {
     TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
@@ -455,7 +497,7 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
     attr[0].val.clusterDim.x = plan.parts;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = plan.parts > 1 ? 1 : 0;
     TTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, z, t, dz, p));
   };
   with_type(a.z_type, [&](auto* tz) {
@@ -467,12 +509,19 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
         const auto* zp = static_cast<const TZ*>(a.z);
         const auto* tp = static_cast<const TT*>(a.t);
         auto* gp = static_cast<TG*>(a.dz);
-        if (gp == nullptr)
-          two ? launch(distill_kernel<TZ, TT, TG, false, true>, zp, tp, gp)
-              : launch(distill_kernel<TZ, TT, TG, false, false>, zp, tp, gp);
-        else
-          two ? launch(distill_kernel<TZ, TT, TG, true, true>, zp, tp, gp)
-              : launch(distill_kernel<TZ, TT, TG, true, false>, zp, tp, gp);
+        auto with_pow = [&](auto w) {
+          constexpr int POW = decltype(w)::value;
+          if (gp == nullptr)
+            launch(distill_kernel<TZ, TT, TG, false, POW>, zp, tp, gp);
+          else
+            launch(distill_kernel<TZ, TT, TG, true, POW>, zp, tp, gp);
+        };
+        switch (pow) {
+          case 0: return with_pow(std::integral_constant<int, 0>{});
+          case 1: return with_pow(std::integral_constant<int, 1>{});
+          case 2: return with_pow(std::integral_constant<int, 2>{});
+          default: return with_pow(std::integral_constant<int, 4>{});
+        }
       };
       if (a.dz != nullptr && a.dz_type != a.z_type)
         with_grad(static_cast<__nv_bfloat16*>(nullptr));

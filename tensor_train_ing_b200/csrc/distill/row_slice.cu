@@ -6,16 +6,23 @@
 namespace ttb {
 namespace rows {
 
+namespace {
+// Two slices of this size and their lists fit an SM: one row's copies run under the other's arithmetic.
+constexpr size_t kTargetSliceBytes = 104 * 1024;
+}  // namespace
+
 Plan plan_rows(long long rows, int cols, int elem_bytes) {
   const int E = 16 / elem_bytes;
   const int total = (cols + 2 * (E - 1)) / E;  // the most vectors a row can touch
+  auto slice = [&](int parts) { return static_cast<size_t>((total + parts - 1) / parts) * 16; };
   Plan p;
   p.parts = 1;
-  while (p.parts < kMaxParts && static_cast<size_t>((total + p.parts - 1) / p.parts) * 16 > 32 * 1024) p.parts *= 2;
-  while (p.parts < kMaxParts && rows * p.parts < num_sms() && total / p.parts > 256) p.parts *= 2;
+  while (p.parts < kMaxParts && slice(p.parts) > kTargetSliceBytes) p.parts *= 2;
+  while (p.parts < kMaxParts && rows * p.parts < num_sms() && total / p.parts > 512) p.parts *= 2;
   p.per = (total + p.parts - 1) / p.parts;
-  p.threads = 256;
-  p.slice_bytes = static_cast<size_t>(p.per) * 16;
+  p.slice_bytes = slice(p.parts);
+  p.threads = 128;
+  while (p.threads < kMaxThreads && p.per > p.threads * 4) p.threads *= 2;
   return p;
 }
 

@@ -1,13 +1,14 @@
 // A teacher's top logits: per row the k largest, their columns and the log-sum-exp, from one read of the row.
 //
-// The row sits in the shared memory of a cluster (row_slice.cuh).  Pass 1 takes every thread's maximum over
-// its elements.  The r-th largest of a CTA's thread maxima, r = ceil(k / parts), has at least r elements of
-// the slice at or above it, so the smallest of these over the CTAs has at least k elements of the row at or
-// above it: a lower bound for the k-th largest logit, and a close one while there are many more threads
-// than r.  Pass 2 sums the exponentials and collects the elements at or above the bound (k and a few more) in
-// the first CTA, which ranks them by counting.  Elements are ordered by (value, lower column first) as one
-// 64-bit key, so the result does not depend on the order of collection.  Rows with so many elements at
-// the bound that the list overflows (ties, rows almost all -inf) find the k-th largest key bit by bit.
+// The row sits in the shared memory of a cluster, usually of one CTA (row_slice.cuh).  As it arrives every thread takes the
+// maximum of its elements.  The r-th largest of a CTA's thread maxima, r = ceil(k / parts), has at least r
+// elements of the slice at or above it, so the smallest of these over the CTAs has at least k elements of the row
+// at or above it: a lower bound for the k-th largest logit, and a close one while there are many more
+// threads than r.  Only threads whose maximum reaches the bound can hold such elements: their vectors (about k
+// threads') are looked through once more, one vector per lane, and the elements found (k and a few more)
+// are ranked by counting in the first CTA.  Elements are ordered by (value, lower column first) as one
+// 64-bit key, so the result does not depend on the order of collection.  Rows with so many elements at the bound that
+// the list overflows (ties, rows almost all -inf), and rows with NaN, find the k-th largest key bit by bit.
 #include "../common/host.h"
 #include "distill_api.h"
 #include "row_slice.cuh"
@@ -18,7 +19,7 @@ namespace {
 using rows::Slice;
 namespace cg = cooperative_groups;
 
-constexpr int kCapacity = 1024;  // collected elements
+constexpr int kCapacity = 640;  // collected elements: about 1.7 times the largest k
 
 // Monotone whole number of a float: larger for larger values, -0 = +0, NaN above all.
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -41,33 +42,16 @@ constexpr int lowest_bit() {
 }
 
 struct Shared {
-  float max[rows::kMaxParts];
+  uint32_t maxima[rows::kMaxThreads];  // ordered() of the thread maxima
+  unsigned short hit[rows::kMaxThreads];
+  float warp_sums[rows::kMaxThreads / 32];
+  int red[rows::kMaxThreads / 32];
   uint32_t bound[rows::kMaxParts];
-  float sum[rows::kMaxParts];
+  float ref[rows::kMaxParts], sum[rows::kMaxParts];
   int count[2][rows::kMaxParts];
-  float red[32];
-  int redi[32];
-  int taken;
+  int hits, taken, nan;
 };
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = warp_max(v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = red[0];
-  for (int i = 1; i < blockDim.x / 32; ++i) t = fmaxf(t, red[i]);
-  __syncthreads();
-  return t;
-}
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = red[0];
-  for (int i = 1; i < blockDim.x / 32; ++i) t += red[i];
-  __syncthreads();
-  return t;
-}
 __device__ __forceinline__ int block_count(int v, int* red) {
   v = __reduce_add_sync(0xffffffffu, v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
@@ -78,108 +62,171 @@ __device__ __forceinline__ int block_count(int v, int* red) {
   return t;
 }
 
+// A value that at least r and, where the values allow it, few more than r of the block's thread maxima reach
+// (0 where fewer than r threads have elements).  One warp; the common leading bits are skipped.
 template <typename T>
-__global__ void __launch_bounds__(512) top_logits_kernel(const T* __restrict__ z, long long ldz, int vocab, int k,
-                                                         float inv_tau, T* __restrict__ values, int* __restrict__ ids,
-                                                         float* __restrict__ lse, int per) {
+__device__ __forceinline__ uint32_t find_bound(const uint32_t* maxima, int threads, int r) {
+  constexpr int kMost = rows::kMaxThreads / 32;
+  const int lane = threadIdx.x & 31, each = threads / 32;
+  uint32_t m[kMost];
+  uint32_t all = 0xFFFFFFFFu, any = 0u;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    m[i] = i < each ? maxima[i * 32 + lane] : 0u;
+    if (i < each) {
+      all &= m[i];
+      any |= m[i];
+    }
+  }
+  all = __reduce_and_sync(0xffffffffu, all);
+  any = __reduce_or_sync(0xffffffffu, any);
+  const uint32_t differ = all ^ any;
+  if (differ == 0 || r > threads) return r > threads ? 0u : all;
+  const int top = 31 - __clz(differ);
+  uint32_t bound = top == 31 ? 0u : all & ~((2u << top) - 1u);
+  for (int bit = top; bit >= lowest_bit<T>(); --bit) {
+    const uint32_t trial = bound | (1u << bit);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) c += m[i] >= trial;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= r) bound = trial;
+    if (c >= r && c <= r + r / 8) break;  // close enough: a higher bound would only shorten the list a little
+  }
+  return bound;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* __restrict__ z, long long ldz,
+                                                                      int vocab, int k, float inv_tau,
+                                                                      T* __restrict__ values, int* __restrict__ ids,
+                                                                      float* __restrict__ lse, int per, int parts) {
   constexpr int E = Slice<T>::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = cluster.num_blocks(), rank = cluster.block_rank();
+  const int rank = parts > 1 ? cluster.block_rank() : 0;
   const long long row = blockIdx.x / parts;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   auto* list = reinterpret_cast<unsigned long long*>(smem + static_cast<size_t>(per) * 16);  // in the first CTA
 
   const Slice<T> s = rows::start_load(reinterpret_cast<T*>(smem), z + row * ldz, vocab, rank, per);
-  if (tid == 0) sh.taken = 0;
-  rows::finish_load();
-  cluster.sync();  // every CTA of the row runs and has its list empty
+  if (tid == 0) sh.hits = sh.taken = sh.nan = 0;
 
-  // pass 1: thread maxima (NaN is left out: it enters the list in pass 2 whatever the bound is)
-  float mx = -CUDART_INF_F;
-  bool any = false;
-  for (int v = tid; v < s.nv; v += blockDim.x) {
-    float e[E];
-    load_vec<E>(s.sm + v * E, e);
-#pragma unroll
-    for (int i = 0; i < E; ++i) mx = fmaxf(mx, e[i]);
-    any = true;
-  }
-  const uint32_t mine = any ? ordered(mx) : 0u;
-  const int r = (k + parts - 1) / parts;
+  // Thread maxima.  NaN is left out here; it shows in the sum.
+  const float mx = rows::max_while_loading(s);
+  sh.maxima[tid] = tid < s.nv ? ordered(mx) : 0u;
+  __syncthreads();
+  if (parts > 1) cluster.barrier_arrive();  // this CTA runs and its counters are set
+  uint32_t top = 0;
+  for (int i = lane; i < blockDim.x; i += 32) top = max(top, sh.maxima[i]);
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float slice_max = top == 0u ? -CUDART_INF_F : from_ordered(top);
+  const float ref = isfinite(slice_max) ? slice_max : 0.f;
   uint32_t bound = 0;
-  for (int bit = 31; bit >= lowest_bit<T>(); --bit) {
-    const uint32_t trial = bound | (1u << bit);
-    const int c = __syncthreads_count(mine >= trial);
-    if (c >= r) bound = trial;
-    if (c >= r && c <= r + r / 4) break;  // close enough: a smaller bound only lengthens the list
+  if (warp == 0) {
+    bound = find_bound<T>(sh.maxima, blockDim.x, (k + parts - 1) / parts);
+    if (parts == 1 && lane == 0) sh.bound[0] = bound;
   }
-  const float top = block_max(mx, sh.red);
-  if (tid < parts) {
-    Shared* peer = cluster.map_shared_rank(&sh, tid);
-    peer->max[rank] = top;
-    peer->bound[rank] = bound;
-  }
-  cluster.sync();
-  float row_max = -CUDART_INF_F;
-  bound = 0xFFFFFFFFu;
-  for (int c = 0; c < parts; ++c) {
-    row_max = fmaxf(row_max, sh.max[c]);
-    bound = min(bound, sh.bound[c]);
-  }
-  const float ref = isfinite(row_max) ? row_max : 0.f;
-  const float least = bound <= ordered(-CUDART_INF_F) ? -CUDART_INF_F : from_ordered(bound);
+  if (parts > 1) cluster.barrier_wait();
+  if (warp == 0 && parts > 1 && lane < parts) cluster.map_shared_rank(&sh, lane)->bound[rank] = bound;
 
-  // pass 2: sum of exponentials; elements that are not below the bound
-  Shared* first = cluster.map_shared_rank(&sh, 0);
-  unsigned long long* first_list = cluster.map_shared_rank(list, 0);
-  const float c2 = inv_tau * CUDART_L2E_F;
-  float sum = 0.f;
-  int found = 0;
+  // sum of exponentials relative to the slice's maximum
+  const float2 c2 = rows::both(inv_tau * CUDART_L2E_F), r2 = rows::both(-ref);
+  float2 acc = rows::both(0.f), acc_b = rows::both(0.f);
   for (int v = tid; v < s.nv; v += blockDim.x) {
-    float e[E];
-    load_vec<E>(s.sm + v * E, e);
-    bool some = false;
+    float2 p[E / 2];
+    rows::load_pairs(s, v, p);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      sum += rows::fast_exp2((e[i] - ref) * c2);
-      some |= !(e[i] < least);
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 x = rows::mul2(rows::add2(p[i], r2), c2);
+      const float2 e = make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
+      if (i & 1)
+        acc_b = rows::add2(acc_b, e);
+      else
+        acc = rows::add2(acc, e);
     }
-    if (some) {
+  }
+  float sum = warp_sum((acc.x + acc.y) + (acc_b.x + acc_b.y));
+  if (lane == 0) sh.warp_sums[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    sum = warp_sum(lane < warps ? sh.warp_sums[lane] : 0.f);
+    if (lane < parts) {
+      Shared* peer = parts > 1 ? cluster.map_shared_rank(&sh, lane) : &sh;
+      peer->sum[rank] = sum;
+      peer->ref[rank] = ref;
+    }
+  }
+  if (parts > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  bound = 0xFFFFFFFFu;
+  float total_ref = 0.f, total_sum = 0.f;  // the row's, each CTA the same
+  for (int c = 0; c < parts; ++c) bound = min(bound, sh.bound[c]);
+  for (int c = 0; c < parts; ++c)
+    if (sh.sum[c] != 0.f && (total_sum == 0.f || sh.ref[c] > total_ref)) {
+      total_ref = sh.ref[c];
+      total_sum = 1.f;
+    }
+  total_sum = 0.f;
+  for (int c = 0; c < parts; ++c)
+    if (sh.sum[c] != 0.f) total_sum += sh.sum[c] * expf((sh.ref[c] - total_ref) * inv_tau);
+
+  // collect: threads that can hold elements at the bound, then their vectors
+  const float least = bound <= ordered(-CUDART_INF_F) ? -CUDART_INF_F : from_ordered(bound);
+  Shared* first = parts > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+  unsigned long long* first_list = parts > 1 ? cluster.map_shared_rank(list, 0) : list;
+  const bool has_nan = total_sum != total_sum;
+  int found = 0;
+  if (!has_nan) {
+    const bool hit = tid < s.nv && mx >= least;
+    const unsigned who = __ballot_sync(0xffffffffu, hit);
+    int at = 0;
+    if (lane == 0 && who != 0) at = atomicAdd(&sh.hits, __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0);
+    if (hit) sh.hit[at + __popc(who & ((1u << lane) - 1u))] = static_cast<unsigned short>(tid);
+    __syncthreads();
+    for (int h = warp; h < sh.hits; h += warps) {
+      for (int v = sh.hit[h] + lane * blockDim.x; v < s.nv; v += 32 * blockDim.x) {
+        float e[E];
+        load_vec<E>(s.sm + v * E, e);
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int col = s.first + v * E + i;
-        if (!(e[i] < least) && col >= 0 && col < vocab) {
-          ++found;
-          const int at = atomicAdd(&first->taken, 1);
-          if (at < kCapacity) first_list[at] = key_of(e[i], col);
+        for (int i = 0; i < E; ++i) {
+          const int col = s.first + v * E + i;
+          if (e[i] >= least && col >= 0 && col < vocab) {
+            ++found;
+            const int to = atomicAdd(&first->taken, 1);
+            if (to < kCapacity) first_list[to] = key_of(e[i], col);
+          }
         }
       }
     }
   }
-  sum = block_sum(sum, sh.red);
-  found = block_count(found, sh.redi);
-  if (tid < parts) {
-    Shared* peer = cluster.map_shared_rank(&sh, tid);
-    peer->sum[rank] = sum;
-    peer->count[0][rank] = found;
+  int total;
+  if (parts > 1) {
+    found = block_count(found, sh.red);
+    if (tid < parts) cluster.map_shared_rank(&sh, tid)->count[0][rank] = found;
+    cluster.sync();
+    total = 0;
+    for (int c = 0; c < parts; ++c) total += sh.count[0][c];
+  } else {
+    __syncthreads();
+    total = sh.taken;
   }
-  cluster.sync();
-  int total = 0;
-  for (int c = 0; c < parts; ++c) total += sh.count[0][c];
 
-  if (total > kCapacity) {
+  if (has_nan || total > kCapacity) {
     // the k-th largest key, highest bit first; the column's upper bits are ones in every key
     const int col_bits = 32 - __clz(vocab);
     unsigned long long kth = 0;
     int side = 1;
     for (int bit = 63; bit >= 0; --bit) {
+      const unsigned long long trial = kth | (1ull << bit);
       if (bit < 32 && bit >= col_bits) {
-        kth |= 1ull << bit;
+        kth = trial;
         continue;
       }
-      const unsigned long long trial = kth | (1ull << bit);
       int c = 0;
       for (int v = tid; v < s.nv; v += blockDim.x) {
         float e[E];
@@ -190,16 +237,21 @@ __global__ void __launch_bounds__(512) top_logits_kernel(const T* __restrict__ z
           c += col >= 0 && col < vocab && key_of(e[i], col) >= trial;
         }
       }
-      c = block_count(c, sh.redi);
-      if (tid < parts) cluster.map_shared_rank(&sh, tid)->count[side][rank] = c;
-      cluster.sync();
-      c = 0;
-      for (int q = 0; q < parts; ++q) c += sh.count[side][q];
-      side ^= 1;
+      c = block_count(c, sh.red);
+      if (parts > 1) {
+        if (tid < parts) cluster.map_shared_rank(&sh, tid)->count[side][rank] = c;
+        cluster.sync();
+        c = 0;
+        for (int q = 0; q < parts; ++q) c += sh.count[side][q];
+        side ^= 1;
+      }
       if (c >= k) kth = trial;
     }
     if (rank == 0 && tid == 0) sh.taken = 0;
-    cluster.sync();
+    if (parts > 1)
+      cluster.sync();
+    else
+      __syncthreads();
     for (int v = tid; v < s.nv; v += blockDim.x) {
       float e[E];
       load_vec<E>(s.sm + v * E, e);
@@ -207,12 +259,15 @@ __global__ void __launch_bounds__(512) top_logits_kernel(const T* __restrict__ z
       for (int i = 0; i < E; ++i) {
         const int col = s.first + v * E + i;
         if (col >= 0 && col < vocab && key_of(e[i], col) >= kth) {
-          const int at = atomicAdd(&first->taken, 1);
-          if (at < kCapacity) first_list[at] = key_of(e[i], col);
+          const int to = atomicAdd(&first->taken, 1);
+          if (to < kCapacity) first_list[to] = key_of(e[i], col);
         }
       }
     }
-    cluster.sync();
+    if (parts > 1)
+      cluster.sync();
+    else
+      __syncthreads();
     total = k;
   }
   if (rank != 0) return;
@@ -226,11 +281,7 @@ __global__ void __launch_bounds__(512) top_logits_kernel(const T* __restrict__ z
       ids[row * k + place] = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key));
     }
   }
-  if (tid == 0) {
-    float t = 0.f;
-    for (int c = 0; c < parts; ++c) t += sh.sum[c];
-    lse[row] = ref * inv_tau + logf(t);
-  }
+  if (tid == 0) lse[row] = total_ref * inv_tau + logf(total_sum);
 }
 
 }  // namespace
@@ -239,7 +290,8 @@ void top_logits(const TopLogitsArgs& a, cudaStream_t stream) {
   TTB_CHECK(a.k >= 1 && a.k <= kTopLogitsMaxK && a.k <= a.vocab, "top logits: k must be between 1 and min(256, columns)");
   TTB_CHECK(logits_row_fits(a.vocab, a.type), "top logits: the rows are too long");
   if (a.rows == 0) return;
-  const rows::Plan p = rows::plan_rows(a.rows, a.vocab, scalar_bytes(a.type));
+  rows::Plan p = rows::plan_rows(a.rows, a.vocab, scalar_bytes(a.type));
+  while (p.threads < rows::kMaxThreads && p.threads < 4 * ((a.k + p.parts - 1) / p.parts)) p.threads *= 2;
   TTB_CHECK(a.rows * p.parts <= 0x7FFFFFFFLL, "top logits: too many rows");
   const size_t smem = p.slice_bytes + kCapacity * sizeof(unsigned long long);
   with_type(a.type, [&](auto* tz) {
@@ -256,9 +308,9 @@ void top_logits(const TopLogitsArgs& a, cudaStream_t stream) {
     attr[0].val.clusterDim.x = p.parts;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = p.parts > 1 ? 1 : 0;
     TTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(a.z), a.ldz, a.vocab, a.k, a.inv_tau,
-                                      static_cast<T*>(a.values), a.ids, a.lse, p.per));
+                                      static_cast<T*>(a.values), a.ids, a.lse, p.per, p.parts));
   });
 }
 
