@@ -27,21 +27,23 @@ namespace {
 using rows::Slice;
 namespace cg = cooperative_groups;
 
-struct Part {  // what one CTA knows of its slice; sums are relative to ref
-  float ref;
+struct Part {  // what one CTA knows of its slice; sums are relative to its references at tau and at 1
+  rows::Ref ref, ref1;
   float rest, rest1;  // unlisted columns, at tau and at 1
   float list, list1;  // listed columns (each counted once)
   int listed;
 };
 
 struct Shared {
+  uint64_t bars[rows::kStages];
   Part part[rows::kMaxParts], again_part[rows::kMaxParts];
   float red[rows::kMaxThreads / 32][4];
   float red_max[rows::kMaxThreads / 32];
   float target_logit;
   float mass, rest;  // P and m
-  // the row's scalars for the gradient: q_j = exp((z_j - top) / tau) inv_sum, the passes over the slice use ref
-  float ref, A, B, top, inv_sum, inv_sum1, all_mass;
+  // the row's scalars for the gradient: q_j = 2^(z_j c - top) inv_sum; the passes over the slice use ref
+  rows::Ref ref, ref1, top, top1;
+  float A, B, inv_sum, inv_sum1, all_mass;
   int again, repeats, target_listed, listed;
 };
 
@@ -89,15 +91,25 @@ __device__ __forceinline__ void zero_row(T* row, int cols, int first, int step) 
   for (int i = head + vecs * E + first; i < cols; i += step) row[i] = from_f32<T>(0.f);
 }
 
+// The reference at temperature 1 that goes with `ref` at tau: with e^POW for the exponentials, exactly POW times it.
 template <int POW>
-__device__ __forceinline__ float2 at_one(float2 e, float2 x) {  // exp(z - R) from e and x = (z - R) log2(e) / tau
+__device__ __forceinline__ rows::Ref ref_at_one(const rows::Ref& ref) {
+  if constexpr (POW == 1) return rows::Ref(ref.z, CUDART_L2E_F);
+  rows::Ref r = ref;
+  if constexpr (POW > 1) r.r = POW * ref.r;
+  return r;
+}
+// exp(z - reference) of a pair of logits, from e = exp((z - reference) / tau) where POW says so.
+template <int POW, bool FAR>
+__device__ __forceinline__ float2 at_one(float2 e, float2 z, const rows::Ref& ref1) {
   if constexpr (POW == 2) {
     return rows::mul2(e, e);
   } else if constexpr (POW == 4) {
     const float2 sq = rows::mul2(e, e);
     return rows::mul2(sq, sq);
   } else {
-    return make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
+    return rows::exp2_pair(
+        rows::log2_pair<FAR>(z, rows::both(CUDART_L2E_F), rows::both(FAR ? -ref1.z : -ref1.r)));
   }
 }
 
@@ -127,7 +139,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     }
   }
 
-  const Slice<TZ> s = rows::start_load(reinterpret_cast<TZ*>(smem), zrow, p.vocab, rank, p.per);
+  const Slice<TZ> s = rows::start_load(reinterpret_cast<TZ*>(smem), sh.bars, zrow, p.vocab, rank, p.per);
   if (warp == 0) {
     // The teacher's list and the student's logits at it, by every CTA for itself.
     float top = -CUDART_INF_F;
@@ -182,12 +194,13 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
       sh.again = sh.repeats = sh.listed = 0;
     }
   }
-  float mx = warp_max(rows::max_while_loading(s));
+  float mx = warp_max(rows::max_while_loading(s, sh.bars, p.status));
   if (lane == 0) sh.red_max[warp] = mx;
   __syncthreads();
   if (parts > 1) cluster.barrier_arrive();  // this CTA runs: its shared memory may be written
   mx = warp_max(lane < warps ? sh.red_max[lane] : -CUDART_INF_F);
-  float ref = isfinite(mx) ? mx : 0.f;
+  const float c = p.inv_tau * CUDART_L2E_F, c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
+  const rows::Ref ref(mx, c), ref1 = ref_at_one<POW>(ref);
 
   // Take the listed logits out of the slice.  Entries that share a column agree on one: the slot holds the number
   // of its last writer until that one puts -inf there (no number has -inf's bits).
@@ -195,12 +208,12 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     if (list[i].col >= 0 && s.holds(list[i].col)) put_mark(s.sm + (list[i].col - s.first), i);
   __syncthreads();
   for (int i = tid; i < p.k; i += blockDim.x) {
-    const int c = list[i].col;
+    const int col = list[i].col;
     bool owner = false;
-    if (c >= 0 && s.holds(c)) {
-      owner = get_mark(s.sm + (c - s.first)) == i;
+    if (col >= 0 && s.holds(col)) {
+      owner = get_mark(s.sm + (col - s.first)) == i;
       if (!owner) sh.repeats = 1;
-      if (owner) s.sm[c - s.first] = rows::neg_inf<TZ>();
+      if (owner) s.sm[col - s.first] = rows::neg_inf<TZ>();
     }
     list[i].owner = owner;
     if (owner && p.k >= p.vocab) atomicAdd(&sh.listed, 1);  // only such a list can name every column
@@ -209,30 +222,30 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   if (parts > 1) cluster.barrier_wait();
 
   // sums over the slice and its listed columns, relative to the slice's largest logit
-  const float2 c2 = rows::both(p.inv_tau * CUDART_L2E_F), l2 = rows::both(CUDART_L2E_F);
   {
-    const float2 r2 = rows::both(-ref);
     float2 acc[2] = {rows::both(0.f), rows::both(0.f)}, acc1[2] = {rows::both(0.f), rows::both(0.f)};
-    for (int v = tid; v < s.nv; v += blockDim.x) {
-      float2 q[E / 2];
-      rows::load_pairs(s, v, q);
+    rows::by_kind(ref, [&](auto far) {
+      constexpr bool FAR = decltype(far)::value;
+      const float2 c2 = rows::both(c), n2 = rows::both(FAR ? -ref.z : -ref.r);
+      rows::for_vectors(s, [&](int v) {
+        float2 q[E / 2];
+        rows::load_pairs(s, v, q);
 #pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const float2 d = rows::add2(q[i], r2);
-        const float2 x = rows::mul2(d, c2);
-        const float2 e = make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
-        acc[i & 1] = rows::add2(acc[i & 1], e);
-        if constexpr (POW == 2) acc1[i & 1] = rows::fma2(e, e, acc1[i & 1]);
-        if constexpr (POW == 1 || POW == 4) acc1[i & 1] = rows::add2(acc1[i & 1], at_one<POW>(e, rows::mul2(d, l2)));
-      }
-    }
+        for (int i = 0; i < E / 2; ++i) {
+          const float2 e = rows::exp2_pair(rows::log2_pair<FAR>(q[i], c2, n2));
+          acc[i & 1] = rows::add2(acc[i & 1], e);
+          if constexpr (POW == 2) acc1[i & 1] = rows::fma2(e, e, acc1[i & 1]);
+          if constexpr (POW == 1 || POW == 4)
+            acc1[i & 1] = rows::add2(acc1[i & 1], at_one<POW, FAR>(e, q[i], ref1));
+        }
+      });
+    });
     float sum[4] = {(acc[0].x + acc[0].y) + (acc[1].x + acc[1].y), (acc1[0].x + acc1[0].y) + (acc1[1].x + acc1[1].y),
                     0.f, 0.f};
     for (int i = tid; i < p.k; i += blockDim.x) {
       if (list[i].owner) {
-        const float x = list[i].z - ref;
-        sum[2] += expf(x * p.inv_tau);
-        if (POW != 0) sum[3] += expf(x);
+        sum[2] += exp2f(ref.log2_of(list[i].z, c));
+        if (POW != 0) sum[3] += exp2f(ref1.log2_of(list[i].z, c1));
       }
     }
 #pragma unroll
@@ -248,7 +261,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
         if (POW != 0 || !(i & 1)) sum[i] = warp_sum(lane < warps ? sh.red[lane][i] : 0.f);
       if (lane < parts) {
         Part* to = &(parts > 1 ? cluster.map_shared_rank(&sh, lane) : &sh)->part[rank];
-        *to = Part{ref, sum[0], sum[1], sum[2], sum[3], sh.listed};
+        *to = Part{ref, ref1, sum[0], sum[1], sum[2], sum[3], sh.listed};
       }
       __syncwarp();
     }
@@ -256,65 +269,70 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   if (parts > 1) cluster.sync();
 
   // The row's scalars, by the first warp of every CTA, the parts in the same order.
-  float top = 0.f, S = 0.f, total = 0.f, total1 = 0.f, m = 0.f;
-  // With the rest's sum S relative to `at` and the logarithm of its probability: what the gradient needs, and the loss.
-  auto finish = [&](float at, float rest_sum, float log_rest) {
+  rows::Ref top(0.f, c), top1 = ref_at_one<POW>(top);
+  float S = 0.f, total = 0.f, total1 = 0.f, m = 0.f;
+  // What the gradient needs, and the loss, from the rest's sum relative to `at` and the logarithm of the rest's probability.
+  auto finish = [&](const rows::Ref& at, float rest_sum, float log_rest) {
     const float scale = p.scale != nullptr ? *p.scale : 1.f;
     const float mass = sh.mass + m;
-    const float f = at == top ? 1.f : expf((at - top) * p.inv_tau), f1 = at == top ? 1.f : expf(at - top);
+    const rows::Ref at1 = ref_at_one<POW>(at);
     if (lane == 0) {
-      float A = mass != 0.f ? mass * f / total : 0.f;
+      float A = mass != 0.f ? mass * exp2f(top.log2_of(at, c)) / total : 0.f;
       if (m > 0.f && rest_sum > 0.f) A -= m / rest_sum;
       A *= scale * p.kd * p.tau;
-      float B = p.ce != 0.f ? scale * p.ce * f1 / total1 : 0.f;
+      float B = p.ce != 0.f ? scale * p.ce * exp2f(top1.log2_of(at1, c1)) / total1 : 0.f;
       if (POW == 0) {  // one exponential serves both terms
         A += B;
         B = 0.f;
       }
       sh.ref = at;
+      sh.ref1 = at1;
       sh.A = A;
       sh.B = B;
       sh.top = top;
+      sh.top1 = top1;
       sh.inv_sum = 1.f / total;
       sh.inv_sum1 = 1.f / total1;
       sh.all_mass = mass;
     }
     if (rank == 0) {
-      const float log_total = logf(total);
+      const float log2_total = log2f(total);
       float kl = 0.f;
       for (int i = lane; i < p.k; i += 32) {
-        const float logq = (list[i].z - top) * p.inv_tau - log_total;
+        const float logq = (top.log2_of(list[i].z, c) - log2_total) * CUDART_LN2_F;
         if (list[i].p != 0.f) kl += list[i].p * (list[i].logp - logq);
       }
       kl = warp_sum(kl);
       if (lane == 0) {
         if (m > 0.f) kl += m * (logf(m) - log_rest);
         float loss = p.kd != 0.f ? p.kd * p.tau * p.tau * kl : 0.f;
-        if (p.ce != 0.f) loss += p.ce * (logf(total1) - (sh.target_logit - top));
+        if (p.ce != 0.f) loss += p.ce * (log2f(total1) - top1.log2_of(sh.target_logit, c1)) * CUDART_LN2_F;
         p.loss[row] = scale * loss;
       }
     }
   };
   if (warp == 0) {
-    top = -CUDART_INF_F;
-    int all_listed = 0;
-    for (int c = 0; c < parts; ++c) {
-      const Part& q = sh.part[c];
-      if (q.rest != 0.f || q.list != 0.f) top = fmaxf(top, q.ref);
-      all_listed += q.listed;
+    int best = -1, all_listed = 0;
+    for (int q = 0; q < parts; ++q) {
+      const Part& w = sh.part[q];
+      if ((w.rest != 0.f || w.list != 0.f) && (best < 0 || w.ref.z > sh.part[best].ref.z)) best = q;
+      all_listed += w.listed;
     }
-    if (top == -CUDART_INF_F) top = 0.f;
+    if (best >= 0) {
+      top = sh.part[best].ref;
+      top1 = sh.part[best].ref1;
+    }
     float L = 0.f, S1 = 0.f, L1 = 0.f;
-    for (int c = 0; c < parts; ++c) {
-      const Part& q = sh.part[c];
-      if (q.rest == 0.f && q.list == 0.f) continue;
-      const float f = expf((q.ref - top) * p.inv_tau);
-      S += q.rest * f;
-      L += q.list * f;
+    for (int q = 0; q < parts; ++q) {
+      const Part& w = sh.part[q];
+      if (w.rest == 0.f && w.list == 0.f) continue;
+      const float f = q == best ? 1.f : exp2f(top.log2_of(w.ref, c));
+      S += w.rest * f;
+      L += w.list * f;
       if (POW != 0) {
-        const float f1 = expf(q.ref - top);
-        S1 += q.rest1 * f1;
-        L1 += q.list1 * f1;
+        const float f1 = q == best ? 1.f : exp2f(top1.log2_of(w.ref1, c1));
+        S1 += w.rest1 * f1;
+        L1 += w.list1 * f1;
       }
     }
     total = S + L;
@@ -338,13 +356,13 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     if (lane == 0) sh.red_max[warp] = rest_max;
     __syncthreads();
     rest_max = warp_max(lane < warps ? sh.red_max[lane] : -CUDART_INF_F);
-    const float at = isfinite(rest_max) ? rest_max : 0.f;
+    const rows::Ref at(rest_max, c);
     float sum = 0.f;
     for (int v = tid; v < s.nv; v += blockDim.x) {
       float e[E];
       load_vec<E>(s.sm + v * E, e);
 #pragma unroll
-      for (int i = 0; i < E; ++i) sum += rows::fast_exp2((e[i] - at) * c2.x);
+      for (int i = 0; i < E; ++i) sum += rows::fast_exp2(at.log2_of(e[i], c));
     }
     sum = warp_sum(sum);
     if (lane == 0) sh.red[warp][0] = sum;
@@ -353,21 +371,21 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
       sum = warp_sum(lane < warps ? sh.red[lane][0] : 0.f);
       if (lane < parts) {
         Part* to = &(parts > 1 ? cluster.map_shared_rank(&sh, lane) : &sh)->again_part[rank];
-        *to = Part{at, sum, 0.f, 0.f, 0.f, 0};
+        *to = Part{at, at, sum, 0.f, 0.f, 0.f, 0};
       }
       __syncwarp();
     }
     if (parts > 1) cluster.sync();
     if (warp == 0) {
-      float own_top = -CUDART_INF_F;
-      for (int c = 0; c < parts; ++c)
-        if (sh.again_part[c].rest != 0.f) own_top = fmaxf(own_top, sh.again_part[c].ref);
+      int best = -1;
+      for (int q = 0; q < parts; ++q)
+        if (sh.again_part[q].rest != 0.f && (best < 0 || sh.again_part[q].ref.z > sh.again_part[best].ref.z)) best = q;
+      const rows::Ref own = best >= 0 ? sh.again_part[best].ref : top;  // else nothing finite outside the list
       S = 0.f;
-      if (own_top == -CUDART_INF_F) own_top = top;  // nothing finite outside the list
-      for (int c = 0; c < parts; ++c)
-        if (sh.again_part[c].rest != 0.f)
-          S += sh.again_part[c].rest * expf((sh.again_part[c].ref - own_top) * p.inv_tau);
-      finish(own_top, S, logf(S) + (own_top - top) * p.inv_tau - logf(total));
+      for (int q = 0; q < parts; ++q)
+        if (sh.again_part[q].rest != 0.f) S += sh.again_part[q].rest * exp2f(own.log2_of(sh.again_part[q].ref, c));
+      // (natural units: c times the type's lowest value is no fp32 number)
+      finish(own, S, logf(S) + (own.z - top.z) * p.inv_tau - logf(total));
     }
     __syncthreads();
   }
@@ -379,60 +397,60 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
       sizeof(TG) == sizeof(TZ)
           ? (reinterpret_cast<uintptr_t>(drow) & 15) / sizeof(TG) == static_cast<uintptr_t>(s.off)
           : s.off == 0 && (reinterpret_cast<uintptr_t>(drow) & (E * sizeof(TG) - 1)) == 0;
-  const float2 r2 = rows::both(-sh.ref), A2 = rows::both(A), B2 = rows::both(B);
-  for (int v = tid; v < s.nv; v += blockDim.x) {
-    float2 q[E / 2];
-    rows::load_pairs(s, v, q);
-    float g[E];
+  const rows::Ref at = sh.ref, at1 = sh.ref1;
+  const float2 A2 = rows::both(A), B2 = rows::both(B);
+  rows::by_kind(at, [&](auto far) {
+    constexpr bool FAR = decltype(far)::value;
+    const float2 c2 = rows::both(c), n2 = rows::both(FAR ? -at.z : -at.r);
+    rows::for_vectors(s, [&](int v) {
+      float2 q[E / 2];
+      rows::load_pairs(s, v, q);
+      float g[E];
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const float2 d = rows::add2(q[i], r2);
-      const float2 x = rows::mul2(d, c2);
-      const float2 e = make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
-      float2 r;
-      if constexpr (POW == 0)
-        r = rows::mul2(e, A2);
-      else if constexpr (POW == 2)
-        r = rows::mul2(e, rows::fma2(e, B2, A2));
-      else
-        r = rows::fma2(at_one<POW>(e, rows::mul2(d, l2)), B2, rows::mul2(e, A2));
-      g[2 * i] = r.x;
-      g[2 * i + 1] = r.y;
-    }
-    const int col = s.first + v * E;
-    if (same_vectors && col >= 0 && col + E <= p.vocab) {
-      store_vec<E>(drow + col, g);
-    } else {
+      for (int i = 0; i < E / 2; ++i) {
+        const float2 e = rows::exp2_pair(rows::log2_pair<FAR>(q[i], c2, n2));
+        float2 r;
+        if constexpr (POW == 0)
+          r = rows::mul2(e, A2);
+        else if constexpr (POW == 2)
+          r = rows::mul2(e, rows::fma2(e, B2, A2));
+        else
+          r = rows::fma2(at_one<POW, FAR>(e, q[i], at1), B2, rows::mul2(e, A2));
+        g[2 * i] = r.x;
+        g[2 * i + 1] = r.y;
+      }
+      const int col = s.first + v * E;
+      if (same_vectors && col >= 0 && col + E <= p.vocab) {
+        store_vec<E>(drow + col, g);
+      } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (col + i >= 0 && col + i < p.vocab) drow[col + i] = from_f32<TG>(g[i]);
-    }
-  }
+        for (int i = 0; i < E; ++i)
+          if (col + i >= 0 && col + i < p.vocab) drow[col + i] = from_f32<TG>(g[i]);
+      }
+    });
+  });
   if (rank == parts - 1)
-    for (int c = p.vocab + tid; c < p.dz_cols; c += blockDim.x) drow[c] = from_f32<TG>(0.f);
+    for (int i = p.vocab + tid; i < p.dz_cols; i += blockDim.x) drow[i] = from_f32<TG>(0.f);
   __syncthreads();
   const float scale = p.scale != nullptr ? *p.scale : 1.f;
   const float kd = scale * p.kd * p.tau, ce = scale * p.ce;
   for (int i = tid; i < p.k; i += blockDim.x) {
     if (!list[i].owner) continue;
-    const int c = list[i].col;
+    const int col = list[i].col;
     float share = list[i].p;
     if (sh.repeats) {
       share = 0.f;
       for (int j = 0; j < p.k; ++j)
-        if (list[j].col == c) share += list[j].p;
+        if (list[j].col == col) share += list[j].p;
     }
-    const float d = list[i].z - sh.top;
-    float g = kd != 0.f ? kd * (expf(d * p.inv_tau) * sh.inv_sum * sh.all_mass - share) : 0.f;
-    if (ce != 0.f) g += ce * (expf(d) * sh.inv_sum1 - (c == target ? 1.f : 0.f));
-    drow[c] = from_f32<TG>(g);
+    float g = kd != 0.f ? kd * (exp2f(sh.top.log2_of(list[i].z, c)) * sh.inv_sum * sh.all_mass - share) : 0.f;
+    if (ce != 0.f) g += ce * (exp2f(sh.top1.log2_of(list[i].z, c1)) * sh.inv_sum1 - (col == target ? 1.f : 0.f));
+    drow[col] = from_f32<TG>(g);
   }
   if (tid == 0 && ce != 0.f && !sh.target_listed && s.holds(static_cast<int>(target))) {
-    const float2 d = rows::add2(rows::both(to_f32(s.sm[target - s.first])), r2);
-    const float2 x = rows::mul2(d, c2);
-    const float2 e = rows::both(rows::fast_exp2(x.x));
-    float g = e.x * A - ce;
-    if constexpr (POW != 0) g += at_one<POW>(e, rows::mul2(d, l2)).x * B;
+    const float v = to_f32(s.sm[target - s.first]);
+    float g = rows::fast_exp2(at.log2_of(v, c)) * A - ce;
+    if (POW != 0) g += rows::fast_exp2(at1.log2_of(v, c1)) * B;
     drow[target] = from_f32<TG>(g);
   }
 }

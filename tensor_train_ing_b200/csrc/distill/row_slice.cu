@@ -21,8 +21,11 @@ Plan plan_rows(long long rows, int cols, int elem_bytes) {
   while (p.parts < kMaxParts && rows * p.parts < num_sms() && total / p.parts > 512) p.parts *= 2;
   p.per = (total + p.parts - 1) / p.parts;
   p.slice_bytes = slice(p.parts);
+  // Many rows: about 8 to 16 vectors per thread, so that what every warp does once per row weighs little.  Few rows:
+  // more threads, for the latency of one row.
+  const int most = rows * p.parts < 2 * num_sms() ? 4 : 16;
   p.threads = 128;
-  while (p.threads < kMaxThreads && p.per > p.threads * 4) p.threads *= 2;
+  while (p.threads < kMaxThreads && p.per > p.threads * most) p.threads *= 2;
   return p;
 }
 

@@ -3,8 +3,8 @@
 // the row's first element, so that rows at any element offset are copied in aligned 16-byte pieces;
 // positions outside the row (before its first element, past its last) hold -inf.
 //
-// Thread t copies, and in every later pass works on, the vectors t, t + threads, ... of its slice: a pass
-// over the slice needs no block barrier after the copies, only the thread's own copies to have arrived.
+// The slice arrives in kStages bulk copies with a barrier each.  Thread t works, in every pass, on the vectors t, t +
+// threads, ... of the slice, and stage g holds a whole number of such rounds.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -18,7 +18,7 @@ namespace rows {
 
 namespace cg = cooperative_groups;
 
-constexpr int kStages = 4;  // groups of copies that can be waited for one after the other
+constexpr int kStages = 4;
 
 template <typename T>
 struct Slice {
@@ -27,19 +27,31 @@ struct Slice {
   int first;   // negative in slice 0 of a row that starts off a 16-byte boundary
   int nv;      // vectors in this slice
   int off;     // elements between the 16-byte boundary and the row's first element
-  int stage;   // vectors per stage and thread
+  int rounds;  // vectors that every thread has; the threads below nv - rounds * threads have one more
+  int stage;   // rounds per stage
 
   __device__ __forceinline__ bool holds(int col) const { return col >= first && col < first + nv * kVec; }
 };
+
+// f(v) for each of the thread's vectors.
+template <typename T, typename F>
+__device__ __forceinline__ void for_vectors(const Slice<T>& s, F&& f) {
+  int v = threadIdx.x;
+#pragma unroll 2
+  for (int i = 0; i < s.rounds; ++i, v += blockDim.x) f(v);
+  if (v < s.nv) f(v);
+}
 
 template <typename T>
 __device__ __forceinline__ T neg_inf() {
   return from_f32<T>(-CUDART_INF_F);
 }
 
-// Issues the asynchronous copies of this CTA's slice in kStages groups.
+// Starts the copies of this CTA's slice (all threads; ends with a block barrier).  The at most two vectors that reach
+// over the row's ends are read element by element by the threads that own them.
 template <typename T>
-__device__ __forceinline__ Slice<T> start_load(T* sm, const T* row, int cols, int rank, int per) {
+__device__ __forceinline__ Slice<T> start_load(T* sm, uint64_t (&bars)[kStages], const T* row, int cols, int rank,
+                                               int per) {
   constexpr int E = Slice<T>::kVec;
   Slice<T> s;
   s.sm = sm;
@@ -48,50 +60,71 @@ __device__ __forceinline__ Slice<T> start_load(T* sm, const T* row, int cols, in
   const int v0 = min(rank * per, total);
   s.nv = min(per, total - v0);
   s.first = v0 * E - s.off;
-  const int each = (s.nv + blockDim.x - 1) / blockDim.x;
-  s.stage = (each + kStages - 1) / kStages;
-  int v = threadIdx.x;
+  s.rounds = s.nv / static_cast<int>(blockDim.x);
+  s.stage = s.rounds / kStages + 1;
+  const int lo = s.first < 0 ? 1 : 0;                                // whole vectors: [lo, hi)
+  const int hi = s.first + s.nv * E > cols ? s.nv - 1 : s.nv;
+  if (threadIdx.x == 0) {
 #pragma unroll
-  for (int g = 0; g < kStages; ++g) {
-    for (int i = 0; i < s.stage && v < s.nv; ++i, v += blockDim.x) {
-      const int col = s.first + v * E;
-      if (col >= 0 && col + E <= cols) {
-        cp_async16(smem_u32(sm + v * E), row + col);
+    for (int g = 0; g < kStages; ++g) mbar_init(&bars[g], 1);
+    fence_mbar_init();
+#pragma unroll
+    for (int g = 0; g < kStages; ++g) {
+      const int a = max(lo, g * s.stage * static_cast<int>(blockDim.x));
+      const int b = min(hi, (g + 1) * s.stage * static_cast<int>(blockDim.x));
+      if (a < b) {
+        mbar_arrive_expect_tx(&bars[g], (b - a) * 16);
+        bulk_load(sm + a * E, row + s.first + a * E, (b - a) * 16, &bars[g]);
       } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) sm[v * E + e] = (col + e >= 0 && col + e < cols) ? row[col + e] : neg_inf<T>();
+        mbar_arrive(&bars[g]);
       }
     }
-    cp_async_commit();
   }
+  const int edges[2] = {lo == 1 ? 0 : -1, hi < s.nv && !(lo == 1 && s.nv == 1) ? s.nv - 1 : -1};
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int v = edges[q];
+    if (v >= 0 && v % static_cast<int>(blockDim.x) == threadIdx.x) {
+      const int col = s.first + v * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sm[v * E + e] = (col + e >= 0 && col + e < cols) ? row[col + e] : neg_inf<T>();
+    }
+  }
+  __syncthreads();
   return s;
 }
 
-// The largest element of the thread's vectors (NaN left out), taken as the copies arrive; all of
-// the thread's own copies have arrived when it returns.
+// Waits for stage g.  The wait is bounded; one that runs out is reported and waited for once more, so that the
+// copy does not outlive the CTA.
+__device__ __forceinline__ void wait_stage(uint64_t* bar, uint32_t* status) {
+  if (!mbar_wait(bar, 0, status, kErrTimeoutProducer)) mbar_wait(bar, 0, status, kErrTimeoutProducer);
+}
+
+// The largest element of the thread's vectors (NaN left out), taken as the stages arrive; the whole slice has
+// arrived when it returns.
 template <typename T>
-__device__ __forceinline__ float max_while_loading(const Slice<T>& s) {
+__device__ __forceinline__ float max_while_loading(const Slice<T>& s, uint64_t (&bars)[kStages], uint32_t* status) {
   constexpr int E = Slice<T>::kVec;
   float mx = -CUDART_INF_F;
   uint32_t packed = 0;  // two running maxima of a 16-bit type
   if constexpr (sizeof(T) == 2) packed = pack2<T>(mx, mx);
-  int v = threadIdx.x;
+  auto take = [&](int v) {
+    const uint4 u = *reinterpret_cast<const uint4*>(s.sm + v * E);
+    if constexpr (sizeof(T) == 4)
+      mx = fmaxf(fmaxf(mx, fmaxf(__uint_as_float(u.x), __uint_as_float(u.y))),
+                 fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    else
+      packed = max2<T>(max2<T>(packed, max2<T>(u.x, u.y)), max2<T>(u.z, u.w));
+  };
+  int v = threadIdx.x, done = 0;
 #pragma unroll
   for (int g = 0; g < kStages; ++g) {
-    if (g == 0) cp_async_wait<3>();
-    if (g == 1) cp_async_wait<2>();
-    if (g == 2) cp_async_wait<1>();
-    if (g == 3) cp_async_wait<0>();
-    for (int i = 0; i < s.stage && v < s.nv; ++i, v += blockDim.x) {
-      const uint4 u = *reinterpret_cast<const uint4*>(s.sm + v * E);
-      if constexpr (sizeof(T) == 4) {
-        mx = fmaxf(fmaxf(mx, fmaxf(__uint_as_float(u.x), __uint_as_float(u.y))),
-                   fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
-      } else {
-        packed = max2<T>(max2<T>(packed, max2<T>(u.x, u.y)), max2<T>(u.z, u.w));
-      }
-    }
+    wait_stage(&bars[g], status);
+    const int end = min(s.rounds, (g + 1) * s.stage);
+#pragma unroll 2
+    for (; done < end; ++done, v += blockDim.x) take(v);
   }
+  if (v < s.nv) take(v);
   if constexpr (sizeof(T) == 2) {
     float lo, hi;
     unpack2<T>(packed, lo, hi);
@@ -139,6 +172,43 @@ __device__ __forceinline__ void load_pairs(const Slice<T>& s, int v, float2 (&p)
     unpack2<T>(u.z, p[2].x, p[2].y);
     unpack2<T>(u.w, p[3].x, p[3].y);
   }
+}
+
+// Exponentials are taken as powers of two of z c - r, c = log2(e) / tau, in one fused multiply-add: r is the fp32
+// number nearest to (largest logit) c, and everything about a row is kept relative to 2^r, so r's rounding
+// cancels.  Where the largest logit is so large in size that the product could overflow (rows at the type's lowest value), z is
+// instead compared with the logit itself first.
+struct Ref {
+  float z, r;  // the reference logit and z c
+  bool far;    // |z c| is no ordinary number
+  __device__ __forceinline__ Ref() {}
+  __device__ __forceinline__ Ref(float zmax, float c) {
+    z = isfinite(zmax) ? zmax : 0.f;
+    far = !(fabsf(z * c) < 1e30f);
+    r = z * c;
+  }
+  // log2 of exp((v - reference) / tau)
+  __device__ __forceinline__ float log2_of(float v, float c) const { return far ? (v - z) * c : fmaf(v, c, -r); }
+  // ... of another reference, of the same row and so of the same kind or infinitely far below
+  __device__ __forceinline__ float log2_of(const Ref& o, float c) const {
+    return far || o.far ? (o.z - z) * c : o.r - r;
+  }
+};
+
+// The exponents of a pair; FAR: ref.far, n = -ref.z there, else -ref.r.
+template <bool FAR>
+__device__ __forceinline__ float2 log2_pair(float2 q, float2 c, float2 n) {
+  return FAR ? mul2(add2(q, n), c) : fma2(q, c, n);
+}
+__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
+
+// f(std::bool_constant<ref.far>): the passes are compiled for both kinds of row.
+template <typename F>
+__device__ __forceinline__ void by_kind(const Ref& ref, F&& f) {
+  if (ref.far)
+    f(std::true_type{});
+  else
+    f(std::false_type{});
 }
 
 // How rows are spread: `parts` CTAs per row (a cluster), `per` vectors each, `threads` threads each.

@@ -42,14 +42,17 @@ constexpr int lowest_bit() {
 }
 
 struct Shared {
+  uint64_t bars[rows::kStages];
   uint32_t maxima[rows::kMaxThreads];  // ordered() of the thread maxima
   unsigned short hit[rows::kMaxThreads];
+  uint32_t warp_max[rows::kMaxThreads / 32];
   float warp_sums[rows::kMaxThreads / 32];
   int red[rows::kMaxThreads / 32];
   uint32_t bound[rows::kMaxParts];
-  float ref[rows::kMaxParts], sum[rows::kMaxParts];
+  rows::Ref ref[rows::kMaxParts];
+  float sum[rows::kMaxParts];
   int count[2][rows::kMaxParts];
-  int hits, taken, nan;
+  int hits, taken;
 };
 
 __device__ __forceinline__ int block_count(int v, int* red) {
@@ -100,7 +103,8 @@ template <typename T>
 __global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* __restrict__ z, long long ldz,
                                                                       int vocab, int k, float inv_tau,
                                                                       T* __restrict__ values, int* __restrict__ ids,
-                                                                      float* __restrict__ lse, int per, int parts) {
+                                                                      float* __restrict__ lse, int per, int parts,
+                                                                      uint32_t* status) {
   constexpr int E = Slice<T>::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
@@ -110,44 +114,41 @@ __global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   auto* list = reinterpret_cast<unsigned long long*>(smem + static_cast<size_t>(per) * 16);  // in the first CTA
 
-  const Slice<T> s = rows::start_load(reinterpret_cast<T*>(smem), z + row * ldz, vocab, rank, per);
-  if (tid == 0) sh.hits = sh.taken = sh.nan = 0;
+  if (tid == 0) sh.hits = sh.taken = 0;
+  const Slice<T> s = rows::start_load(reinterpret_cast<T*>(smem), sh.bars, z + row * ldz, vocab, rank, per);
+  if (parts > 1) cluster.barrier_arrive();  // this CTA runs and its counters are set
 
   // Thread maxima.  NaN is left out here; it shows in the sum.
-  const float mx = rows::max_while_loading(s);
-  sh.maxima[tid] = tid < s.nv ? ordered(mx) : 0u;
+  const float mx = rows::max_while_loading(s, sh.bars, status);
+  const uint32_t mine = tid < s.nv ? ordered(mx) : 0u;
+  sh.maxima[tid] = mine;
+  uint32_t top = __reduce_max_sync(0xffffffffu, mine);
+  if (lane == 0) sh.warp_max[warp] = top;
   __syncthreads();
-  if (parts > 1) cluster.barrier_arrive();  // this CTA runs and its counters are set
-  uint32_t top = 0;
-  for (int i = lane; i < blockDim.x; i += 32) top = max(top, sh.maxima[i]);
-  top = __reduce_max_sync(0xffffffffu, top);
-  const float slice_max = top == 0u ? -CUDART_INF_F : from_ordered(top);
-  const float ref = isfinite(slice_max) ? slice_max : 0.f;
-  uint32_t bound = 0;
-  if (warp == 0) {
-    bound = find_bound<T>(sh.maxima, blockDim.x, (k + parts - 1) / parts);
-    if (parts == 1 && lane == 0) sh.bound[0] = bound;
-  }
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? sh.warp_max[lane] : 0u);
+  const float c = inv_tau * CUDART_L2E_F;
+  const rows::Ref ref(top == 0u ? -CUDART_INF_F : from_ordered(top), c);
   if (parts > 1) cluster.barrier_wait();
-  if (warp == 0 && parts > 1 && lane < parts) cluster.map_shared_rank(&sh, lane)->bound[rank] = bound;
+  if (warp == 0) {
+    const uint32_t bound = find_bound<T>(sh.maxima, blockDim.x, (k + parts - 1) / parts);
+    if (lane < parts) (parts > 1 ? cluster.map_shared_rank(&sh, lane) : &sh)->bound[rank] = bound;
+  }
 
   // sum of exponentials relative to the slice's maximum
-  const float2 c2 = rows::both(inv_tau * CUDART_L2E_F), r2 = rows::both(-ref);
-  float2 acc = rows::both(0.f), acc_b = rows::both(0.f);
-  for (int v = tid; v < s.nv; v += blockDim.x) {
-    float2 p[E / 2];
-    rows::load_pairs(s, v, p);
+  float2 acc[2] = {rows::both(0.f), rows::both(0.f)};
+  rows::by_kind(ref, [&](auto far) {
+    constexpr bool FAR = decltype(far)::value;
+    const float2 c2 = rows::both(c), n2 = rows::both(FAR ? -ref.z : -ref.r);
+    rows::for_vectors(s, [&](int v) {
+      float2 q[E / 2];
+      rows::load_pairs(s, v, q);
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const float2 x = rows::mul2(rows::add2(p[i], r2), c2);
-      const float2 e = make_float2(rows::fast_exp2(x.x), rows::fast_exp2(x.y));
-      if (i & 1)
-        acc_b = rows::add2(acc_b, e);
-      else
-        acc = rows::add2(acc, e);
-    }
-  }
-  float sum = warp_sum((acc.x + acc.y) + (acc_b.x + acc_b.y));
+      for (int i = 0; i < E / 2; ++i)
+        acc[i & 1] = rows::add2(acc[i & 1], rows::exp2_pair(rows::log2_pair<FAR>(q[i], c2, n2)));
+    });
+  });
+  acc[0] = rows::add2(acc[0], acc[1]);
+  float sum = warp_sum(acc[0].x + acc[0].y);
   if (lane == 0) sh.warp_sums[warp] = sum;
   __syncthreads();
   if (warp == 0) {
@@ -162,44 +163,61 @@ __global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* 
     cluster.sync();
   else
     __syncthreads();
-  bound = 0xFFFFFFFFu;
-  float total_ref = 0.f, total_sum = 0.f;  // the row's, each CTA the same
-  for (int c = 0; c < parts; ++c) bound = min(bound, sh.bound[c]);
-  for (int c = 0; c < parts; ++c)
-    if (sh.sum[c] != 0.f && (total_sum == 0.f || sh.ref[c] > total_ref)) {
-      total_ref = sh.ref[c];
-      total_sum = 1.f;
-    }
-  total_sum = 0.f;
-  for (int c = 0; c < parts; ++c)
-    if (sh.sum[c] != 0.f) total_sum += sh.sum[c] * expf((sh.ref[c] - total_ref) * inv_tau);
+  // the row's bound, reference and sum: every CTA computes the same
+  uint32_t bound = sh.bound[0];
+  int best = 0;
+  for (int q = 1; q < parts; ++q) {
+    bound = min(bound, sh.bound[q]);
+    if (sh.sum[q] != 0.f && (sh.sum[best] == 0.f || sh.ref[q].z > sh.ref[best].z)) best = q;
+  }
+  float total_sum = sh.sum[best];
+  for (int q = 0; q < parts; ++q)
+    if (q != best && sh.sum[q] != 0.f) total_sum += sh.sum[q] * exp2f(sh.ref[best].log2_of(sh.ref[q], c));
 
-  // collect: threads that can hold elements at the bound, then their vectors
-  const float least = bound <= ordered(-CUDART_INF_F) ? -CUDART_INF_F : from_ordered(bound);
+  // Collect: the threads that can hold elements at the bound, then their vectors, a vector per lane.  Without a
+  // bound (fewer vectors than r) a short row is taken whole.
+  const bool whole = bound <= ordered(-CUDART_INF_F);
+  const bool search = total_sum != total_sum || (whole && vocab > kCapacity);  // NaN, or no bound
   Shared* first = parts > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
   unsigned long long* first_list = parts > 1 ? cluster.map_shared_rank(list, 0) : list;
-  const bool has_nan = total_sum != total_sum;
+  const auto take = [&](float value, int col) {
+    const int to = atomicAdd(&first->taken, 1);
+    if (to < kCapacity) first_list[to] = key_of(value, col);
+  };
   int found = 0;
-  if (!has_nan) {
-    const bool hit = tid < s.nv && mx >= least;
+  if (!search && whole) {
+    for (int i = tid; i < s.nv * E; i += blockDim.x) {
+      const int col = s.first + i;
+      if (col >= 0 && col < vocab) {
+        ++found;
+        take(to_f32(s.sm[i]), col);
+      }
+    }
+  } else if (!search) {
+    const float least = from_ordered(bound);
+    const bool hit = mine >= bound;
     const unsigned who = __ballot_sync(0xffffffffu, hit);
     int at = 0;
     if (lane == 0 && who != 0) at = atomicAdd(&sh.hits, __popc(who));
     at = __shfl_sync(0xffffffffu, at, 0);
     if (hit) sh.hit[at + __popc(who & ((1u << lane) - 1u))] = static_cast<unsigned short>(tid);
     __syncthreads();
-    for (int h = warp; h < sh.hits; h += warps) {
-      for (int v = sh.hit[h] + lane * blockDim.x; v < s.nv; v += 32 * blockDim.x) {
-        float e[E];
-        load_vec<E>(s.sm + v * E, e);
+    // 16 lanes look through a thread's vectors (it has up to 16 unless a slice is very long)
+    const int hits = sh.hits, half = lane & 15;
+    for (int h = 2 * warp + (lane >> 4); h < hits; h += 2 * warps) {
+      for (int v = sh.hit[h] + half * blockDim.x; v < s.nv; v += 16 * blockDim.x) {
+        float2 q[E / 2];
+        rows::load_pairs(s, v, q);
+        unsigned mask = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int col = s.first + v * E + i;
-          if (e[i] >= least && col >= 0 && col < vocab) {
-            ++found;
-            const int to = atomicAdd(&first->taken, 1);
-            if (to < kCapacity) first_list[to] = key_of(e[i], col);
-          }
+        for (int i = 0; i < E / 2; ++i) {
+          mask |= (q[i].x >= least ? 1u : 0u) << (2 * i);
+          mask |= (q[i].y >= least ? 1u : 0u) << (2 * i + 1);
+        }
+        found += __popc(mask);
+        for (; mask != 0; mask &= mask - 1) {
+          const int i = v * E + __ffs(mask) - 1;
+          take(to_f32(s.sm[i]), s.first + i);
         }
       }
     }
@@ -210,13 +228,13 @@ __global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* 
     if (tid < parts) cluster.map_shared_rank(&sh, tid)->count[0][rank] = found;
     cluster.sync();
     total = 0;
-    for (int c = 0; c < parts; ++c) total += sh.count[0][c];
+    for (int q = 0; q < parts; ++q) total += sh.count[0][q];
   } else {
     __syncthreads();
     total = sh.taken;
   }
 
-  if (has_nan || total > kCapacity) {
+  if (search || total > kCapacity) {
     // the k-th largest key, highest bit first; the column's upper bits are ones in every key
     const int col_bits = 32 - __clz(vocab);
     unsigned long long kth = 0;
@@ -227,25 +245,25 @@ __global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* 
         kth = trial;
         continue;
       }
-      int c = 0;
+      int n = 0;
       for (int v = tid; v < s.nv; v += blockDim.x) {
         float e[E];
         load_vec<E>(s.sm + v * E, e);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           const int col = s.first + v * E + i;
-          c += col >= 0 && col < vocab && key_of(e[i], col) >= trial;
+          n += col >= 0 && col < vocab && key_of(e[i], col) >= trial;
         }
       }
-      c = block_count(c, sh.red);
+      n = block_count(n, sh.red);
       if (parts > 1) {
-        if (tid < parts) cluster.map_shared_rank(&sh, tid)->count[side][rank] = c;
+        if (tid < parts) cluster.map_shared_rank(&sh, tid)->count[side][rank] = n;
         cluster.sync();
-        c = 0;
-        for (int q = 0; q < parts; ++q) c += sh.count[side][q];
+        n = 0;
+        for (int q = 0; q < parts; ++q) n += sh.count[side][q];
         side ^= 1;
       }
-      if (c >= k) kth = trial;
+      if (n >= k) kth = trial;
     }
     if (rank == 0 && tid == 0) sh.taken = 0;
     if (parts > 1)
@@ -258,10 +276,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* 
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int col = s.first + v * E + i;
-        if (col >= 0 && col < vocab && key_of(e[i], col) >= kth) {
-          const int to = atomicAdd(&first->taken, 1);
-          if (to < kCapacity) first_list[to] = key_of(e[i], col);
-        }
+        if (col >= 0 && col < vocab && key_of(e[i], col) >= kth) take(e[i], col);
       }
     }
     if (parts > 1)
@@ -272,16 +287,22 @@ __global__ void __launch_bounds__(rows::kMaxThreads) top_logits_kernel(const T* 
   }
   if (rank != 0) return;
 
-  for (int i = tid; i < total; i += blockDim.x) {
-    const unsigned long long key = list[i];
+  // four lanes count the larger keys of each
+  for (int i = tid >> 2; i - (lane >> 2) < total; i += blockDim.x / 4) {
+    const unsigned long long key = list[min(i, total - 1)];
     int place = 0;
-    for (int j = 0; j < total; ++j) place += list[j] > key;
-    if (place < k) {
+    for (int j = tid & 3; j < total; j += 4) place += list[j] > key;
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    place += __shfl_xor_sync(0xffffffffu, place, 2);
+    if ((tid & 3) == 0 && i < total && place < k) {
       values[row * k + place] = from_f32<T>(from_ordered(static_cast<uint32_t>(key >> 32)));
       ids[row * k + place] = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key));
     }
   }
-  if (tid == 0) lse[row] = total_ref * inv_tau + logf(total_sum);
+  if (tid == 0) {
+    const rows::Ref r = sh.ref[best];
+    lse[row] = r.far ? r.z * inv_tau + logf(total_sum) : (r.r + log2f(total_sum)) * CUDART_LN2_F;
+  }
 }
 
 }  // namespace
@@ -310,7 +331,7 @@ void top_logits(const TopLogitsArgs& a, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = p.parts > 1 ? 1 : 0;
     TTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(a.z), a.ldz, a.vocab, a.k, a.inv_tau,
-                                      static_cast<T*>(a.values), a.ids, a.lse, p.per, p.parts));
+                                      static_cast<T*>(a.values), a.ids, a.lse, p.per, p.parts, status_ptr()));
   });
 }
 
