@@ -52,6 +52,8 @@ struct Params {
   bool ids64;
   float inv_tau, tau, kd, ce;
   const void* ids;
+  const void* t;
+  ScalarType t_type;
   const float* teacher_lse;
   const long long* targets;
   const float* scale;
@@ -59,6 +61,12 @@ struct Params {
   long long ldz, lddz;
   uint32_t* status;
 };
+
+__device__ __forceinline__ float teacher_logit(const Params& p, long long i) {
+  if (p.t_type == ScalarType::kF32) return static_cast<const float*>(p.t)[i];
+  if (p.t_type == ScalarType::kBF16) return to_f32(static_cast<const __nv_bfloat16*>(p.t)[i]);
+  return to_f32(static_cast<const __half*>(p.t)[i]);
+}
 
 // Entry i of the shared-memory copy of the teacher's list.
 struct Entry {
@@ -113,9 +121,9 @@ __device__ __forceinline__ float2 at_one(float2 e, float2 z, const rows::Ref& re
   }
 }
 
-template <typename TZ, typename TT, typename TG, bool GRAD, int POW>
+template <typename TZ, typename TG, bool GRAD, int POW>
 __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __restrict__ z,
-                                                                   const TT* __restrict__ t, TG* __restrict__ dz,
+                                                                   TG* __restrict__ dz,
                                                                    const __grid_constant__ Params p) {
   constexpr int E = Slice<TZ>::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -148,7 +156,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     for (int i = lane; i < p.k; i += 32) {
       long long c = p.ids64 ? static_cast<const long long*>(p.ids)[row * p.k + i]
                             : static_cast<const int*>(p.ids)[row * p.k + i];
-      const float raw = to_f32(t[row * p.k + i]) * p.inv_tau;
+      const float raw = teacher_logit(p, row * p.k + i) * p.inv_tau;
       if (c >= p.vocab) {
         if (rank == 0) record_error(p.status, kErrBadIndex);
         c = -1;
@@ -494,6 +502,8 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   p.kd = a.kd;
   p.ce = a.ce;
   p.ids = a.ids;
+  p.t = a.t;
+  p.t_type = a.t_type;
   p.teacher_lse = a.teacher_lse;
   p.targets = a.targets;
   p.scale = a.scale;
@@ -503,7 +513,7 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   p.status = a.status;
   const int pow = a.ce == 0.f || a.tau == 1.f ? 0 : a.tau == 2.f ? 2 : a.tau == 4.f ? 4 : 1;
   const size_t smem = plan.slice_bytes + a.k * sizeof(Entry);
-  auto launch = [&](auto kernel, auto* z, auto* t, auto* dz) {
+  auto launch = [&](auto kernel, auto* z, auto* dz) {
     TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(a.rows * plan.parts));
@@ -516,23 +526,20 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = plan.parts > 1 ? 1 : 0;
-    TTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, z, t, dz, p));
+    TTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, z, dz, p));
   };
   with_type(a.z_type, [&](auto* tz) {
     using TZ = std::remove_pointer_t<decltype(tz)>;
-    with_type(a.t_type, [&](auto* tt) {
-      using TT = std::remove_pointer_t<decltype(tt)>;
       auto with_grad = [&](auto* tg) {
         using TG = std::remove_pointer_t<decltype(tg)>;
         const auto* zp = static_cast<const TZ*>(a.z);
-        const auto* tp = static_cast<const TT*>(a.t);
         auto* gp = static_cast<TG*>(a.dz);
         auto with_pow = [&](auto w) {
           constexpr int POW = decltype(w)::value;
           if (gp == nullptr)
-            launch(distill_kernel<TZ, TT, TG, false, POW>, zp, tp, gp);
+            launch(distill_kernel<TZ, TG, false, POW>, zp, gp);
           else
-            launch(distill_kernel<TZ, TT, TG, true, POW>, zp, tp, gp);
+            launch(distill_kernel<TZ, TG, true, POW>, zp, gp);
         };
         switch (pow) {
           case 0: return with_pow(std::integral_constant<int, 0>{});
@@ -545,7 +552,6 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
         with_grad(static_cast<__nv_bfloat16*>(nullptr));
       else
         with_grad(static_cast<TZ*>(nullptr));
-    });
   });
 }
 
