@@ -215,8 +215,8 @@ constexpr int kMaxSlots = 8;
 // costs as much as about 20 elements per lane, so few warps with much of a row each beat many with little: the forward at
 // 2048 columns took 61 us with 8 elements (2450 instructions per row) and {FWD} us with 32; the backward, which also
 // holds its columns' sums, {BWD8} us with 8 and {BWD} us with 16.
-constexpr int kFwdPerThread = 32, kBwdPerThread = 16;
-constexpr int kFwdBlocks = 2, kBwdBlocks = 1;  // of 512 threads that fit an SM then
+constexpr int kFwdPerThread = 64, kBwdPerThread = 24;
+constexpr int kFwdBlocks = 1, kBwdBlocks = 1;  // of 512 threads that fit an SM then
 
 struct Ring {
   int slots;        // per group
@@ -255,7 +255,7 @@ __device__ __forceinline__ RingSide ring_side(const Ring& r, uint64_t (*full)[kM
   return RingSide{full[group], smem + static_cast<size_t>(group) * r.slots * r.slot_bytes, 0, 0};
 }
 
-template <typename TX, typename TY, int V, int NV>
+template <typename TX, typename TY, int V, int NV, int SURE>
 __global__ void __launch_bounds__(kThreads, kFwdBlocks) layer_norm_fwd_ring_kernel(
     const TX* __restrict__ x, long long ldx, const float* __restrict__ w, const float* __restrict__ b,
     TY* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, long long rows, int d, float eps, int gw,
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks) layer_norm_fwd_ring_kern
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = i * step + t * V;
-      if (j < d) {
+      if (i < SURE || j < d) {
         load_vec<V>(xr + j, v[i]);
 #pragma unroll
         for (int k = 0; k < V; ++k) s += v[i][k];
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks) layer_norm_fwd_ring_kern
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (i * step + t * V < d) {
+      if (i < SURE || i * step + t * V < d) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           v[i][k] -= mu;
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks) layer_norm_fwd_ring_kern
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = i * step + t * V;
-      if (j < d) {
+      if (i < SURE || j < d) {
         float wv[V], o[V];
         load_vec<V>(w + j, wv);
 #pragma unroll
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks) layer_norm_fwd_ring_kern
   }
 }
 
-template <typename TX, typename TY, int V, int NV>
+template <typename TX, typename TY, int V, int NV, int SURE>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) layer_norm_bwd_ring_kernel(
     const TY* __restrict__ dy, long long lddy, const TX* __restrict__ x, long long ldx, const float* __restrict__ w,
     const float* __restrict__ mean, const float* __restrict__ rstd, TX* __restrict__ dx, float* __restrict__ partials,
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) layer_norm_bwd_ring_kern
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = i * step + t * V;
-      if (j < d) {
+      if (i < SURE || j < d) {
         float wv[V];
         load_vec<V>(xr + j, xh[i]);
         load_vec<V>(dyr + j, g[i]);
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) layer_norm_bwd_ring_kern
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = i * step + t * V;
-      if (j < d) {
+      if (i < SURE || j < d) {
         float o[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) o[k] = r * (g[i][k] - ma - xh[i][k] * mb);
@@ -454,21 +454,28 @@ Split split_row(int d, int v, int most) {
 
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-template <int V, int... NV, typename F>
-void with_vectors(int nv, F&& f) {  // the smallest NV that holds nv
-  bool done = false;
-  ((done || nv > NV ? void() : (done = true, f(std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}))), ...);
-  TTB_CHECK(done, "layer norm: row split");
+// f(V, NV, SURE) with the smallest listed NV >= nv; SURE is the one before it: every thread has that many vectors.
+template <int V, int BEFORE, int FIRST, int... REST, typename F>
+void with_vectors(int nv, F&& f) {
+  using std::integral_constant;
+  if (nv <= FIRST) return f(integral_constant<int, V>{}, integral_constant<int, FIRST>{}, integral_constant<int, BEFORE>{});
+  if constexpr (sizeof...(REST) > 0) return with_vectors<V, FIRST, REST...>(nv, f);
+  TTB_CHECK(false, "layer norm: row split");
 }
 template <typename F>
 void with_split(const Split& s, F&& f) {  // rows straight into registers
-  if (s.v == 4) return with_vectors<4, 1, 2, 4, 8>(s.nv, f);
-  with_vectors<1, 4, 8, 16, 32>(s.nv, f);
+  if (s.v == 4) return with_vectors<4, 0, 1, 2, 4, 8>(s.nv, f);
+  with_vectors<1, 0, 4, 8, 16, 32>(s.nv, f);
 }
 template <typename F>
-void with_ring_split(const Split& s, F&& f) {
-  if (s.v == 8) return with_vectors<8, 1, 2, 3, 4>(s.nv, f);
-  with_vectors<4, 1, 2, 3, 4, 6, 8>(s.nv, f);
+void with_fwd_ring_split(const Split& s, F&& f) {
+  if (s.v == 8) return with_vectors<8, 0, 1, 2, 4, 6, 8>(s.nv, f);
+  with_vectors<4, 0, 1, 2, 4, 8, 12, 16>(s.nv, f);
+}
+template <typename F>
+void with_bwd_ring_split(const Split& s, F&& f) {
+  if (s.v == 8) return with_vectors<8, 0, 1, 2, 3, 4>(s.nv, f);
+  with_vectors<4, 0, 1, 2, 3, 4, 6, 8>(s.nv, f);
 }
 
 // Whether rows of d elements, ld apart, can be copied in 16-byte pieces.
@@ -504,6 +511,15 @@ int blocks_for(const LayerNormShape& s, const Split& sp, int per_sm) {
   return static_cast<int>(need < most ? need : most);
 }
 
+// The ring kernels are built for the pairs of types that models use: fp32 rows to any type, 16-bit rows to their own.
+bool ring_types(const LayerNormShape& s) { return s.x == ScalarType::kF32 || s.x == s.y; }
+template <typename F>
+void with_ring_types(const LayerNormShape& s, F&& f) {
+  if (s.x == ScalarType::kF32) return with_type(s.y, [&](auto* ty) { f(static_cast<float*>(nullptr), ty); });
+  with_type(s.x, [&](auto* tx) {
+    if constexpr (!std::is_same_v<decltype(tx), float*>) f(tx, tx);
+  });
+}
 template <typename F>
 void with_types(const LayerNormShape& s, F&& f) {
   with_type(s.x, [&](auto* tx) { with_type(s.y, [&](auto* ty) { f(tx, ty); }); });
@@ -515,16 +531,16 @@ void layer_norm_fwd(const LayerNormShape& s, const void* x, long long ldx, const
                     float* mean, float* rstd, float eps, cudaStream_t stream) {
   check(s);
   if (s.rows == 0) return;
-  if (whole_rows(x, ldx, s.d, s.x) && s.d % 8 == 0 && aligned(y, 16) && aligned(w, 16) && aligned(b, 16)) {
+  if (ring_types(s) && whole_rows(x, ldx, s.d, s.x) && s.d % 8 == 0 && aligned(y, 16) && aligned(w, 16) && aligned(b, 16)) {
     const Split sp = ring_split(s, kFwdPerThread);
     size_t smem;
     const int bytes = s.d * scalar_bytes(s.x);
     const Ring ring = make_ring(sp, bytes, bytes, kFwdBlocks, 0, smem);
-    with_types(s, [&](auto* tx, auto* ty) {
+    with_ring_types(s, [&](auto* tx, auto* ty) {
       using TX = std::remove_pointer_t<decltype(tx)>;
       using TY = std::remove_pointer_t<decltype(ty)>;
-      with_ring_split(sp, [&](auto v, auto nv) {
-        auto kernel = layer_norm_fwd_ring_kernel<TX, TY, decltype(v)::value, decltype(nv)::value>;
+      with_fwd_ring_split(sp, [&](auto v, auto nv, auto sure) {
+        auto kernel = layer_norm_fwd_ring_kernel<TX, TY, decltype(v)::value, decltype(nv)::value, decltype(sure)::value>;
         TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
         kernel<<<blocks_for(s, sp, kFwdBlocks), kThreads, smem, stream>>>(
             static_cast<const TX*>(x), ldx, w, b, static_cast<TY*>(y), mean, rstd, s.rows, s.d, eps, sp.gw, ring);
@@ -539,7 +555,7 @@ void layer_norm_fwd(const LayerNormShape& s, const void* x, long long ldx, const
   with_types(s, [&](auto* tx, auto* ty) {
     using TX = std::remove_pointer_t<decltype(tx)>;
     using TY = std::remove_pointer_t<decltype(ty)>;
-    with_split(sp, [&](auto v, auto nv) {
+    with_split(sp, [&](auto v, auto nv, auto) {
       layer_norm_fwd_kernel<TX, TY, decltype(v)::value, decltype(nv)::value>
           <<<blocks_for(s, sp, 4), kThreads, 0, stream>>>(static_cast<const TX*>(x), ldx, w, b, static_cast<TY*>(y),
                                                           mean, rstd, s.rows, s.d, eps, sp.gw);
@@ -561,18 +577,18 @@ void layer_norm_bwd(const LayerNormShape& s, const void* dy, long long lddy, con
   TTB_CHECK(s.rows > 0, "layer norm backward: no rows");
   const size_t sums = static_cast<size_t>(s.d) * 2 * sizeof(float);
   int grid = 0;
-  if (whole_rows(x, ldx, s.d, s.x) && whole_rows(dy, lddy, s.d, s.y) && s.d % 8 == 0 && aligned(dx, 16) &&
+  if (ring_types(s) && whole_rows(x, ldx, s.d, s.x) && whole_rows(dy, lddy, s.d, s.y) && s.d % 8 == 0 && aligned(dx, 16) &&
       aligned(w, 16)) {
     const Split sp = ring_split(s, kBwdPerThread);
     size_t smem;
     const int bytes = s.d * scalar_bytes(s.x);
     const Ring ring = make_ring(sp, bytes, bytes + s.d * scalar_bytes(s.y), kBwdBlocks, sums, smem);
     grid = blocks_for(s, sp, kBwdBlocks);
-    with_types(s, [&](auto* tx, auto* ty) {
+    with_ring_types(s, [&](auto* tx, auto* ty) {
       using TX = std::remove_pointer_t<decltype(tx)>;
       using TY = std::remove_pointer_t<decltype(ty)>;
-      with_ring_split(sp, [&](auto v, auto nv) {
-        auto kernel = layer_norm_bwd_ring_kernel<TX, TY, decltype(v)::value, decltype(nv)::value>;
+      with_bwd_ring_split(sp, [&](auto v, auto nv, auto sure) {
+        auto kernel = layer_norm_bwd_ring_kernel<TX, TY, decltype(v)::value, decltype(nv)::value, decltype(sure)::value>;
         TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
         kernel<<<grid, kThreads, smem, stream>>>(static_cast<const TY*>(dy), lddy, static_cast<const TX*>(x), ldx, w,
                                                  mean, rstd, static_cast<TX*>(dx), partials, s.rows, s.d, sp.gw, ring);
@@ -586,7 +602,7 @@ void layer_norm_bwd(const LayerNormShape& s, const void* dy, long long lddy, con
     with_types(s, [&](auto* tx, auto* ty) {
       using TX = std::remove_pointer_t<decltype(tx)>;
       using TY = std::remove_pointer_t<decltype(ty)>;
-      with_split(sp, [&](auto v, auto nv) {
+      with_split(sp, [&](auto v, auto nv, auto) {
         auto kernel = layer_norm_bwd_kernel<TX, TY, decltype(v)::value, decltype(nv)::value>;
         if (sums > 40 * 1024)
           TTB_CUDA_CHECK(
