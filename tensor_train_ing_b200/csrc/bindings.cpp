@@ -2,8 +2,10 @@
 // pointers/strides here; the CUDA translation units never include torch headers.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cmath>
 #include <string>
 #include <vector>
@@ -304,6 +306,41 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x, const Tens
   return {dx, dwb.select(0, 0), dwb.select(0, 1)};
 }
 
+// Kernels launched by the autograd nodes below, which run without passing through Python (the launch counter of
+// ops/_ext.py adds them to those of the bindings).
+std::atomic<int64_t> autograd_launches{0};
+
+// layer_norm with its backward as a node of the graph.  Node and call are C++: at small sizes the time of a call is the
+// host's, and a Python autograd function costs more of it than both kernels.
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                        const c10::optional<Tensor>& b, double eps, int64_t out) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto r = layer_norm_fwd(x, w, b, eps, static_cast<torch::ScalarType>(out), true);
+    ctx->save_for_backward({x, w, r[1]});
+    ctx->saved_data["bias"] = b.has_value();
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    Tensor dy = grads[0];
+    if (dy.size(1) > 1 && dy.stride(1) != 1) dy = dy.contiguous();
+    const auto r = layer_norm_bwd(dy, saved[0], saved[1], saved[2]);
+    if (saved[0].size(0) > 0) autograd_launches += 2;
+    return {r[0], r[1], ctx->saved_data["bias"].toBool() ? r[2] : Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// x [N, d] -> y [N, d], differentiable where gradients are recorded.
+Tensor layer_norm(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& b, double eps,
+                  torch::ScalarType out) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (b.has_value() && b->requires_grad())))
+    return LayerNormNode::apply(x, w, b, eps, static_cast<int64_t>(out));
+  return layer_norm_fwd(x, w, b, eps, out, false)[0];
+}
+
 // ------------------------------------------------------------------ distillation
 // z [N, V] -> (values [N, k], ids int32 [N, k], lse [N])
 std::vector<Tensor> top_logits(const Tensor& z, int64_t k, double tau) {
@@ -394,6 +431,50 @@ void scale_rows_(Tensor& dz, const Tensor& g) {
   check_f32_vector(g, "g", g.numel() == 1 ? 1 : N, dz);
   ttb::scale_in_place(dz.data_ptr(), scalar_type(dz, "dz"), N, static_cast<int>(dz.size(1)), dz.stride(0),
                       g.data_ptr<float>(), g.numel() == 1 ? 0 : 1, cur_stream());
+}
+
+// An uninitialised gradient with the rows' stride where that wastes little: its rows then have the alignment of the
+// logits' rows, and the kernel stores whole vectors.
+Tensor gradient_like(const Tensor& z) {
+  const int64_t n = z.size(0), v = z.size(1), ld = n > 1 ? z.stride(0) : v;
+  return at::empty_strided({n, v}, {ld >= v && ld < v + 64 ? ld : v, 1}, z.options());
+}
+
+// distill_loss with its gradient formed in the same pass over the logits and kept instead of them; the backward
+// multiplies it by the incoming factor in place, so it can run once.
+struct DistillNode : torch::autograd::Function<DistillNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& z, const Tensor& ids, const Tensor& t,
+                        const c10::optional<Tensor>& teacher_lse, const c10::optional<Tensor>& targets, double tau,
+                        double kd, double ce, const c10::optional<Tensor>& scale, bool total) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    Tensor dz = gradient_like(z);
+    Tensor loss = distill_loss(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, dz);
+    ctx->saved_data["dz"] = dz;
+    return total ? loss.sum() : loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto& kept = ctx->saved_data["dz"];
+    TORCH_CHECK(kept.isTensor(), "distillation_loss: the gradient was handed out by an earlier backward");
+    Tensor dz = kept.toTensor();
+    kept = c10::IValue();
+    scale_rows_(dz, grads[0].contiguous());
+    if (dz.size(0) > 0) autograd_launches += 1;
+    torch::autograd::variable_list out(10);
+    out[0] = dz;
+    return out;
+  }
+};
+
+// Rows of the distillation loss, or their sum; differentiable with respect to z where gradients are recorded.
+Tensor distillation(const Tensor& z, const Tensor& ids, const Tensor& t, const c10::optional<Tensor>& teacher_lse,
+                    const c10::optional<Tensor>& targets, double tau, double kd, double ce,
+                    const c10::optional<Tensor>& scale, bool total) {
+  if (at::GradMode::is_enabled() && z.requires_grad())
+    return DistillNode::apply(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, total);
+  const Tensor loss = distill_loss(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, c10::nullopt);
+  return total ? loss.sum() : loss;
 }
 
 bool logits_row_fits(int64_t columns, torch::ScalarType type) {
@@ -918,16 +999,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_bwd", &rmsnorm_bwd, "(group) RMSNorm backward; adds dx into the residual grad, returns dw",
         py::arg("dy"), py::arg("x"), py::arg("w"), py::arg("rstd"), py::arg("dres"), py::arg("accumulate"),
         py::arg("groups"), py::arg("out16") = py::none(), py::arg("scale16") = 1.0);
-  m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm: y and, on request, the rows' mean and 1/std", py::arg("x"),
-        py::arg("w"), py::arg("b"), py::arg("eps"), py::arg("out"), py::arg("stats"));
-  m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward: dx, dw, db", py::arg("dy"), py::arg("x"),
-        py::arg("w"), py::arg("stat"));
+  m.def("layer_norm", &layer_norm, "layer norm of rows, differentiable", py::arg("x"), py::arg("w"), py::arg("b"),
+        py::arg("eps"), py::arg("out"));
+  m.def("autograd_launches", [] { return autograd_launches.load(); },
+        "kernels launched so far by the library's own autograd nodes");
   m.def("top_logits", &top_logits, "the k largest logits of each row, their columns and the row's log-sum-exp",
         py::arg("z"), py::arg("k"), py::arg("tau"));
   m.def("distill_loss", &distill_loss, "distillation loss of each row and, into dz, its gradient", py::arg("z"),
         py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),
         py::arg("ce"), py::arg("scale"), py::arg("dz"));
-  m.def("scale_rows_", &scale_rows_, "rows of dz times their factor, in place", py::arg("dz"), py::arg("g"));
+  m.def("distillation", &distillation, "distillation loss of rows or their sum, differentiable", py::arg("z"),
+        py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),
+        py::arg("ce"), py::arg("scale"), py::arg("total"));
   m.def("logits_row_fits", &logits_row_fits, "whether rows of this many logits fit the distillation kernels");
   m.def("rope_", &rope_, "in-place rotary embedding (or its inverse) on a bf16 [N, ld] buffer");
   m.def("embed_fwd", &embed_fwd, "fp32 embedding gather");

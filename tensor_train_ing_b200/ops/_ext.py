@@ -34,8 +34,8 @@ KERNELS_PER_CALL = {"mm": 1, "bilinear": 1, "bilinear_grad": 1, "rmsnorm_fwd": 1
                     "rs_accumulate": 1, "ce_bwd_from_logits": 1, "adamw_update": 2, "muon_prepare": 1,
                     "muon_normalize": 1, "muon_apply": 1, "norm_variant_fwd": 1,
                     "norm_variant_bwd": _norm_variant_bwd_kernels, "spectral_cast": 2, "spectral_grad": 2,
-                    "spectral_power_step": 4, "gather_rows": 1, "layer_norm_fwd": 1, "layer_norm_bwd": 2, "top_logits": 1,
-                    "distill_loss": 1, "scale_rows_": 1}
+                    "spectral_power_step": 4, "gather_rows": 1, "layer_norm": 1, "top_logits": 1,
+                    "distill_loss": 1, "distillation": 1}
 
 
 class _Counting:
@@ -72,12 +72,17 @@ class launch_counter:
         _PROXY.enabled = True
         _PROXY.count = 0
         _PROXY.by_name = {}
+        self._autograd = _PROXY.autograd_launches()
         return self
 
     def __exit__(self, *exc):
         _PROXY.enabled = False
         self.count = _PROXY.count
         self.by_name = dict(_PROXY.by_name)
+        backward = _PROXY.autograd_launches() - self._autograd  # C++ autograd nodes: layer norm, distillation
+        if backward:
+            self.count += backward
+            self.by_name["autograd"] = backward
         return False
 
 

@@ -65,34 +65,9 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     return TopLogits(values.view(*lead, k), ids.view(*lead, k), lse.view(lead))
 
 
-def _gradient_like(rows: torch.Tensor) -> torch.Tensor:
-    """An uninitialised gradient with the rows' stride where that wastes little: its rows then have
-    the alignment of the logits' rows, and the kernel stores whole vectors."""
-    n, v = rows.shape
-    ld = rows.stride(0) if n > 1 else v
-    return torch.empty_strided((n, v), (ld if v <= ld < v + 64 else v, 1), dtype=rows.dtype, device=rows.device)
-
-
-class DistillationFn(torch.autograd.Function):
-    """The forward forms the gradient in the same pass over the logits and keeps it instead of them; the
-    backward multiplies it by the incoming factor in place (nothing to do when that is 1, which ``scale``
-    makes the usual case).  It can therefore run once."""
-
-    @staticmethod
-    def forward(ctx, rows, ids, t, teacher_lse, targets, tau, kd, ce, scale, reduction):
-        dz = _gradient_like(rows)
-        loss = lib().distill_loss(rows, ids, t, teacher_lse, targets, tau, kd, ce, scale, dz)
-        ctx.dz = dz
-        return loss.sum() if reduction == "sum" else loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        dz, ctx.dz = ctx.dz, None
-        if dz is None:
-            raise RuntimeError("distillation_loss: the gradient was handed out by an earlier backward")
-        lib().scale_rows_(dz, g.contiguous())
-        return (dz,) + (None,) * 9
+def _flat(t, *shape):
+    """``t`` as a dense tensor of this shape, itself where it is one already."""
+    return t if t.shape == shape and t.is_contiguous() else t.reshape(shape).contiguous()
 
 
 def _list_arguments(rows, teacher_ids, teacher_logits, teacher_lse, targets, ce_weight, scale):
@@ -116,17 +91,16 @@ def _list_arguments(rows, teacher_ids, teacher_logits, teacher_lse, targets, ce_
         if value is not None and value.numel() != n:
             raise ValueError(f"distillation_loss: {name} has {value.numel()} elements for {n} rows")
     if teacher_lse is not None:
-        teacher_lse = teacher_lse.detach().reshape(-1).float().contiguous()
+        teacher_lse = _flat(teacher_lse.detach().float(), n)
     if targets is not None:
-        targets = targets.reshape(-1).contiguous()
+        targets = _flat(targets, n)
     if scale is not None:
         if not isinstance(scale, torch.Tensor):
             scale = torch.full((1,), float(scale), device=rows.device)
         if scale.numel() != 1:
             raise ValueError(f"distillation_loss: scale must be one number, not {tuple(scale.shape)}")
-        scale = scale.detach().reshape(1).float()
-    return (teacher_ids.reshape(n, k).contiguous(), teacher_logits.detach().reshape(n, k).contiguous(), teacher_lse,
-            targets, scale)
+        scale = scale.detach().float()
+    return _flat(teacher_ids, n, k), _flat(teacher_logits.detach(), n, k), teacher_lse, targets, scale
 
 
 def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
@@ -145,7 +119,8 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     the update's target count) multiplies loss and gradient inside the kernel, before the gradient is rounded
     to the logits' type, so that ``backward()`` has nothing left to do.
 
-    Differentiable with respect to ``logits`` alone, once.  A teacher's mass outside its list at or below
+    Differentiable with respect to ``logits`` alone, once: the forward forms the gradient in the same pass over the
+    logits and keeps it instead of them; the backward multiplies it by the incoming factor in place.  A teacher's mass outside its list at or below
     2^-20 counts as none (that is what rounding leaves of 1 - sum p)."""
     if not temperature > 0:
         raise ValueError(f"distillation_loss: the temperature must be positive, not {temperature}")
@@ -154,11 +129,6 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     rows = _rows(logits, "distillation_loss")
     ids, t, teacher_lse, targets, scale = _list_arguments(rows, teacher_ids, teacher_logits, teacher_lse, targets,
                                                           ce_weight, scale)
-    args = (ids, t, teacher_lse, targets, float(temperature), float(kd_weight), float(ce_weight), scale)
-    if torch.is_grad_enabled() and rows.requires_grad:
-        loss = DistillationFn.apply(rows, *args, reduction)
-    else:
-        loss = lib().distill_loss(rows, *args, None)
-        if reduction == "sum":
-            loss = loss.sum()
+    loss = lib().distillation(rows, ids, t, teacher_lse, targets, temperature, kd_weight, ce_weight, scale,
+                              reduction == "sum")
     return loss if reduction == "sum" or logits.dim() == 2 else loss.view(logits.shape[:-1])

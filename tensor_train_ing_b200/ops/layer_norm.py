@@ -15,34 +15,16 @@ MAX_DIM = 16384
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-class LayerNormFn(torch.autograd.Function):
-    """x: [N, d] rows.  The backward reads x again with the forward's per-row mean and rstd; weight and
-    bias gradients are summed in a fixed order (the same inputs give the same bits)."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, out_dtype):
-        y, stat = lib().layer_norm_fwd(x, weight, bias, eps, out_dtype, True)
-        ctx.save_for_backward(x, weight, stat)
-        ctx.has_bias = bias is not None
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, stat = ctx.saved_tensors
-        if dy.stride(-1) != 1:
-            dy = dy.contiguous()
-        dx, dw, db = lib().layer_norm_bwd(dy, x, weight, stat)
-        return dx, dw, db if ctx.has_bias else None, None, None
-
-
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, eps: float = 1e-5,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Normalise ``x`` (..., d) over its last dimension.
 
     ``x``: fp32, bf16 or fp16 on CUDA, any strides (rows with a unit column stride are read in place),
     1 <= d <= 16384.  ``weight`` and the optional ``bias``: fp32 [d].  The result is ``out_dtype`` (default
-    x's), dense.  Statistics and sums are fp32; the result is rounded once.  Runs on the current stream."""
+    x's), dense.  Statistics and sums are fp32; the result is rounded once.  Runs on the current stream.
+
+    Differentiable with respect to ``x``, ``weight`` and ``bias``: the backward reads ``x`` again with the forward's
+    per-row mean and rstd, and sums the weight and bias gradients in a fixed order (the same inputs give the same bits)."""
     if not x.is_cuda:
         raise ValueError("layer_norm: x must be a CUDA tensor (models.normalization.LayerNorm has the CPU form)")
     out_dtype = x.dtype if out_dtype is None else out_dtype
@@ -54,13 +36,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must not be negative ({eps})")
     rows = x if x.dim() == 2 else x.reshape(-1, d)
-    if rows.stride(1) != 1 and d > 1:
+    if d > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
-    weight = weight.contiguous()
-    bias = bias.contiguous() if bias is not None else None
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
-        y = LayerNormFn.apply(rows, weight, bias, float(eps), out_dtype)
-    else:
-        y = lib().layer_norm_fwd(rows, weight, bias, float(eps), out_dtype, False)[0]
+    y = lib().layer_norm(rows, weight.contiguous(), bias.contiguous() if bias is not None else None, eps, out_dtype)
     return y if x.dim() == 2 else y.view(x.shape)
