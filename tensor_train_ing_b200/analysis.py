@@ -31,7 +31,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .models.attention import apply_rope, doc_positions, rope_tables, visible_mask
-from .models.normalization import (DynamicNorm, GroupRMSNorm, LaggedRMS, RMSNorm, SpectralLinear, TaperRMS,
+from .models.normalization import (DynamicNorm, GroupRMSNorm, LaggedRMS, LayerNorm, RMSNorm, SpectralLinear, TaperRMS,
                                    dynamic_norms, upcast)
 
 QUANTILES = (0.01, 0.05, 0.5, 0.95, 0.99)
@@ -66,6 +66,8 @@ def gain(norm: nn.Module, d: int, device) -> torch.Tensor:
         if g == 0.0 and bool(norm.frozen):
             return float(norm.c) * upcast(norm.weight_tilde.detach())
         raise ValueError(f"a TaperRMS at gate {g} (frozen={bool(norm.frozen)}) has no fixed map to fold")
+    if isinstance(norm, LayerNorm):
+        raise ValueError("a layer norm subtracts the mean and adds a bias: it is no per-feature map to fold")
     w = getattr(norm, "weight", None)
     if w is None:  # nn.Identity
         return torch.ones(d, device=device)

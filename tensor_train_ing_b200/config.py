@@ -8,6 +8,8 @@ section (``project``, ``data``, ``evaluation``, ``b200`` ...) is kept verbatim i
 Additions of this framework:
   * ``attention_backend`` also accepts ``"cuda"``; ``"triton"`` (the reference's name for its
     tiled kernel) selects the same hand-written sm_100a kernels here;
+  * ``normalization="pre_ln"`` and ``final_normalization="layer"`` use layer norm (mean subtracted, gain and bias),
+    the norm of conventional transformers, for controls and teachers;
   * ``attention_backend="recurrent"`` runs polynomial attention in its chunked linear-state form
     (``models/long_context.py``): no T x T matrix, for very long contexts.
 """
@@ -20,8 +22,8 @@ import yaml
 
 MLP_KINDS = ("bilinear", "affine_bilinear", "swiglu")
 ATTN_KINDS = ("signed_product", "offset_square", "lower_degree_mix", "softmax")
-NORM_PACKAGES = ("pre_rms", "branch_rms", "sandwich_rms", "group_rms", "spectral_rms", "lagged", "taper")
-FINAL_NORMS = ("rms", "lagged", "taper")
+NORM_PACKAGES = ("pre_rms", "branch_rms", "sandwich_rms", "group_rms", "spectral_rms", "lagged", "taper", "pre_ln")
+FINAL_NORMS = ("rms", "lagged", "taper", "layer")
 ATTN_BACKENDS = ("reference", "triton", "cuda", "auto", "recurrent")
 
 

@@ -1008,6 +1008,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_loss", &distill_loss, "distillation loss of each row and, into dz, its gradient", py::arg("z"),
         py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),
         py::arg("ce"), py::arg("scale"), py::arg("dz"));
+  m.def("scale_rows_", &scale_rows_, "rows of dz times their factor, in place", py::arg("dz"), py::arg("g"));
   m.def("distillation", &distillation, "distillation loss of rows or their sum, differentiable", py::arg("z"),
         py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),
         py::arg("ce"), py::arg("scale"), py::arg("total"));

@@ -112,12 +112,16 @@ class TrainEngine:
     def begin_update(self):
         self.zero_grad()
 
-    def forward_loss(self, idx, doc_ids, targets):
-        """One micro-batch's forward: (summed loss, valid-target count) on the device."""
+    def forward_loss(self, idx, doc_ids, targets, teacher=None, scale=None):
+        """One micro-batch's forward: (summed loss, valid-target count) on the device.  ``teacher`` (its lists for these
+        tokens) makes it the distillation loss, times ``scale``."""
         if self._recompute_auto:
             self._resolve_auto_recompute(idx.numel())
         i, d, t = (self._to_device(x) for x in (idx, doc_ids, targets))
-        _, loss, n = self.model(i, d, t, reduction="sum")
+        if teacher is None:
+            _, loss, n = self.model(i, d, t, reduction="sum")
+        else:
+            _, loss, n = self.model(i, d, t, reduction="sum", teacher=teacher, scale=scale)
         return loss, n
 
     def backward(self, objective):
@@ -163,19 +167,27 @@ class TrainEngine:
         self._mark(marks, "gather_params")
         return self.last_grad_norm
 
-    def forward_backward(self, idx, doc_ids, targets, inv_count):
+    def forward_backward(self, idx, doc_ids, targets, inv_count, teacher=None):
         """Accumulate gradients of sum(loss) * inv_count over micro-batches; returns the loss sum."""
         loss_total = torch.zeros((), device=self.device, dtype=torch.float32)
         rows = idx.shape[0]
         for s in range(0, rows, self.micro_batch):
             e = min(rows, s + self.micro_batch)
-            loss, _ = self.forward_loss(idx[s:e], doc_ids[s:e], targets[s:e])
-            self.backward(loss * inv_count)
-            loss_total += loss.detach().float()
+            if teacher is None:
+                loss, _ = self.forward_loss(idx[s:e], doc_ids[s:e], targets[s:e])
+                self.backward(loss * inv_count)
+                loss_total += loss.detach().float()
+            else:  # 1 / count goes into the loss kernel, which rounds the logits' gradient after it
+                loss, _ = self.forward_loss(idx[s:e], doc_ids[s:e], targets[s:e], teacher.rows(s, e, self.device),
+                                            inv_count)
+                self.backward(loss)
+                loss_total += loss.detach().float() / inv_count
         return loss_total
 
-    def step(self, idx, doc_ids, targets, lr_multiplier: float | None = None):
-        """One optimizer update on this rank's rows.  Returns (loss_sum, global_count) on the device."""
+    def step(self, idx, doc_ids, targets, lr_multiplier: float | None = None, teacher=None):
+        """One optimizer update on this rank's rows.  Returns (loss_sum, global_count) on the device.
+        ``teacher`` (``ops.distill.Teacher``, lists for this rank's rows, host or device): distil from it instead of
+        learning the targets alone."""
         if lr_multiplier is not None:
             for g in self.optimizer.param_groups:
                 g["lr"] = g.get("base_lr", g["lr"]) * lr_multiplier
@@ -188,7 +200,7 @@ class TrainEngine:
         if self.world > 1:
             dist.all_reduce(count, group=self.group)
         inv = 1.0 / count.clamp_min(1).to(torch.float32)
-        loss_sum = self.forward_backward(idx, doc_ids, targets, inv)
+        loss_sum = self.forward_backward(idx, doc_ids, targets, inv, teacher)
         self._mark(marks, "forward_backward")
         if self.world > 1:
             dist.all_reduce(loss_sum, group=self.group)

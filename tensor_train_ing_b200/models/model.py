@@ -35,6 +35,7 @@ PACKAGES = {
     "spectral_rms": ("rms", None, True),
     "lagged": ("lagged", None, False),
     "taper": ("taper", None, False),
+    "pre_ln": ("layer", None, False),
 }
 # operator classes from least to most general: polynomial, normalised, general (softmax / SiLU)
 CLASS_ORDER = {"P": 0, "N": 1, "G": 2}
@@ -371,13 +372,32 @@ class TensorLM(nn.Module):
         wide = logits.to(torch.promote_types(logits.dtype, torch.float32))
         return logits, F.cross_entropy(wide.flatten(0, 1), targets.flatten(), ignore_index=-100, reduction="sum")
 
-    def forward(self, idx, doc_ids=None, targets=None, reduction="mean"):
+    def _distill(self, x, targets, teacher, scale):
+        """Summed distillation loss (module path): on the kernels where the logits are theirs, else in plain PyTorch."""
+        from ..ops import distill
+        logits = self.unembed(x)[..., :self.cfg.vocab_size]
+        if self.cfg.width_scaling_base:
+            logits = logits * self.logit_multiplier
+        on_kernels = logits.is_cuda and logits.dtype in (torch.float32, torch.bfloat16, torch.float16)
+        loss = distill.distillation_loss if on_kernels else distill.distillation_loss_reference
+        return loss(logits, teacher.ids, teacher.values, teacher.lse, targets, teacher.temperature, teacher.kd_weight,
+                    teacher.ce_weight, scale)
+
+    def forward(self, idx, doc_ids=None, targets=None, reduction="mean", teacher=None, scale=None):
         """Logits (no targets), else (logits or None, loss sum, valid targets) for ``reduction="sum"``
-        or (logits or None, mean loss)."""
+        or (logits or None, mean loss).
+
+        ``teacher`` (``ops.distill.Teacher`` for these tokens): the loss is the distillation loss against
+        its lists instead of cross-entropy, over the tokens with a valid target.  ``scale`` (a one-element tensor,
+        with a teacher): multiplies that loss, and its gradient before that is rounded."""
+        if teacher is not None and targets is None:
+            raise ValueError("distillation needs targets: they say which tokens count (-100 leaves one out)")
+        if scale is not None and teacher is None:
+            raise ValueError("scale belongs to the distillation loss: pass a teacher")
         ctx = self.make_ctx(idx, doc_ids)
         if ctx.get("fused"):
             from ..ops.block import model_forward
-            return model_forward(self, idx, ctx, targets, reduction)
+            return model_forward(self, idx, ctx, targets, reduction, teacher, scale)
         if getattr(self, "_ttb_weights_remote", False):
             raise RuntimeError("this parameter-sharded model holds non-owned weights only as the fused path's bf16 "
                                "caches; the module path cannot run it")
@@ -385,6 +405,9 @@ class TensorLM(nn.Module):
         if targets is None:
             logits = self.unembed(x)[..., :self.cfg.vocab_size]
             return logits * self.logit_multiplier if self.cfg.width_scaling_base else logits
-        logits, loss = self._loss(x, targets)
+        if teacher is not None:
+            logits, loss = None, self._distill(x, targets, teacher, scale)
+        else:
+            logits, loss = self._loss(x, targets)
         n = (targets != -100).sum()
         return (logits, loss, n) if reduction == "sum" else (logits, loss / n.clamp_min(1))

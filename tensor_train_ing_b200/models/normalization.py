@@ -10,6 +10,10 @@ so CPU trajectories agree bit for bit:
                            ema_num, ema_den, ema_r, ema_steps, frozen
   SpectralLinear           weight, [bias], gamma, u, v
 
+and, of this framework alone,
+
+  LayerNorm                weight, bias                                   class "N"
+
 Structure: ``DynamicNorm`` is an input-dependent divisor with analysis hooks (record / clamp / const);
 ``_StatNorm`` is the base of the two norms that learn statistics while training (a valid-token mask,
 count-weighted accumulators summed across data-parallel ranks at commit); ``SpectralLinear`` keeps
@@ -97,6 +101,37 @@ class GroupRMSNorm(DynamicNorm):
     def denom(self, x):
         xg = upcast(x).unflatten(-1, (self.groups, -1))
         return _rms(xg, self.eps).expand_as(xg).flatten(-2)
+
+
+class LayerNorm(nn.Module):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the features, with the biased variance: the norm of
+    conventional transformers.  CUDA rows run on the kernels of ops/layer_norm.py; ``plain`` is the definition
+    they are tested against and the CPU path."""
+
+    op_class = "N"
+
+    def __init__(self, d: int, eps: float):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(d))
+        self.bias = nn.Parameter(torch.zeros(d))
+
+    def plain(self, x):
+        xf = upcast(x)
+        centred = xf - xf.mean(-1, keepdim=True)
+        y = centred / torch.sqrt(centred.pow(2).mean(-1, keepdim=True) + self.eps)
+        return (y * upcast(self.weight) + upcast(self.bias)).to(x.dtype)
+
+    def kernel_ok(self, x) -> bool:
+        from ..ops.layer_norm import MAX_DIM
+        return (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16, torch.float16) and x.shape[-1] <= MAX_DIM
+                and self.weight.dtype == self.bias.dtype == torch.float32)
+
+    def forward(self, x):
+        if not self.kernel_ok(x):
+            return self.plain(x)
+        from ..ops.layer_norm import layer_norm
+        return layer_norm(x, self.weight, self.bias, self.eps)
 
 
 # ------------------------------------------------------------------------------------ learned statistics
@@ -421,6 +456,7 @@ _NORM_KINDS = {
     "group": lambda d, cfg: GroupRMSNorm(d, cfg.norm_groups, cfg.rms_eps),
     "lagged": lambda d, cfg: LaggedRMS(d, cfg.rms_eps, cfg.lagged_half_life_tokens),
     "taper": lambda d, cfg: TaperRMS(d, cfg.rms_eps, cfg.taper_ema_rate),
+    "layer": lambda d, cfg: LayerNorm(d, cfg.rms_eps),
 }
 
 

@@ -78,7 +78,8 @@ def count_params(cfg: ModelConfig) -> dict:
     per_block = sum(p.numel() for p in blk.parameters())
     per_block_mat = sum(p.numel() for p in blk.parameters() if p.dim() >= 2)
     emb = cfg.padded_vocab * cfg.d_model * (1 if cfg.tie_embeddings else 2)
-    return {"total": cfg.layers * per_block + emb + cfg.d_model, "matrices": cfg.layers * per_block_mat + emb,
+    final = cfg.d_model * (2 if cfg.final_normalization == "layer" else 1)  # gain, and a layer norm's bias
+    return {"total": cfg.layers * per_block + emb + final, "matrices": cfg.layers * per_block_mat + emb,
             "non_embedding": cfg.layers * per_block_mat, "per_block": per_block, "embedding": emb}
 
 

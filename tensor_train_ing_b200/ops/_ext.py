@@ -35,7 +35,7 @@ KERNELS_PER_CALL = {"mm": 1, "bilinear": 1, "bilinear_grad": 1, "rmsnorm_fwd": 1
                     "muon_normalize": 1, "muon_apply": 1, "norm_variant_fwd": 1,
                     "norm_variant_bwd": _norm_variant_bwd_kernels, "spectral_cast": 2, "spectral_grad": 2,
                     "spectral_power_step": 4, "gather_rows": 1, "layer_norm": 1, "top_logits": 1,
-                    "distill_loss": 1, "distillation": 1}
+                    "distill_loss": 1, "distillation": 1, "scale_rows_": 1}
 
 
 class _Counting:

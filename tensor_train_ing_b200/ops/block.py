@@ -16,8 +16,9 @@ import torch
 import torch.nn as nn
 
 from ..models.attention import rope_inv_freq, row_scale_vector
-from ..models.normalization import GroupRMSNorm, LaggedRMS, RMSNorm, SpectralLinear, TaperRMS
+from ..models.normalization import GroupRMSNorm, LaggedRMS, LayerNorm, RMSNorm, SpectralLinear, TaperRMS
 from . import fused, norms
+from .layer_norm import layer_norm
 from .weights import group_for, spectral_group_for
 
 
@@ -71,6 +72,8 @@ def norm_to_bf16(norm: nn.Module, x: torch.Tensor) -> torch.Tensor:
         return norms.lagged_to_bf16(norm, x)
     if isinstance(norm, TaperRMS) and x.shape[-1] % 4 == 0:
         return norms.taper_to_bf16(norm, x)
+    if isinstance(norm, LayerNorm) and norm.kernel_ok(x):
+        return layer_norm(x, norm.weight, norm.bias, norm.eps, torch.bfloat16)
     return norm(x).to(torch.bfloat16)
 
 
@@ -168,7 +171,7 @@ def block_forward(blk, x, ctx):
     return x
 
 
-def model_forward(model, idx, ctx, targets, reduction):
+def model_forward(model, idx, ctx, targets, reduction, teacher=None, scale=None):
     cfg = model.cfg
     B, T = idx.shape
     x = fused.embedding(idx.reshape(-1), group_for(model, "embed", [model.embed.weight]))
@@ -186,7 +189,11 @@ def model_forward(model, idx, ctx, targets, reduction):
     V = cfg.vocab_size
     ug = group_for(model, "unembed", [model.unembed.weight])
     alpha = model.logit_multiplier
-    if targets is not None and cfg.loss_chunk_tokens > 0:
+    if teacher is not None:
+        chunk = cfg.loss_chunk_tokens or 8192
+        loss = fused.linear_distillation(h, targets.reshape(-1), ug, V, teacher, alpha, chunk, scale)
+        logits = None
+    elif targets is not None and cfg.loss_chunk_tokens > 0:
         loss = fused.linear_cross_entropy(h, targets.reshape(-1), ug, V, alpha, cfg.loss_chunk_tokens)
         logits = None
     else:

@@ -15,6 +15,7 @@ tau^2 keeps the gradient's size independent of the temperature (Hinton, Vinyals,
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -32,6 +33,22 @@ class TopLogits(NamedTuple):
     values: torch.Tensor
     ids: torch.Tensor
     lse: torch.Tensor
+
+
+class Teacher(NamedTuple):
+    """What a student learns from: lists for its (B, T) tokens and how the loss weighs them.  ``ids`` and
+    ``values`` (B, T, k), ``lse`` (B, T) or None, as ``top_logits`` gives them at the same ``temperature``."""
+    ids: torch.Tensor
+    values: torch.Tensor
+    lse: torch.Tensor | None = None
+    temperature: float = 1.0
+    kd_weight: float = 1.0
+    ce_weight: float = 0.0
+
+    def rows(self, start: int, end: int, device=None) -> "Teacher":
+        """The lists of the sequences [start, end), on ``device``."""
+        part = lambda t: None if t is None else t[start:end].to(device or t.device, non_blocking=True)  # noqa: E731
+        return self._replace(ids=part(self.ids), values=part(self.values), lse=part(self.lse))
 
 
 def _rows(logits: torch.Tensor, what: str) -> torch.Tensor:
@@ -132,3 +149,53 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     loss = lib().distillation(rows, ids, t, teacher_lse, targets, temperature, kd_weight, ce_weight, scale,
                               reduction == "sum")
     return loss if reduction == "sum" or logits.dim() == 2 else loss.view(logits.shape[:-1])
+
+
+# ------------------------------------------------------------------------------------ plain forms
+@torch.no_grad()
+def top_logits_reference(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """``top_logits`` in plain PyTorch (any device)."""
+    values, ids = torch.sort(logits, dim=-1, descending=True, stable=True)
+    wide = logits.to(torch.promote_types(logits.dtype, torch.float32))
+    return TopLogits(values[..., :k], ids[..., :k].to(torch.int32), torch.logsumexp(wide / temperature, -1))
+
+
+def distillation_loss_reference(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                                teacher_lse: torch.Tensor | None = None, targets: torch.Tensor | None = None,
+                                temperature: float = 1.0, kd_weight: float = 1.0, ce_weight: float = 0.0,
+                                scale=None, reduction: str = "sum") -> torch.Tensor:
+    """``distillation_loss`` in plain PyTorch: any device, differentiable by autograd, in at least fp32 (an fp64
+    student stays fp64).  The definition the kernels are tested against and the CPU path of the model."""
+    z = logits.to(torch.promote_types(logits.dtype, torch.float32)).flatten(0, -2)
+    n, v = z.shape
+    ids = teacher_ids.reshape(n, -1).long()
+    there = (ids >= 0) & (ids < v)
+    at = torch.where(there, ids, 0)
+    a = (teacher_logits.reshape(n, -1).to(z.dtype) / temperature).masked_fill(~there, -math.inf)
+    top = a.amax(1)
+    some = there.any(1) & (top > -math.inf) if teacher_lse is None else there.any(1)
+    norm = torch.logsumexp(a, 1) if teacher_lse is None else teacher_lse.reshape(n).to(z.dtype)
+    logp = a - torch.where(some, norm, 0)[:, None]
+    p = logp.exp()
+    logq = torch.log_softmax(z / temperature, 1)
+    kl = torch.where(p > 0, p * (logp - logq.gather(1, at)), 0).sum(1)
+    if teacher_lse is not None:
+        listed = torch.zeros(n, v + 1, dtype=torch.bool, device=z.device)
+        listed = listed.scatter_(1, torch.where(there, ids, v), True)[:, :v]
+        m = torch.where(some & ~listed.all(1), 1 - p.sum(1), 0)
+        counts = m > 2.0 ** -20  # what rounding leaves of 1 - sum p is no mass
+        rest = torch.logsumexp(logq.masked_fill(listed, -math.inf), 1)
+        kl = kl + torch.where(counts, m * (m.clamp_min(2.0 ** -20).log() - torch.where(counts, rest, 0)), 0)
+    loss = kd_weight * temperature ** 2 * kl
+    if targets is not None:
+        y = targets.reshape(n)
+        live = (y >= 0) & (y < v)
+        if ce_weight:
+            ce = torch.log_softmax(z, 1).gather(1, torch.where(live, y, 0)[:, None]).squeeze(1)
+            loss = loss - ce_weight * ce
+        loss = torch.where(live, loss, 0)
+    elif ce_weight:
+        raise ValueError("distillation_loss: the cross-entropy term needs targets")
+    if scale is not None:
+        loss = loss * scale
+    return loss.sum() if reduction == "sum" else loss.view(logits.shape[:-1])

@@ -405,6 +405,81 @@ class LinearCEFn(torch.autograd.Function):
         return dx, None, None, None, None, None, gw
 
 
+# ============================================================================ fused linear + distillation
+class LinearDistillFn(torch.autograd.Function):
+    """Summed distillation loss (ops/distill.py) of (alpha * x W[:V]^T) against a teacher's lists, chunked over rows.
+
+    Per chunk the logits GEMM writes fp32 logits and one pass over them forms the row losses and, while these
+    fit in ``KEEP_BYTES``, the bf16 gradient of the logits, which is all that is kept.  Otherwise the backward runs
+    both once more.  dx = dlogits W and dW += dlogits^T x follow."""
+
+    KEEP_BYTES = 8 << 30
+
+    @staticmethod
+    def forward(ctx, x, targets, ids, t, lse, group, V, alpha, chunk, tau, kd, ce, scale, weight):
+        w16 = group.bf16()
+        N, Vp = x.shape[0], w16.shape[0]
+        grad = any(ctx.needs_input_grad)
+        keep = grad and N * Vp * 2 <= LinearDistillFn.KEEP_BYTES
+        dz = torch.empty(N, Vp, device=x.device, dtype=torch.bfloat16) if keep else None
+        total = torch.zeros((), device=x.device, dtype=torch.float32)
+        z = torch.empty(min(chunk, N), Vp, device=x.device, dtype=torch.float32)
+        for s in range(0, N, chunk):
+            e = min(N, s + chunk)
+            _mm(x[s:e], w16.t(), z[: e - s], alpha=alpha)
+            total += lib().distill_loss(z[: e - s, :V], ids[s:e], t[s:e], lse[s:e] if lse is not None else None,
+                                        targets[s:e], tau, kd, ce, scale, dz[s:e] if keep else None).sum()
+        if grad:
+            ctx.save_for_backward(x, targets, ids, t, lse, scale)
+        ctx.group, ctx.dz, ctx.args = group, dz, (V, alpha, chunk, tau, kd, ce)
+        return total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, targets, ids, t, lse, scale = ctx.saved_tensors
+        V, alpha, chunk, tau, kd, ce = ctx.args
+        group, dz = ctx.group, ctx.dz
+        ctx.dz = None
+        w16 = group.bf16()
+        N, Vp = x.shape[0], w16.shape[0]
+        g32 = g.detach().float().reshape(1).contiguous()
+        dx = torch.empty(N, x.shape[1], device=x.device, dtype=torch.float32)
+        z = d = None
+        if dz is None:
+            z = torch.empty(min(chunk, N), Vp, device=x.device, dtype=torch.float32)
+            d = torch.empty(min(chunk, N), Vp, device=x.device, dtype=torch.bfloat16)
+
+        def compute(out, beta):
+            for s in range(0, N, chunk):
+                e = min(N, s + chunk)
+                if dz is None:
+                    part = d[: e - s]
+                    _mm(x[s:e], w16.t(), z[: e - s], alpha=alpha)
+                    lib().distill_loss(z[: e - s, :V], ids[s:e], t[s:e], lse[s:e] if lse is not None else None,
+                                       targets[s:e], tau, kd, ce, scale, part)
+                else:
+                    part = dz[s:e]
+                lib().scale_rows_(part, g32)
+                _mm(part, w16, dx[s:e], alpha=alpha)
+                _mm(part.t(), x[s:e], out, c=out, alpha=alpha, beta=beta if s == 0 else 1.0)
+
+        (gw,) = group.sink_grad(compute)
+        return (dx,) + (None,) * 12 + (gw,)
+
+
+def linear_distillation(x, targets, group, V, teacher, alpha=1.0, chunk=8192, scale=None):
+    """``teacher``: a ``distill.Teacher`` whose lists cover x's rows; ``targets`` below 0 leave rows out; ``scale``: a
+    one-element fp32 tensor that multiplies loss and gradient."""
+    n = x.shape[0]
+    k = teacher.ids.shape[-1]
+    lse = teacher.lse.reshape(n).float().contiguous() if teacher.lse is not None else None
+    return LinearDistillFn.apply(x.contiguous(), targets.contiguous().view(-1), teacher.ids.reshape(n, k).contiguous(),
+                                 teacher.values.reshape(n, k).contiguous(), lse, group, int(V), float(alpha), int(chunk),
+                                 float(teacher.temperature), float(teacher.kd_weight), float(teacher.ce_weight),
+                                 scale.detach().reshape(1).float() if scale is not None else None, group.params[0])
+
+
 def linear_cross_entropy(x, targets, group, V, alpha=1.0, chunk=8192):
     return LinearCEFn.apply(x.contiguous(), targets.contiguous().view(-1), group, int(V), float(alpha), int(chunk),
                             group.params[0])
