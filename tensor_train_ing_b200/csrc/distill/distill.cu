@@ -18,11 +18,16 @@
 // special-function unit gives 16 a cycle and SM, and two more per element would bound 16-bit logits), else (1) by
 // another exponential.
 #include "../common/host.h"
-#include "distill_api.h"
-#include "row_slice.cuh"
+#include "distill_common.cuh"
 
 namespace ttb {
 namespace {
+
+using distill::get_mark;
+using distill::Params;
+using distill::put_mark;
+using distill::teacher_logit;
+using distill::zero_row;
 
 using rows::Slice;
 namespace cg = cooperative_groups;
@@ -47,27 +52,6 @@ struct Shared {
   int again, repeats, target_listed, listed;
 };
 
-struct Params {
-  int vocab, k, per, parts, dz_cols;
-  bool ids64;
-  float inv_tau, tau, kd, ce;
-  const void* ids;
-  const void* t;
-  ScalarType t_type;
-  const float* teacher_lse;
-  const long long* targets;
-  const float* scale;
-  float* loss;
-  long long ldz, lddz;
-  uint32_t* status;
-};
-
-__device__ __forceinline__ float teacher_logit(const Params& p, long long i) {
-  if (p.t_type == ScalarType::kF32) return static_cast<const float*>(p.t)[i];
-  if (p.t_type == ScalarType::kBF16) return to_f32(static_cast<const __nv_bfloat16*>(p.t)[i]);
-  return to_f32(static_cast<const __half*>(p.t)[i]);
-}
-
 // Entry i of the shared-memory copy of the teacher's list.
 struct Entry {
   int col;      // -1: absent
@@ -75,51 +59,6 @@ struct Entry {
   float z;      // the student's logit at col
   int owner;    // whether this entry stands for its column here (the first CTA-local entry with this column)
 };
-
-// The smem element a listed column's slot holds while entries compete for it, as bits of a finite value.
-template <typename T>
-__device__ __forceinline__ void put_mark(T* p, int i) {
-  if constexpr (sizeof(T) == 4) *reinterpret_cast<int*>(p) = i;
-  else *reinterpret_cast<unsigned short*>(p) = static_cast<unsigned short>(i);
-}
-template <typename T>
-__device__ __forceinline__ int get_mark(const T* p) {
-  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const int*>(p);
-  else return *reinterpret_cast<const unsigned short*>(p);
-}
-
-// Threads first, first + step, ... write the row's zeros: 16 bytes each between the ragged ends.
-template <typename T>
-__device__ __forceinline__ void zero_row(T* row, int cols, int first, int step) {
-  constexpr int E = 16 / static_cast<int>(sizeof(T));
-  const int head = min(cols, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(T)));
-  const int vecs = (cols - head) / E;
-  for (int i = first; i < head; i += step) row[i] = from_f32<T>(0.f);
-  for (int i = first; i < vecs; i += step) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
-  for (int i = head + vecs * E + first; i < cols; i += step) row[i] = from_f32<T>(0.f);
-}
-
-// The reference at temperature 1 that goes with `ref` at tau: with e^POW for the exponentials, exactly POW times it.
-template <int POW>
-__device__ __forceinline__ rows::Ref ref_at_one(const rows::Ref& ref) {
-  if constexpr (POW == 1) return rows::Ref(ref.z, CUDART_L2E_F);
-  rows::Ref r = ref;
-  if constexpr (POW > 1) r.r = POW * ref.r;
-  return r;
-}
-// exp(z - reference) of a pair of logits, from e = exp((z - reference) / tau) where POW says so.
-template <int POW, bool FAR>
-__device__ __forceinline__ float2 at_one(float2 e, float2 z, const rows::Ref& ref1) {
-  if constexpr (POW == 2) {
-    return rows::mul2(e, e);
-  } else if constexpr (POW == 4) {
-    const float2 sq = rows::mul2(e, e);
-    return rows::mul2(sq, sq);
-  } else {
-    return rows::exp2_pair(
-        rows::log2_pair<FAR>(z, rows::both(CUDART_L2E_F), rows::both(FAR ? -ref1.z : -ref1.r)));
-  }
-}
 
 template <typename TZ, typename TG, bool GRAD, int POW>
 __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __restrict__ z,
@@ -208,7 +147,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   if (parts > 1) cluster.barrier_arrive();  // this CTA runs: its shared memory may be written
   mx = warp_max(lane < warps ? sh.red_max[lane] : -CUDART_INF_F);
   const float c = p.inv_tau * CUDART_L2E_F, c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
-  const rows::Ref ref(mx, c), ref1 = ref_at_one<POW>(ref);
+  const rows::Ref ref(mx, c), ref1 = rows::ref_at_one<POW>(ref);
 
   // Take the listed logits out of the slice.  Entries that share a column agree on one: the slot holds the number
   // of its last writer until that one puts -inf there (no number has -inf's bits).
@@ -244,7 +183,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
           acc[i & 1] = rows::add2(acc[i & 1], e);
           if constexpr (POW == 2) acc1[i & 1] = rows::fma2(e, e, acc1[i & 1]);
           if constexpr (POW == 1 || POW == 4)
-            acc1[i & 1] = rows::add2(acc1[i & 1], at_one<POW, FAR>(e, q[i], ref1));
+            acc1[i & 1] = rows::add2(acc1[i & 1], rows::at_one<POW, FAR>(e, q[i], ref1));
         }
       });
     });
@@ -277,13 +216,13 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   if (parts > 1) cluster.sync();
 
   // The row's scalars, by the first warp of every CTA, the parts in the same order.
-  rows::Ref top(0.f, c), top1 = ref_at_one<POW>(top);
+  rows::Ref top(0.f, c), top1 = rows::ref_at_one<POW>(top);
   float S = 0.f, total = 0.f, total1 = 0.f, m = 0.f;
   // What the gradient needs, and the loss, from the rest's sum relative to `at` and the logarithm of the rest's probability.
   auto finish = [&](const rows::Ref& at, float rest_sum, float log_rest) {
     const float scale = p.scale != nullptr ? *p.scale : 1.f;
     const float mass = sh.mass + m;
-    const rows::Ref at1 = ref_at_one<POW>(at);
+    const rows::Ref at1 = rows::ref_at_one<POW>(at);
     if (lane == 0) {
       float A = mass != 0.f ? mass * exp2f(top.log2_of(at, c)) / total : 0.f;
       if (m > 0.f && rest_sum > 0.f) A -= m / rest_sum;
@@ -423,7 +362,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
         else if constexpr (POW == 2)
           r = rows::mul2(e, rows::fma2(e, B2, A2));
         else
-          r = rows::fma2(at_one<POW, FAR>(e, q[i], at1), B2, rows::mul2(e, A2));
+          r = rows::fma2(rows::at_one<POW, FAR>(e, q[i], at1), B2, rows::mul2(e, A2));
         g[2 * i] = r.x;
         g[2 * i + 1] = r.y;
       }
@@ -512,6 +451,7 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   p.lddz = a.lddz;
   p.status = a.status;
   const int pow = a.ce == 0.f || a.tau == 1.f ? 0 : a.tau == 2.f ? 2 : a.tau == 4.f ? 4 : 1;
+  if (plan.parts == 1 && distill::loss_by_ring(a, p, pow, stream)) return;
   const size_t smem = plan.slice_bytes + a.k * sizeof(Entry);
   auto launch = [&](auto kernel, auto* z, auto* dz) {
     TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
@@ -528,30 +468,16 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
     cfg.numAttrs = plan.parts > 1 ? 1 : 0;
     TTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, z, dz, p));
   };
-  with_type(a.z_type, [&](auto* tz) {
-    using TZ = std::remove_pointer_t<decltype(tz)>;
-      auto with_grad = [&](auto* tg) {
-        using TG = std::remove_pointer_t<decltype(tg)>;
-        const auto* zp = static_cast<const TZ*>(a.z);
-        auto* gp = static_cast<TG*>(a.dz);
-        auto with_pow = [&](auto w) {
-          constexpr int POW = decltype(w)::value;
-          if (gp == nullptr)
-            launch(distill_kernel<TZ, TG, false, POW>, zp, gp);
-          else
-            launch(distill_kernel<TZ, TG, true, POW>, zp, gp);
-        };
-        switch (pow) {
-          case 0: return with_pow(std::integral_constant<int, 0>{});
-          case 1: return with_pow(std::integral_constant<int, 1>{});
-          case 2: return with_pow(std::integral_constant<int, 2>{});
-          default: return with_pow(std::integral_constant<int, 4>{});
-        }
-      };
-      if (a.dz != nullptr && a.dz_type != a.z_type)
-        with_grad(static_cast<__nv_bfloat16*>(nullptr));
+  distill::with_kernel_types(a, [&](const auto* z, auto* dz) {
+    using TZ = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
+    using TG = std::remove_pointer_t<decltype(dz)>;
+    distill::with_pow(pow, [&](auto w) {
+      constexpr int POW = decltype(w)::value;
+      if (dz == nullptr)
+        launch(distill_kernel<TZ, TG, false, POW>, z, dz);
       else
-        with_grad(static_cast<TZ*>(nullptr));
+        launch(distill_kernel<TZ, TG, true, POW>, z, dz);
+    });
   });
 }
 

@@ -1,0 +1,519 @@
+// The distillation loss where a CTA holds a row and there are many rows: a persistent kernel whose warps have roles, so that
+// no step of a row waits for another row's memory latency.
+//
+//   consumers  sum the row as it arrives, then (gradient) write exp((z - R) / tau) A + exp(z - R) B over it
+//   producer   keeps the row's stages coming: a stage of the next row as soon as the consumers are done with it
+//   lister     reads the teacher's list of the next row, and the student's logits at it, while this row is worked on
+//   patcher    takes the listed columns out of each stage as it arrives (replaces them by -inf)
+//   finisher   turns the sums into the loss and the gradient's scalars, and writes the listed columns' gradient
+//
+// What they hand over is double-buffered by row; every hand-over is an mbarrier with bounded waits, and a wait that runs
+// out ends all roles.  The arithmetic is that of distill.cu, of which this is the form for long rows: 4096 rows of 50257
+// bf16 logits, the loss alone, took 142 us there, with two CTAs of an SM each waiting through about 6 us of latencies per
+// row, and {EVAL} us here; loss and gradient of 8192 rows at tau 2 took 422 us and {TRAIN} us.
+#include "../common/host.h"
+#include "distill_common.cuh"
+#include "row_ring.cuh"
+
+namespace ttb {
+namespace distill {
+namespace {
+
+using rows::Ref;
+using rows::Span;
+using rows::kRingThreads;
+using rows::kRingWarps;
+using rows::kStages;
+
+constexpr int kThreads = 512;
+constexpr int kProducer = kRingWarps, kLister = kRingWarps + 1, kPatcher = kRingWarps + 2, kFinisher = kRingWarps + 3;
+static_assert(kFinisher == kThreads / 32 - 1);
+
+struct Listed {
+  int col;        // -1: absent
+  float logp, p;  // log p_i and p_i (0: no mass)
+  float z;        // the student's logit at col
+  int stage;      // that brings col; kStages: an edge column
+  int owner;      // the one entry that stands for its column
+};
+
+struct Row {  // what the lister says about a row
+  long long row;  // -1: no more rows
+  int live, target;
+  float mass, rest, target_logit, list_top;
+  unsigned edges;  // listed edge columns, by slot
+  int off;         // of the row from the 16-byte boundary before it, in elements
+  int repeats, target_listed;
+};
+
+struct Scalars {
+  float at, A, B;
+};
+
+struct Shared {
+  uint64_t full[kStages], ready[kStages], empty[kStages];
+  uint64_t list_ready[2], side_free[2], sums_ready[2], scalars_ready[2], gradient_done[2];
+  Row row[2];
+  Scalars scalars[2];
+  rows::WarpSum sums[2][kRingWarps];
+  int stop;
+};
+
+// Whether the barrier's phase completed; false when it, or a wait of another role, ran out.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, int parity, Shared& sh, uint32_t* status) {
+  bool ok = mbar_test(bar, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    while (!(ok = mbar_test(bar, parity))) {
+      if (*reinterpret_cast<volatile int*>(&sh.stop) != 0) break;
+      if (clock64() - t0 > kWaitLimitCycles) {
+        record_error(status, kErrTimeoutProducer);
+        *reinterpret_cast<volatile int*>(&sh.stop) = 1;
+        break;
+      }
+    }
+  }
+  return ok;
+}
+__device__ __forceinline__ bool warp_waits(uint64_t* bar, int parity, Shared& sh, uint32_t* status) {
+  return __all_sync(0xffffffffu, wait_for(bar, parity, sh, status));
+}
+__device__ __forceinline__ void warp_arrives(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+__device__ __forceinline__ bool counts(const Params& p, long long row, long long& target) {
+  target = p.targets != nullptr ? p.targets[row] : 0;
+  return target >= 0 && target < p.vocab;
+}
+
+template <typename TZ>
+__device__ __forceinline__ void produce(const TZ* z, TZ* sm, Shared& sh, const Params& p) {
+  long long target;
+  bool live = blockIdx.x < p.rows && counts(p, blockIdx.x, target);
+  int turn = 0;
+  bool ok = true;
+  for (long long row = blockIdx.x; row < p.rows && ok; row += gridDim.x) {
+    const bool now = live;
+    if (row + gridDim.x < p.rows) live = counts(p, row + gridDim.x, target);
+    if (!now) continue;
+    const Span<TZ> s(z + row * p.ldz, p.vocab);
+    for (int g = 0; g < kStages && ok; ++g) {
+      if (turn > 0) ok = wait_for(&sh.empty[g], (turn - 1) & 1, sh, p.status);
+      if (ok) s.load_stage(sm, sh.full, g);
+    }
+    ++turn;
+  }
+  if (!ok)  // copies under way end before the CTA does
+    for (int g = 0; g < kStages; ++g)
+      if (turn > 0) mbar_wait(&sh.full[g], (turn - 1) & 1, p.status, kErrTimeoutProducer);
+}
+
+template <typename TZ>
+__device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh, const Params& p) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (long long row = blockIdx.x;; row += gridDim.x, ++n) {
+    const int side = n & 1;
+    if (n >= 2 && !warp_waits(&sh.side_free[side], ((n >> 1) - 1) & 1, sh, p.status)) return;
+    Row& r = sh.row[side];
+    if (row >= p.rows) {
+      if (lane == 0) r.row = -1;
+      warp_arrives(&sh.list_ready[side]);
+      return;
+    }
+    long long target;
+    const bool live = counts(p, row, target);
+    if (!live) {
+      if (lane == 0) {
+        if (target >= p.vocab) record_error(p.status, kErrBadIndex);
+        r.row = row;
+        r.live = 0;
+      }
+      warp_arrives(&sh.list_ready[side]);
+      continue;
+    }
+    if (p.targets == nullptr) target = -1;
+    const Span<TZ> s(z + row * p.ldz, p.vocab);
+    Listed* list = lists + side * p.k;
+    float top = -CUDART_INF_F, list_top = -CUDART_INF_F;
+    bool present = false, has_target = false;
+    for (int i = lane; i < p.k; i += 32) {
+      long long col = p.ids64 ? static_cast<const long long*>(p.ids)[row * p.k + i]
+                              : static_cast<const int*>(p.ids)[row * p.k + i];
+      const float a = teacher_logit(p, row * p.k + i) * p.inv_tau;
+      if (col >= p.vocab) {
+        record_error(p.status, kErrBadIndex);
+        col = -1;
+      }
+      Listed e;
+      e.col = col < 0 ? -1 : static_cast<int>(col);
+      e.logp = col < 0 ? -CUDART_INF_F : a;
+      e.p = 0.f;
+      e.z = col < 0 ? 0.f : to_f32(s.row[col]);
+      e.stage = col < 0 ? -1 : s.stage_of(e.col);
+      e.owner = 0;
+      list[i] = e;
+      top = fmaxf(top, e.logp);
+      if (col >= 0) list_top = fmaxf(list_top, e.z);
+      present |= col >= 0;
+      has_target |= col >= 0 && col == target;
+    }
+    const float target_logit = p.ce != 0.f ? to_f32(s.row[target]) : 0.f;
+    present = __any_sync(0xffffffffu, present);
+    has_target = __any_sync(0xffffffffu, has_target);
+    top = warp_max(top);
+    list_top = warp_max(list_top);
+    // p_i = exp(a_i - base) / sum
+    float base = 0.f, inv = 1.f, log_sum = 0.f;
+    if (p.teacher_lse != nullptr) {
+      base = p.teacher_lse[row];
+    } else if (top != -CUDART_INF_F) {
+      base = top;
+      float e = 0.f;
+      for (int i = lane; i < p.k; i += 32) e += expf(list[i].logp - base);
+      e = warp_sum(e);
+      inv = 1.f / e;
+      log_sum = logf(e);
+    }
+    float mass = 0.f;
+    for (int i = lane; i < p.k; i += 32) {
+      const float a = list[i].logp - base;
+      list[i].logp = a - log_sum;
+      list[i].p = expf(a) * inv;
+      mass += list[i].p;
+    }
+    mass = warp_sum(mass);
+    if (lane == 0) {
+      const float rest = p.teacher_lse != nullptr && present ? 1.f - mass : 0.f;
+      r.row = row;
+      r.live = 1;
+      r.target = static_cast<int>(target);
+      r.mass = mass;
+      r.rest = rest > kDistillLeastRest ? rest : 0.f;
+      r.target_logit = target_logit;
+      r.list_top = fabsf(list_top) < CUDART_INF_F ? list_top : 0.f;
+      r.edges = 0u;
+      r.off = s.off;
+      r.repeats = 0;
+      r.target_listed = has_target;
+    }
+    __syncwarp();
+    for (int i = lane; i < p.k; i += 32) {  // edge columns are never in shared memory: they are settled here
+      if (list[i].stage != kStages) continue;
+      const unsigned bit = 1u << s.edge_slot(list[i].col);
+      const bool owner = !(atomicOr(&r.edges, bit) & bit);
+      list[i].owner = owner;
+      if (!owner) r.repeats = 1;
+    }
+    warp_arrives(&sh.list_ready[side]);
+  }
+}
+
+template <typename TZ>
+__device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, const Params& p) {
+  const int lane = threadIdx.x & 31;
+  int turn = 0;
+  for (int n = 0;; ++n) {
+    const int side = n & 1;
+    if (!warp_waits(&sh.list_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    Row& r = sh.row[side];
+    if (r.row < 0) return;
+    Listed* list = lists + side * p.k;
+    for (int g = 0; g < kStages && r.live; ++g) {
+      if (!warp_waits(&sh.full[g], turn & 1, sh, p.status)) return;
+      // Entries that share a column agree on one: the slot holds the number of its last writer until that one puts
+      // -inf there (no number has -inf's bits).  Element e of the row lies at e + off from the slice's start.
+      for (int i = lane; i < p.k; i += 32)
+        if (list[i].stage == g) put_mark(sm + list[i].col + r.off, i);
+      __syncwarp();
+      for (int i = lane; i < p.k; i += 32) {
+        if (list[i].stage != g) continue;
+        TZ* slot = sm + list[i].col + r.off;
+        const bool owner = get_mark(slot) == i;
+        list[i].owner = owner;
+        if (owner)
+          *slot = rows::neg_inf<TZ>();
+        else
+          r.repeats = 1;
+      }
+      fence_proxy_async_smem();  // before the stage's next copy
+      warp_arrives(&sh.ready[g]);
+    }
+    turn += r.live;
+    warp_arrives(&sh.side_free[side]);
+  }
+}
+
+template <typename TZ, typename TG, bool GRAD, int POW>
+__device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Shared& sh, const Params& p, float c,
+                                        float c1) {
+  constexpr int E = Span<TZ>::kVec;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int turn = 0, on_side[2] = {0, 0};
+  for (int n = 0;; ++n) {
+    const int side = n & 1;
+    if (!warp_waits(&sh.list_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    const long long row = sh.row[side].row;
+    if (row < 0) return;
+    TG* drow = GRAD ? dz + row * p.lddz : nullptr;
+    if (!sh.row[side].live) {
+      if (GRAD) zero_row(drow, p.dz_cols, tid, kRingThreads);
+      warp_arrives(&sh.sums_ready[side]);
+      continue;
+    }
+    const Span<TZ> s(z + row * p.ldz, p.vocab);
+    const int edge = tid < 16 ? s.edge_column(tid) : -1;
+    const float edge_z = edge >= 0 ? to_f32(s.row[edge]) : 0.f;
+
+    rows::Sums<POW> sums(c);
+#pragma unroll 1
+    for (int g = 0; g < kStages; ++g) {
+      if (!warp_waits(&sh.ready[g], turn & 1, sh, p.status)) return;
+      s.for_stage(sm, g, [&](const auto& u, int) {
+        sums.see(rows::max_of<TZ>(u), c);
+        sums.template add_batch<TZ>(u, c);
+      });
+      if (!GRAD) warp_arrives(&sh.empty[g]);
+    }
+    if (edge >= 0 && !((sh.row[side].edges >> tid) & 1u)) sums.add_one(edge_z, c);
+    const rows::WarpSum mine = rows::warp_total<POW>(sums, c, c1);
+    if (lane == 0) sh.sums[side][warp] = mine;
+    warp_arrives(&sh.sums_ready[side]);
+
+    if (GRAD) {
+      if (!warp_waits(&sh.scalars_ready[side], on_side[side] & 1, sh, p.status)) return;
+      const Scalars k = sh.scalars[side];
+      const Ref at(k.at, c), at1 = rows::ref_at_one<POW>(at);
+      const auto gradient = [&](float2 q, auto far) {
+        constexpr bool FAR = decltype(far)::value;
+        const float2 e = rows::exp2_pair(rows::log2_pair<FAR>(q, rows::both(c), rows::both(FAR ? -at.z : -at.r)));
+        if constexpr (POW == 0)
+          return rows::mul2(e, rows::both(k.A));
+        else if constexpr (POW == 2)
+          return rows::mul2(e, rows::fma2(e, rows::both(k.B), rows::both(k.A)));
+        else
+          return rows::fma2(rows::at_one<POW, FAR>(e, q, at1), rows::both(k.B), rows::mul2(e, rows::both(k.A)));
+      };
+      const bool same_vectors =
+          sizeof(TG) == sizeof(TZ)
+              ? (reinterpret_cast<uintptr_t>(drow) & 15) / sizeof(TG) == static_cast<uintptr_t>(s.off)
+              : s.off == 0 && (reinterpret_cast<uintptr_t>(drow) & (E * sizeof(TG) - 1)) == 0;
+      const auto stage = [&](int g, auto far) {
+        s.for_stage(sm, g, [&](const auto& u, int v) {
+          constexpr int N = sizeof(u) / sizeof(uint4);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            float2 q[E / 2];
+            rows::to_pairs<TZ>(u[i], q);
+            float out[E];
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j) {
+              const float2 o = gradient(q[j], far);
+              out[2 * j] = o.x;
+              out[2 * j + 1] = o.y;
+            }
+            TG* to = drow + s.first + (v + i * kRingThreads) * E;
+            if (same_vectors) {
+              store_vec<E>(to, out);
+            } else {
+#pragma unroll
+              for (int j = 0; j < E; ++j) to[j] = from_f32<TG>(out[j]);
+            }
+          }
+        });
+      };
+#pragma unroll 1
+      for (int g = 0; g < kStages; ++g) {
+        if (at.far)
+          stage(g, std::true_type{});
+        else
+          stage(g, std::false_type{});
+        warp_arrives(&sh.empty[g]);
+      }
+      if (edge >= 0) {
+        const float2 q = rows::both(edge_z);
+        drow[edge] = from_f32<TG>((at.far ? gradient(q, std::true_type{}) : gradient(q, std::false_type{})).x);
+      }
+      for (int i = p.vocab + tid; i < p.dz_cols; i += kRingThreads) drow[i] = from_f32<TG>(0.f);
+      warp_arrives(&sh.gradient_done[side]);
+    }
+    ++on_side[side];
+    ++turn;
+  }
+}
+
+template <typename TG, bool GRAD, int POW>
+__device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, const Params& p, float c, float c1) {
+  const int lane = threadIdx.x & 31;
+  const float scale = p.scale != nullptr ? *p.scale : 1.f;
+  int on_side[2] = {0, 0};
+  for (int n = 0;; ++n) {
+    const int side = n & 1;
+    if (!warp_waits(&sh.list_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    const Row& r = sh.row[side];
+    if (r.row < 0) return;
+    if (!warp_waits(&sh.sums_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    if (!r.live) {
+      if (lane == 0) p.loss[r.row] = 0.f;
+      warp_arrives(&sh.side_free[side]);
+      continue;
+    }
+    Listed* list = lists + side * p.k;
+    // the rest's sums, relative to its own reference
+    const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
+    const float rest_top = warp_max(w.z);
+    const bool some = rest_top != -CUDART_INF_F;
+    const Ref list_ref(r.list_top, c);
+    const Ref own(some ? rest_top : r.list_top, c), own1 = rows::ref_at_one<POW>(own);
+    const Ref of(w.z == -CUDART_INF_F ? 0.f : w.z, c);
+    const float S = warp_sum(w.sum != 0.f ? w.sum * exp2f(own.log2_of(of, c)) : 0.f);
+    const float S1 =
+        POW != 0 ? warp_sum(w.sum1 != 0.f ? w.sum1 * exp2f(own1.log2_of(rows::ref_at_one<POW>(of), c1)) : 0.f) : 0.f;
+    // the row's reference: the larger of the rest's and the list's
+    bool any = false;
+    for (int i = lane; i < p.k; i += 32) any |= list[i].owner != 0;
+    any = __any_sync(0xffffffffu, any);
+    const Ref ref(any && r.list_top > own.z ? r.list_top : own.z, c), ref1 = rows::ref_at_one<POW>(ref);
+    float L = 0.f, L1 = 0.f, listed = 0.f;
+    for (int i = lane; i < p.k; i += 32) {
+      if (!list[i].owner) continue;
+      L += exp2f(ref.log2_of(list[i].z, c));
+      if (POW != 0) L1 += exp2f(ref1.log2_of(list[i].z, c1));
+      listed += 1.f;
+    }
+    L = warp_sum(L);
+    if (POW != 0) L1 = warp_sum(L1);
+    const bool same = ref.z == own.z;
+    const float f = same ? 1.f : exp2f(ref.log2_of(own, c)), f1 = same ? 1.f : exp2f(ref1.log2_of(own1, c1));
+    const float total = S * f + L, total1 = POW != 0 ? S1 * f1 + L1 : total;
+    const float inv_sum = 1.f / total, inv_sum1 = 1.f / total1;
+    // a list that names every column leaves no rest, whatever rounding says
+    const float m = p.k >= p.vocab && static_cast<int>(warp_sum(listed)) >= p.vocab ? 0.f : r.rest;
+    const float mass = r.mass + m;
+    float A = mass != 0.f ? mass * f * inv_sum : 0.f;
+    if (m > 0.f && S > 0.f) A -= m / S;
+    A *= scale * p.kd * p.tau;
+    float B = p.ce != 0.f ? scale * p.ce * f1 * inv_sum1 : 0.f;
+    if (POW == 0) {  // one exponential serves both terms
+      A += B;
+      B = 0.f;
+    }
+    if (GRAD) {
+      if (lane == 0) sh.scalars[side] = Scalars{own.z, A, B};
+      warp_arrives(&sh.scalars_ready[side]);
+    }
+    const float log2_total = log2f(total);
+    float kl = 0.f;
+    for (int i = lane; i < p.k; i += 32) {
+      const float logq = (ref.log2_of(list[i].z, c) - log2_total) * CUDART_LN2_F;
+      if (list[i].p != 0.f) kl += list[i].p * (list[i].logp - logq);
+    }
+    kl = warp_sum(kl);
+    if (lane == 0) {
+      if (m > 0.f)  // log q_rest from its parts where the probability itself leaves fp32's range
+        kl += m * (f > 1e-30f ? logf(m / (S * f * inv_sum))
+                              : logf(m) - (logf(S) + (own.z - ref.z) * p.inv_tau - logf(total)));
+      float loss = p.kd != 0.f ? p.kd * p.tau * p.tau * kl : 0.f;
+      if (p.ce != 0.f) loss += p.ce * (log2f(total1) - ref1.log2_of(r.target_logit, c1)) * CUDART_LN2_F;
+      p.loss[r.row] = scale * loss;
+    }
+    if (GRAD) {
+      if (!warp_waits(&sh.gradient_done[side], on_side[side] & 1, sh, p.status)) return;
+      TG* drow = dz + r.row * p.lddz;
+      const float kd = scale * p.kd * p.tau, ce = scale * p.ce;
+      for (int i = lane; i < p.k; i += 32) {
+        if (!list[i].owner) continue;
+        const int col = list[i].col;
+        float share = list[i].p;
+        if (r.repeats) {
+          share = 0.f;
+          for (int j = 0; j < p.k; ++j)
+            if (list[j].col == col) share += list[j].p;
+        }
+        float g = kd != 0.f ? kd * (exp2f(ref.log2_of(list[i].z, c)) * inv_sum * mass - share) : 0.f;
+        if (ce != 0.f) g += ce * (exp2f(ref1.log2_of(list[i].z, c1)) * inv_sum1 - (col == r.target ? 1.f : 0.f));
+        drow[col] = from_f32<TG>(g);
+      }
+      if (lane == 0 && ce != 0.f && !r.target_listed) {
+        float g = rows::fast_exp2(own.log2_of(r.target_logit, c)) * A - ce;
+        if (POW != 0) g += rows::fast_exp2(own1.log2_of(r.target_logit, c1)) * B;
+        drow[r.target] = from_f32<TG>(g);
+      }
+    }
+    ++on_side[side];
+    warp_arrives(&sh.side_free[side]);
+  }
+}
+
+template <typename TZ, typename TG, bool GRAD, int POW>
+__global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __restrict__ z, TG* __restrict__ dz,
+                                                                  const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ Shared sh;
+  TZ* sm = reinterpret_cast<TZ*>(smem);
+  auto* lists = reinterpret_cast<Listed*>(smem + static_cast<size_t>(p.per) * 16);
+  if (threadIdx.x == 0) {
+    for (int g = 0; g < kStages; ++g) {
+      mbar_init(&sh.full[g], 1);
+      mbar_init(&sh.ready[g], 1);
+      mbar_init(&sh.empty[g], kRingWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.list_ready[i], 1);
+      mbar_init(&sh.side_free[i], 2);  // finisher and patcher: the roles that nothing else makes wait for a dead row
+      mbar_init(&sh.sums_ready[i], kRingWarps);
+      mbar_init(&sh.scalars_ready[i], 1);
+      mbar_init(&sh.gradient_done[i], kRingWarps);
+    }
+    sh.stop = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const float c = p.inv_tau * CUDART_L2E_F, c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
+  const int warp = threadIdx.x >> 5;
+  if (warp < kRingWarps) {
+    consume<TZ, TG, GRAD, POW>(z, dz, sm, sh, p, c, c1);
+  } else if (warp == kProducer) {
+    if ((threadIdx.x & 31) == 0) produce(z, sm, sh, p);
+  } else if (warp == kLister) {
+    list_rows(z, lists, sh, p);
+  } else if (warp == kPatcher) {
+    patch_stages(sm, lists, sh, p);
+  } else {
+    finish_rows<TG, GRAD, POW>(dz, lists, sh, p, c, c1);
+  }
+}
+
+}  // namespace
+
+bool loss_by_ring(const DistillArgs& a, const Params& params, int pow, cudaStream_t stream) {
+  constexpr size_t kLeastSlice = 16 * 1024;            // below, several rows per SM hide each other's latencies
+  constexpr size_t kMostBytes = 112 * 1024;            // two CTAs on an SM
+  const size_t slice = static_cast<size_t>(params.per) * 16;
+  const size_t smem = slice + 2 * static_cast<size_t>(a.k) * sizeof(Listed);
+  if (slice < kLeastSlice || smem + sizeof(Shared) + 1024 > kMostBytes || a.rows < 4LL * num_sms()) return false;
+  Params p = params;
+  p.rows = a.rows;
+  auto launch = [&](auto kernel, auto* z, auto* dz) {
+    TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    kernel<<<2 * num_sms(), kThreads, smem, stream>>>(z, dz, p);
+    TTB_CUDA_CHECK(cudaGetLastError());
+  };
+  with_kernel_types(a, [&](const auto* z, auto* dz) {
+    using TZ = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
+    using TG = std::remove_pointer_t<decltype(dz)>;
+    with_pow(pow, [&](auto w) {
+      constexpr int POW = decltype(w)::value;
+      if (dz == nullptr)
+        launch(distill_ring_kernel<TZ, TG, false, POW>, z, dz);
+      else
+        launch(distill_ring_kernel<TZ, TG, true, POW>, z, dz);
+    });
+  });
+  return true;
+}
+
+}  // namespace distill
+}  // namespace ttb

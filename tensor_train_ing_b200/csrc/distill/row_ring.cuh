@@ -1,0 +1,214 @@
+// A row of logits in the shared memory of a CTA whose warps have roles: `kRingThreads` consumer threads work on rows
+// that other warps bring in and finish.
+//
+// A row is cut into 16-byte vectors counted from the 16-byte boundary at or below its first element, so that
+// rows at any element offset are copied in whole aligned vectors; the at most two vectors that reach over the
+// row's ends are its edges and are read from global memory element by element.  Consumer thread t works on the whole
+// vectors lo + t, lo + t + kRingThreads, ...  They arrive in kStages bulk copies with a barrier each, and a stage's memory is
+// given to the CTA's next row as soon as the last pass over it is done.
+#pragma once
+
+#include "row_slice.cuh"
+
+namespace ttb {
+namespace rows {
+
+constexpr int kRingWarps = 12;
+constexpr int kRingThreads = 32 * kRingWarps;
+
+template <typename T>
+struct Span {
+  static constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  const T* row;
+  int columns;
+  int first;   // column of vector 0 (negative where that vector starts before the row)
+  int lo, hi;  // the whole vectors: [lo, hi)
+  int off;     // elements between the 16-byte boundary and the row's first element
+  int rounds;  // whole vectors that every thread has; the threads below hi - lo - rounds * threads have one more
+  int stage;   // rounds per stage
+
+  __device__ __forceinline__ Span(const T* r, int cols) {
+    constexpr int E = kVec;
+    row = r;
+    off = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
+    const int nv = (off + cols + E - 1) / E;
+    columns = cols;
+    first = -off;
+    lo = off > 0 ? 1 : 0;
+    hi = max(lo, nv * E - off > cols ? nv - 1 : nv);
+    rounds = (hi - lo) / kRingThreads;
+    stage = rounds / kStages + 1;
+  }
+  __device__ __forceinline__ int vector_of(int col) const { return (col + off) / kVec; }
+  // The stage that brings a column, or kStages for an edge column.
+  __device__ __forceinline__ int stage_of(int col) const {
+    const int v = vector_of(col);
+    return v >= lo && v < hi ? (v - lo) / (stage * kRingThreads) : kStages;
+  }
+  // Edge columns have slots 0..7 (before the first whole vector) and 8..15 (after the last); -1 for no column.
+  __device__ __forceinline__ int edge_slot(int col) const {
+    return col < first + lo * kVec ? col : 8 + col - (first + hi * kVec);
+  }
+  __device__ __forceinline__ int edge_column(int slot) const {
+    const int head = min(columns, first + lo * kVec), tail = max(head, first + hi * kVec);
+    const int col = slot < 8 ? slot : tail + slot - 8;
+    return slot < 8 ? (col < head ? col : -1) : (col < columns ? col : -1);
+  }
+  // One thread: starts the copy of stage g into `sm`.
+  __device__ __forceinline__ void load_stage(T* sm, uint64_t* bars, int g) const {
+    const int a = lo + g * stage * kRingThreads;
+    const int b = min(hi, a + stage * kRingThreads);
+    if (a < b) {
+      mbar_arrive_expect_tx(&bars[g], (b - a) * 16);
+      bulk_load(sm + a * kVec, row + first + a * kVec, (b - a) * 16, &bars[g]);
+    } else {
+      mbar_arrive(&bars[g]);
+    }
+  }
+  // f(vectors, first vector number) over the thread's vectors of stage g: two (threads apart) at a time, then one.
+  template <typename F>
+  __device__ __forceinline__ void for_stage(const T* sm, int g, F&& f) const {
+    const int step = kRingThreads, end = min((g + 1) * stage, rounds);
+    int i = g * stage, v = lo + threadIdx.x + i * step;
+    for (; i + 2 <= end; i += 2, v += 2 * step) {
+      uint4 u[2] = {*reinterpret_cast<const uint4*>(sm + v * kVec),
+                    *reinterpret_cast<const uint4*>(sm + (v + step) * kVec)};
+      f(u, v);
+    }
+    // the stage's odd round, and in the stage that has it the round that only some threads have
+    const int last = min((g + 1) * stage, rounds + 1);
+    for (; i < last && v < hi; ++i, v += step) {
+      uint4 u[1] = {*reinterpret_cast<const uint4*>(sm + v * kVec)};
+      f(u, v);
+    }
+  }
+};
+
+// The elements of a vector as pairs.
+template <typename T>
+__device__ __forceinline__ void to_pairs(const uint4& u, float2 (&p)[Span<T>::kVec / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    p[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    p[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  } else {
+    unpack2<T>(u.x, p[0].x, p[0].y);
+    unpack2<T>(u.y, p[1].x, p[1].y);
+    unpack2<T>(u.z, p[2].x, p[2].y);
+    unpack2<T>(u.w, p[3].x, p[3].y);
+  }
+}
+
+// The largest element of some vectors (NaN left out).
+template <typename T, int N>
+__device__ __forceinline__ float max_of(const uint4 (&u)[N]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u[i].x), __uint_as_float(u[i].y)),
+                         fmaxf(__uint_as_float(u[i].z), __uint_as_float(u[i].w))));
+    return m;
+  } else {
+    uint32_t m = max2<T>(max2<T>(u[0].x, u[0].y), max2<T>(u[0].z, u[0].w));
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = max2<T>(m, max2<T>(max2<T>(u[i].x, u[i].y), max2<T>(u[i].z, u[i].w)));
+    float a, b;
+    unpack2<T>(m, a, b);
+    return fmaxf(fmaxf(a, b), -CUDART_INF_F);  // two NaN halves give -inf
+  }
+}
+
+// A thread's running sums of exp((z - ref) / tau) and, for POW > 0, exp(z - ref), over whatever it has seen.  The
+// reference is the largest logit of its first batch and moves only when a batch exceeds it by more than 2^40, so
+// that almost no batch rescales anything and no sum can overflow.
+template <int POW>
+struct Sums {
+  Ref ref, ref1;
+  bool set;  // whether any finite logit has been seen; until then the reference is 0
+  float2 acc[2], acc1[2];
+
+  __device__ __forceinline__ explicit Sums(float c) : ref(0.f, c), ref1(0.f, c), set(false) {
+    acc[0] = acc[1] = acc1[0] = acc1[1] = both(0.f);
+  }
+  __device__ __forceinline__ void move(float logit, float c) {
+    const Ref next(logit, c), next1 = ref_at_one<POW>(next);
+    if (set) {
+      const float2 f = both(fast_exp2(next.log2_of(ref, c)));
+      acc[0] = mul2(acc[0], f);
+      acc[1] = mul2(acc[1], f);
+      if (POW != 0) {
+        const float c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
+        const float2 f1 = both(fast_exp2(next1.log2_of(ref1, c1)));
+        acc1[0] = mul2(acc1[0], f1);
+        acc1[1] = mul2(acc1[1], f1);
+      }
+    }
+    ref = next;
+    ref1 = next1;
+    set = true;
+  }
+  // before adding logits of which `top` is the largest
+  __device__ __forceinline__ void see(float top, float c) {
+    if ((!set || ref.log2_of(top, c) > 40.f) && fabsf(top) < CUDART_INF_F) move(top, c);
+  }
+  template <bool FAR>
+  __device__ __forceinline__ void add(float2 z, int i, float c) {
+    const float2 e = exp2_pair(log2_pair<FAR>(z, both(c), both(FAR ? -ref.z : -ref.r)));
+    acc[i & 1] = add2(acc[i & 1], e);
+    if constexpr (POW == 2) acc1[i & 1] = fma2(e, e, acc1[i & 1]);
+    if constexpr (POW == 1 || POW == 4) acc1[i & 1] = add2(acc1[i & 1], at_one<POW, FAR>(e, z, ref1));
+  }
+  template <typename T, bool FAR, int N>
+  __device__ __forceinline__ void add_vectors(const uint4 (&u)[N], float c) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float2 q[Span<T>::kVec / 2];
+      to_pairs<T>(u[n], q);
+#pragma unroll
+      for (int i = 0; i < Span<T>::kVec / 2; ++i) add<FAR>(q[i], i, c);
+    }
+  }
+  template <typename T, int N>
+  __device__ __forceinline__ void add_batch(const uint4 (&u)[N], float c) {
+    if (ref.far)
+      add_vectors<T, true>(u, c);
+    else
+      add_vectors<T, false>(u, c);
+  }
+  __device__ __forceinline__ void add_one(float z, float c) {
+    see(z, c);
+    const float2 pair = make_float2(z, -CUDART_INF_F);
+    if (ref.far)
+      add<true>(pair, 0, c);
+    else
+      add<false>(pair, 0, c);
+  }
+  __device__ __forceinline__ float sum() const { return (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y); }
+  __device__ __forceinline__ float sum1() const { return (acc1[0].x + acc1[0].y) + (acc1[1].x + acc1[1].y); }
+};
+
+// What a warp's threads have summed, relative to one reference (lane 0 has the sums).
+struct WarpSum {
+  float z;  // the reference logit; -inf where the warp has seen no finite logit
+  float sum, sum1;
+};
+template <int POW>
+__device__ __forceinline__ WarpSum warp_total(const Sums<POW>& s, float c, float c1) {
+  WarpSum w;
+  w.z = warp_max(s.set ? s.ref.z : -CUDART_INF_F);
+  const Ref ref(w.z == -CUDART_INF_F ? 0.f : w.z, c);
+  w.sum = s.sum();
+  if (w.sum != 0.f) w.sum *= fast_exp2(ref.log2_of(s.ref, c));
+  w.sum = warp_sum(w.sum);
+  w.sum1 = 0.f;
+  if (POW != 0) {
+    const Ref ref1 = ref_at_one<POW>(ref);
+    w.sum1 = s.sum1();
+    if (w.sum1 != 0.f) w.sum1 *= fast_exp2(ref1.log2_of(s.ref1, c1));
+    w.sum1 = warp_sum(w.sum1);
+  }
+  return w;
+}
+
+}  // namespace rows
+}  // namespace ttb

@@ -202,6 +202,28 @@ __device__ __forceinline__ float2 log2_pair(float2 q, float2 c, float2 n) {
 }
 __device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
 
+// The reference at temperature 1 that goes with `ref` at tau: with e^POW for the exponentials, exactly POW times it.
+template <int POW>
+__device__ __forceinline__ Ref ref_at_one(const Ref& ref) {
+  if constexpr (POW == 1) return Ref(ref.z, CUDART_L2E_F);
+  Ref r = ref;
+  if constexpr (POW > 1) r.r = POW * ref.r;
+  return r;
+}
+// exp(z - reference) of a pair of logits, from e = exp((z - reference) / tau) where POW says so.
+template <int POW, bool FAR>
+__device__ __forceinline__ float2 at_one(float2 e, float2 z, const Ref& ref1) {
+  if constexpr (POW == 2) {
+    return mul2(e, e);
+  } else if constexpr (POW == 4) {
+    const float2 sq = mul2(e, e);
+    return mul2(sq, sq);
+  } else {
+    return exp2_pair(
+        log2_pair<FAR>(z, both(CUDART_L2E_F), both(FAR ? -ref1.z : -ref1.r)));
+  }
+}
+
 // f(std::bool_constant<ref.far>): the passes are compiled for both kinds of row.
 template <typename F>
 __device__ __forceinline__ void by_kind(const Ref& ref, F&& f) {

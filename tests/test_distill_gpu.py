@@ -268,6 +268,54 @@ def test_loss_of_strided_and_misaligned_rows(dtype, offset, ld):
     _check_loss(z, ids.long(), t, lse, None, 1.0, 1.0, 0.0, 1.0)
 
 
+# Many rows of logits that one CTA holds: the persistent kernel.  Its CTAs take several rows each, with and without
+# left-out ones between them; odd widths and offsets give rows with edges on either side.
+@pytest.mark.parametrize("dtype,v,ld,offset", [(BF16, 8192, 8192, 0), (BF16, 9001, 9001, 3), (F16, 20011, 20032, 1),
+                                               (F32, 4100, 4100, 0), (F32, 12345, 12345, 2), (BF16, 50257, 50257, 0)])
+@pytest.mark.parametrize("k,rest,tau,ce", [(1, False, 1.0, 0.0), (40, True, 2.0, 0.5), (200, True, 1.5, 0.25),
+                                           (64, False, 4.0, 0.5)])
+def test_loss_of_many_rows(dtype, v, ld, offset, k, rest, tau, ce):
+    n = 601 if v > 30000 else 1201
+    z = _logits(n, v, dtype, v + k, ld=ld, offset=offset)
+    ids, t, lse = _teacher(z, k, F32, k, rest, tau)
+    ids[5:9] = -1
+    if k > 2:
+        ids[20, 0], ids[20, 1], ids[20, 2] = 0, v - 1, 0  # both ends of the row, and a column named twice
+        ids[21, :3] = 4099 % v
+    y = _targets(n, v, ids, 5)
+    y[torch.rand(n, device="cuda", generator=_gen(6)) < 0.3] = -100
+    y[30:330] = -100
+    y[20], y[22] = 0, v - 1
+    _check_loss(z, ids, t, lse, y if ce or v % 2 else None, tau, 0.9, ce, 0.5)
+
+
+def test_every_row_of_many_left_out():
+    z = _logits(800, 9001, BF16, 50)
+    ids, t, lse = _teacher(z, 8, F32, 51, True, 1.0)
+    _check_loss(z, ids, t, lse, torch.full((800,), -100, device="cuda"))
+
+
+def test_non_finite_rows_among_many():
+    z = _logits(700, 9001, F32, 52)
+    ids, t, lse = _teacher(z, 8, F32, 53, True, 1.0)
+    clean = _ops().distillation_loss(z, ids, t, lse, reduction="none")
+    bad = torch.zeros(700, dtype=torch.bool, device="cuda")
+    bad[[3, 299, 699]] = True
+    zz = z.clone()
+    zz[3, 1], zz[299, 9000], zz[699, 4000] = float("nan"), float("nan"), float("inf")
+    rows = _ops().distillation_loss(zz, ids, t, lse, reduction="none")
+    assert torch.equal(rows[~bad], clean[~bad]) and not torch.isfinite(rows[bad]).any()
+    low = z.clone()
+    low[:, 5000:] = torch.finfo(F32).min
+    low[10] = torch.finfo(F32).min  # a row at the lowest value throughout: uniform
+    _check_loss(torch.cat([low[:10], low[11:]]), torch.cat([ids[:10], ids[11:]]).clamp_max(4999),
+                torch.cat([t[:10], t[11:]]), torch.cat([lse[:10], lse[11:]]))
+    flat = low.clone()
+    flat[10] = 0
+    a = _ops().distillation_loss(low, ids, t, lse, reduction="none")[10]
+    assert a == _ops().distillation_loss(flat, ids, t, lse, reduction="none")[10]
+
+
 def test_types_of_the_list_mix():
     z = _logits(8, 3000, BF16, 6)
     for t_dtype in (F32, BF16, F16):
