@@ -7,7 +7,7 @@
 //   patcher    takes the listed columns out of each stage as it arrives (replaces them by -inf)
 //   finisher   turns the sums into the loss and the gradient's scalars, and writes the listed columns' gradient
 //
-// What they hand over is double-buffered by row; every hand-over is an mbarrier with bounded waits, and a wait that runs
+// What they hand over is kept for several rows; every hand-over is an mbarrier with bounded waits, and a wait that runs
 // out ends all roles.  The arithmetic is that of distill.cu, of which this is the form for long rows: 4096 rows of 50257
 // bf16 logits, the loss alone, took 142 us there, with two CTAs of an SM each waiting through about 6 us of latencies per
 // row, and {EVAL} us here; loss and gradient of 8192 rows at tau 2 took 422 us and {TRAIN} us.
@@ -28,13 +28,16 @@ using rows::kStages;
 constexpr int kThreads = 512;
 constexpr int kProducer = kRingWarps, kLister = kRingWarps + 1, kPatcher = kRingWarps + 2, kFinisher = kRingWarps + 3;
 static_assert(kFinisher == kThreads / 32 - 1);
+// Rows that are between their list and their end at one time: the lister runs up to three rows ahead, which covers its two
+// dependent reads of global memory and the finisher's turn before them.
+constexpr int kSides = 4;
 
 struct Listed {
   int col;        // -1: absent
   float logp, p;  // log p_i and p_i (0: no mass)
   float z;        // the student's logit at col
-  int stage;      // that brings col; kStages: an edge column
-  int owner;      // the one entry that stands for its column
+  short stage;    // that brings col; kStages: an edge column, -1: none
+  short owner;    // the one entry that stands for its column
 };
 
 struct Row {  // what the lister says about a row
@@ -52,10 +55,10 @@ struct Scalars {
 
 struct Shared {
   uint64_t full[kStages], ready[kStages], empty[kStages];
-  uint64_t list_ready[2], side_free[2], sums_ready[2], scalars_ready[2], gradient_done[2];
-  Row row[2];
-  Scalars scalars[2];
-  rows::WarpSum sums[2][kRingWarps];
+  uint64_t list_ready[kSides], side_free[kSides], sums_ready[kSides], scalars_ready[kSides], gradient_done[kSides];
+  Row row[kSides];
+  Scalars scalars[kSides];
+  rows::WarpSum sums[kSides][kRingWarps];
   int stop;
 };
 
@@ -115,8 +118,8 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
   const int lane = threadIdx.x & 31;
   int n = 0;
   for (long long row = blockIdx.x;; row += gridDim.x, ++n) {
-    const int side = n & 1;
-    if (n >= 2 && !warp_waits(&sh.side_free[side], ((n >> 1) - 1) & 1, sh, p.status)) return;
+    const int side = n % kSides;
+    if (n >= kSides && !warp_waits(&sh.side_free[side], (n / kSides - 1) & 1, sh, p.status)) return;
     Row& r = sh.row[side];
     if (row >= p.rows) {
       if (lane == 0) r.row = -1;
@@ -216,8 +219,8 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
   const int lane = threadIdx.x & 31;
   int turn = 0;
   for (int n = 0;; ++n) {
-    const int side = n & 1;
-    if (!warp_waits(&sh.list_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    const int side = n % kSides;
+    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, sh, p.status)) return;
     Row& r = sh.row[side];
     if (r.row < 0) return;
     Listed* list = lists + side * p.k;
@@ -251,10 +254,11 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
                                         float c1) {
   constexpr int E = Span<TZ>::kVec;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int turn = 0, on_side[2] = {0, 0};
+  int turn = 0;
+  unsigned on_side = 0;  // bit s: the parity of the live rows side s has had
   for (int n = 0;; ++n) {
-    const int side = n & 1;
-    if (!warp_waits(&sh.list_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    const int side = n % kSides;
+    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, sh, p.status)) return;
     const long long row = sh.row[side].row;
     if (row < 0) return;
     TG* drow = GRAD ? dz + row * p.lddz : nullptr;
@@ -283,7 +287,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
     warp_arrives(&sh.sums_ready[side]);
 
     if (GRAD) {
-      if (!warp_waits(&sh.scalars_ready[side], on_side[side] & 1, sh, p.status)) return;
+      if (!warp_waits(&sh.scalars_ready[side], (on_side >> side) & 1, sh, p.status)) return;
       const Scalars k = sh.scalars[side];
       const Ref at(k.at, c), at1 = rows::ref_at_one<POW>(at);
       const auto gradient = [&](float2 q, auto far) {
@@ -339,7 +343,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
       for (int i = p.vocab + tid; i < p.dz_cols; i += kRingThreads) drow[i] = from_f32<TG>(0.f);
       warp_arrives(&sh.gradient_done[side]);
     }
-    ++on_side[side];
+    on_side ^= 1u << side;
     ++turn;
   }
 }
@@ -348,49 +352,57 @@ template <typename TG, bool GRAD, int POW>
 __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, const Params& p, float c, float c1) {
   const int lane = threadIdx.x & 31;
   const float scale = p.scale != nullptr ? *p.scale : 1.f;
-  int on_side[2] = {0, 0};
+  int turn = 0;
+  unsigned on_side = 0;  // bit s: the parity of the live rows side s has had
   for (int n = 0;; ++n) {
-    const int side = n & 1;
-    if (!warp_waits(&sh.list_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    const int side = n % kSides;
+    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, sh, p.status)) return;
     const Row& r = sh.row[side];
     if (r.row < 0) return;
-    if (!warp_waits(&sh.sums_ready[side], (n >> 1) & 1, sh, p.status)) return;
+    Listed* list = lists + side * p.k;
+    // The list's sums, each column once, relative to its largest logit.  With a gradient, whose consumers wait for this
+    // warp, already while they sum the last stage (they then cannot run past that stage's phase; without one they can).
+    if (!GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, sh, p.status)) return;
+    const Ref list_ref(r.list_top, c), list_ref1 = rows::ref_at_one<POW>(list_ref);
+    float L = 0.f, L1 = 0.f, listed = 0.f;
+    if (r.live) {
+      if (GRAD && !warp_waits(&sh.ready[kStages - 1], turn & 1, sh, p.status)) return;
+      for (int i = lane; i < p.k; i += 32) {
+        if (!list[i].owner) continue;
+        L += exp2f(list_ref.log2_of(list[i].z, c));
+        if (POW != 0) L1 += exp2f(list_ref1.log2_of(list[i].z, c1));
+        listed += 1.f;
+      }
+      L = warp_sum(L);
+      if (POW != 0) L1 = warp_sum(L1);
+      listed = warp_sum(listed);
+    }
+    if (GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, sh, p.status)) return;
     if (!r.live) {
       if (lane == 0) p.loss[r.row] = 0.f;
       warp_arrives(&sh.side_free[side]);
       continue;
     }
-    Listed* list = lists + side * p.k;
     // the rest's sums, relative to its own reference
     const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
     const float rest_top = warp_max(w.z);
-    const bool some = rest_top != -CUDART_INF_F;
-    const Ref list_ref(r.list_top, c);
-    const Ref own(some ? rest_top : r.list_top, c), own1 = rows::ref_at_one<POW>(own);
+    const Ref own(rest_top != -CUDART_INF_F ? rest_top : r.list_top, c), own1 = rows::ref_at_one<POW>(own);
     const Ref of(w.z == -CUDART_INF_F ? 0.f : w.z, c);
     const float S = warp_sum(w.sum != 0.f ? w.sum * exp2f(own.log2_of(of, c)) : 0.f);
     const float S1 =
         POW != 0 ? warp_sum(w.sum1 != 0.f ? w.sum1 * exp2f(own1.log2_of(rows::ref_at_one<POW>(of), c1)) : 0.f) : 0.f;
     // the row's reference: the larger of the rest's and the list's
-    bool any = false;
-    for (int i = lane; i < p.k; i += 32) any |= list[i].owner != 0;
-    any = __any_sync(0xffffffffu, any);
-    const Ref ref(any && r.list_top > own.z ? r.list_top : own.z, c), ref1 = rows::ref_at_one<POW>(ref);
-    float L = 0.f, L1 = 0.f, listed = 0.f;
-    for (int i = lane; i < p.k; i += 32) {
-      if (!list[i].owner) continue;
-      L += exp2f(ref.log2_of(list[i].z, c));
-      if (POW != 0) L1 += exp2f(ref1.log2_of(list[i].z, c1));
-      listed += 1.f;
+    const Ref ref(listed > 0.f && r.list_top > own.z ? r.list_top : own.z, c), ref1 = rows::ref_at_one<POW>(ref);
+    if (listed > 0.f) {
+      L *= exp2f(ref.log2_of(list_ref, c));
+      if (POW != 0) L1 *= exp2f(ref1.log2_of(list_ref1, c1));
     }
-    L = warp_sum(L);
-    if (POW != 0) L1 = warp_sum(L1);
     const bool same = ref.z == own.z;
     const float f = same ? 1.f : exp2f(ref.log2_of(own, c)), f1 = same ? 1.f : exp2f(ref1.log2_of(own1, c1));
     const float total = S * f + L, total1 = POW != 0 ? S1 * f1 + L1 : total;
     const float inv_sum = 1.f / total, inv_sum1 = 1.f / total1;
     // a list that names every column leaves no rest, whatever rounding says
-    const float m = p.k >= p.vocab && static_cast<int>(warp_sum(listed)) >= p.vocab ? 0.f : r.rest;
+    const float m = p.k >= p.vocab && static_cast<int>(listed) >= p.vocab ? 0.f : r.rest;
     const float mass = r.mass + m;
     float A = mass != 0.f ? mass * f * inv_sum : 0.f;
     if (m > 0.f && S > 0.f) A -= m / S;
@@ -420,7 +432,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       p.loss[r.row] = scale * loss;
     }
     if (GRAD) {
-      if (!warp_waits(&sh.gradient_done[side], on_side[side] & 1, sh, p.status)) return;
+      if (!warp_waits(&sh.gradient_done[side], (on_side >> side) & 1, sh, p.status)) return;
       TG* drow = dz + r.row * p.lddz;
       const float kd = scale * p.kd * p.tau, ce = scale * p.ce;
       for (int i = lane; i < p.k; i += 32) {
@@ -442,7 +454,8 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
         drow[r.target] = from_f32<TG>(g);
       }
     }
-    ++on_side[side];
+    on_side ^= 1u << side;
+    ++turn;
     warp_arrives(&sh.side_free[side]);
   }
 }
@@ -460,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
       mbar_init(&sh.ready[g], 1);
       mbar_init(&sh.empty[g], kRingWarps);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kSides; ++i) {
       mbar_init(&sh.list_ready[i], 1);
       mbar_init(&sh.side_free[i], 2);  // finisher and patcher: the roles that nothing else makes wait for a dead row
       mbar_init(&sh.sums_ready[i], kRingWarps);
@@ -492,7 +505,7 @@ bool loss_by_ring(const DistillArgs& a, const Params& params, int pow, cudaStrea
   constexpr size_t kLeastSlice = 16 * 1024;            // below, several rows per SM hide each other's latencies
   constexpr size_t kMostBytes = 112 * 1024;            // two CTAs on an SM
   const size_t slice = static_cast<size_t>(params.per) * 16;
-  const size_t smem = slice + 2 * static_cast<size_t>(a.k) * sizeof(Listed);
+  const size_t smem = slice + kSides * static_cast<size_t>(a.k) * sizeof(Listed);
   if (slice < kLeastSlice || smem + sizeof(Shared) + 1024 > kMostBytes || a.rows < 4LL * num_sms()) return false;
   Params p = params;
   p.rows = a.rows;
