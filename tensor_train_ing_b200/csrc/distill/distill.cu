@@ -451,7 +451,7 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   p.lddz = a.lddz;
   p.status = a.status;
   const int pow = a.ce == 0.f || a.tau == 1.f ? 0 : a.tau == 2.f ? 2 : a.tau == 4.f ? 4 : 1;
-  if (plan.parts == 1 && distill::loss_by_ring(a, p, pow, stream)) return;
+  if (distill::loss_by_ring(a, p, pow, stream)) return;
   const size_t smem = plan.slice_bytes + a.k * sizeof(Entry);
   auto launch = [&](auto kernel, auto* z, auto* dz) {
     TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));

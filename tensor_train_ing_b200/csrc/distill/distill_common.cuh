@@ -73,7 +73,7 @@ void with_pow(int pow, F&& f) {
   }
 }
 
-// The kernel for rows that one CTA holds and of which there are many (distill_ring.cu); false where it does not apply.
+// The kernel for many long rows (distill_ring.cu); false where it does not apply.
 bool loss_by_ring(const DistillArgs& a, const Params& p, int pow, cudaStream_t stream);
 
 }  // namespace distill

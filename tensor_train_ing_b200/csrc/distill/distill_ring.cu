@@ -1,5 +1,5 @@
-// The distillation loss where a CTA holds a row and there are many rows: a persistent kernel whose warps have roles, so that
-// no step of a row waits for another row's memory latency.
+// The distillation loss of many long rows: a persistent kernel of CTAs, or of clusters that share a row, whose warps have
+// roles, so that no step of a row waits for another row's memory latency.
 //
 //   consumers  sum the row as it arrives, then (gradient) write exp((z - R) / tau) A + exp(z - R) B over it
 //   producer   keeps the row's stages coming: a stage of the next row as soon as the consumers are done with it
@@ -11,6 +11,10 @@
 // out ends all roles.  The arithmetic is that of distill.cu, of which this is the form for long rows: 4096 rows of 50257
 // bf16 logits, the loss alone, took 142 us there, with two CTAs of an SM each waiting through about 6 us of latencies per
 // row, and {EVAL} us here; loss and gradient of 8192 rows at tau 2 took 422 us and {TRAIN} us.
+#include <map>
+#include <mutex>
+#include <tuple>
+
 #include "../common/host.h"
 #include "distill_common.cuh"
 #include "row_ring.cuh"
@@ -45,29 +49,39 @@ struct Row {  // what the lister says about a row
   int live, target;
   float mass, rest, target_logit, list_top;
   unsigned edges;  // listed edge columns, by slot
-  int off;         // of the row from the 16-byte boundary before it, in elements
+  int first;       // column of the slice's first element
   int repeats, target_listed;
+  int target_here;  // the CTA has the target's column
 };
 
 struct Scalars {
   float at, A, B;
 };
 
+struct Part {  // what one CTA of the row's knows of its columns: sums at tau and at 1
+  float ref;          // the reference logit of the unlisted columns' sums (-inf: none)
+  float sum, sum1;
+  float list, list1;  // of the listed columns, each once, relative to the largest listed logit of the row
+};
+
 struct Shared {
   uint64_t full[kStages], ready[kStages], empty[kStages];
-  uint64_t list_ready[kSides], side_free[kSides], sums_ready[kSides], scalars_ready[kSides], gradient_done[kSides];
+  uint64_t list_ready[kSides], side_free[kSides], sums_ready[kSides], scalars_ready[kSides], gradient_done[kSides], part_ready[kSides];
   Row row[kSides];
   Scalars scalars[kSides];
+  Part part[kSides][rows::kMaxParts];
   rows::WarpSum sums[kSides][kRingWarps];
   int stop;
 };
 
 // Whether the barrier's phase completed; false when it, or a wait of another role, ran out.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_for(uint64_t* bar, int parity, Shared& sh, uint32_t* status) {
-  bool ok = mbar_test(bar, parity);
+  const auto test = [&] { return CLUSTER ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity); };
+  bool ok = test();
   if (!ok) {
     const long long t0 = clock64();
-    while (!(ok = mbar_test(bar, parity))) {
+    while (!(ok = test())) {
       if (*reinterpret_cast<volatile int*>(&sh.stop) != 0) break;
       if (clock64() - t0 > kWaitLimitCycles) {
         record_error(status, kErrTimeoutProducer);
@@ -78,13 +92,20 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, int parity, Shared& sh, 
   }
   return ok;
 }
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_waits(uint64_t* bar, int parity, Shared& sh, uint32_t* status) {
-  return __all_sync(0xffffffffu, wait_for(bar, parity, sh, status));
+  return __all_sync(0xffffffffu, wait_for<CLUSTER>(bar, parity, sh, status));
 }
 __device__ __forceinline__ void warp_arrives(uint64_t* bar) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
+
+// The row's CTA this one is, and the rows its cluster takes.
+struct Place {
+  int rank;
+  long long row0, step;
+};
 
 __device__ __forceinline__ bool counts(const Params& p, long long row, long long& target) {
   target = p.targets != nullptr ? p.targets[row] : 0;
@@ -92,16 +113,16 @@ __device__ __forceinline__ bool counts(const Params& p, long long row, long long
 }
 
 template <typename TZ>
-__device__ __forceinline__ void produce(const TZ* z, TZ* sm, Shared& sh, const Params& p) {
+__device__ __forceinline__ void produce(const TZ* z, TZ* sm, Shared& sh, const Params& p, const Place& at) {
   long long target;
-  bool live = blockIdx.x < p.rows && counts(p, blockIdx.x, target);
+  bool live = at.row0 < p.rows && counts(p, at.row0, target);
   int turn = 0;
   bool ok = true;
-  for (long long row = blockIdx.x; row < p.rows && ok; row += gridDim.x) {
+  for (long long row = at.row0; row < p.rows && ok; row += at.step) {
     const bool now = live;
-    if (row + gridDim.x < p.rows) live = counts(p, row + gridDim.x, target);
+    if (row + at.step < p.rows) live = counts(p, row + at.step, target);
     if (!now) continue;
-    const Span<TZ> s(z + row * p.ldz, p.vocab);
+    const Span<TZ> s(z + row * p.ldz, p.vocab, at.rank, p.per);
     for (int g = 0; g < kStages && ok; ++g) {
       if (turn > 0) ok = wait_for(&sh.empty[g], (turn - 1) & 1, sh, p.status);
       if (ok) s.load_stage(sm, sh.full, g);
@@ -114,10 +135,10 @@ __device__ __forceinline__ void produce(const TZ* z, TZ* sm, Shared& sh, const P
 }
 
 template <typename TZ>
-__device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh, const Params& p) {
+__device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh, const Params& p, const Place& at) {
   const int lane = threadIdx.x & 31;
   int n = 0;
-  for (long long row = blockIdx.x;; row += gridDim.x, ++n) {
+  for (long long row = at.row0;; row += at.step, ++n) {
     const int side = n % kSides;
     if (n >= kSides && !warp_waits(&sh.side_free[side], (n / kSides - 1) & 1, sh, p.status)) return;
     Row& r = sh.row[side];
@@ -130,7 +151,7 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
     const bool live = counts(p, row, target);
     if (!live) {
       if (lane == 0) {
-        if (target >= p.vocab) record_error(p.status, kErrBadIndex);
+        if (target >= p.vocab && at.rank == 0) record_error(p.status, kErrBadIndex);
         r.row = row;
         r.live = 0;
       }
@@ -138,7 +159,7 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
       continue;
     }
     if (p.targets == nullptr) target = -1;
-    const Span<TZ> s(z + row * p.ldz, p.vocab);
+    const Span<TZ> s(z + row * p.ldz, p.vocab, at.rank, p.per);
     Listed* list = lists + side * p.k;
     float top = -CUDART_INF_F, list_top = -CUDART_INF_F;
     bool present = false, has_target = false;
@@ -147,7 +168,7 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
                               : static_cast<const int*>(p.ids)[row * p.k + i];
       const float a = teacher_logit(p, row * p.k + i) * p.inv_tau;
       if (col >= p.vocab) {
-        record_error(p.status, kErrBadIndex);
+        if (at.rank == 0) record_error(p.status, kErrBadIndex);
         col = -1;
       }
       Listed e;
@@ -155,7 +176,7 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
       e.logp = col < 0 ? -CUDART_INF_F : a;
       e.p = 0.f;
       e.z = col < 0 ? 0.f : to_f32(s.row[col]);
-      e.stage = col < 0 ? -1 : s.stage_of(e.col);
+      e.stage = col < 0 || !s.holds(e.col) ? -1 : s.stage_of(e.col);
       e.owner = 0;
       list[i] = e;
       top = fmaxf(top, e.logp);
@@ -198,9 +219,10 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
       r.target_logit = target_logit;
       r.list_top = fabsf(list_top) < CUDART_INF_F ? list_top : 0.f;
       r.edges = 0u;
-      r.off = s.off;
+      r.first = s.first;
       r.repeats = 0;
       r.target_listed = has_target;
+      r.target_here = target >= 0 && s.holds(static_cast<int>(target));
     }
     __syncwarp();
     for (int i = lane; i < p.k; i += 32) {  // edge columns are never in shared memory: they are settled here
@@ -229,11 +251,11 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
       // Entries that share a column agree on one: the slot holds the number of its last writer until that one puts
       // -inf there (no number has -inf's bits).  Element e of the row lies at e + off from the slice's start.
       for (int i = lane; i < p.k; i += 32)
-        if (list[i].stage == g) put_mark(sm + list[i].col + r.off, i);
+        if (list[i].stage == g) put_mark(sm + list[i].col - r.first, i);
       __syncwarp();
       for (int i = lane; i < p.k; i += 32) {
         if (list[i].stage != g) continue;
-        TZ* slot = sm + list[i].col + r.off;
+        TZ* slot = sm + list[i].col - r.first;
         const bool owner = get_mark(slot) == i;
         list[i].owner = owner;
         if (owner)
@@ -250,8 +272,8 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
 }
 
 template <typename TZ, typename TG, bool GRAD, int POW>
-__device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Shared& sh, const Params& p, float c,
-                                        float c1) {
+__device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Shared& sh, const Params& p,
+                                        const Place& at, float c, float c1) {
   constexpr int E = Span<TZ>::kVec;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int turn = 0;
@@ -263,11 +285,11 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
     if (row < 0) return;
     TG* drow = GRAD ? dz + row * p.lddz : nullptr;
     if (!sh.row[side].live) {
-      if (GRAD) zero_row(drow, p.dz_cols, tid, kRingThreads);
+      if (GRAD) zero_row(drow, p.dz_cols, at.rank * kRingThreads + tid, p.parts * kRingThreads);
       warp_arrives(&sh.sums_ready[side]);
       continue;
     }
-    const Span<TZ> s(z + row * p.ldz, p.vocab);
+    const Span<TZ> s(z + row * p.ldz, p.vocab, at.rank, p.per);
     const int edge = tid < 16 ? s.edge_column(tid) : -1;
     const float edge_z = edge >= 0 ? to_f32(s.row[edge]) : 0.f;
 
@@ -289,16 +311,16 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
     if (GRAD) {
       if (!warp_waits(&sh.scalars_ready[side], (on_side >> side) & 1, sh, p.status)) return;
       const Scalars k = sh.scalars[side];
-      const Ref at(k.at, c), at1 = rows::ref_at_one<POW>(at);
+      const Ref from(k.at, c), from1 = rows::ref_at_one<POW>(from);
       const auto gradient = [&](float2 q, auto far) {
         constexpr bool FAR = decltype(far)::value;
-        const float2 e = rows::exp2_pair(rows::log2_pair<FAR>(q, rows::both(c), rows::both(FAR ? -at.z : -at.r)));
+        const float2 e = rows::exp2_pair(rows::log2_pair<FAR>(q, rows::both(c), rows::both(FAR ? -from.z : -from.r)));
         if constexpr (POW == 0)
           return rows::mul2(e, rows::both(k.A));
         else if constexpr (POW == 2)
           return rows::mul2(e, rows::fma2(e, rows::both(k.B), rows::both(k.A)));
         else
-          return rows::fma2(rows::at_one<POW, FAR>(e, q, at1), rows::both(k.B), rows::mul2(e, rows::both(k.A)));
+          return rows::fma2(rows::at_one<POW, FAR>(e, q, from1), rows::both(k.B), rows::mul2(e, rows::both(k.A)));
       };
       const bool same_vectors =
           sizeof(TG) == sizeof(TZ)
@@ -330,7 +352,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
       };
 #pragma unroll 1
       for (int g = 0; g < kStages; ++g) {
-        if (at.far)
+        if (from.far)
           stage(g, std::true_type{});
         else
           stage(g, std::false_type{});
@@ -338,9 +360,10 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
       }
       if (edge >= 0) {
         const float2 q = rows::both(edge_z);
-        drow[edge] = from_f32<TG>((at.far ? gradient(q, std::true_type{}) : gradient(q, std::false_type{})).x);
+        drow[edge] = from_f32<TG>((from.far ? gradient(q, std::true_type{}) : gradient(q, std::false_type{})).x);
       }
-      for (int i = p.vocab + tid; i < p.dz_cols; i += kRingThreads) drow[i] = from_f32<TG>(0.f);
+      if (at.rank == p.parts - 1)
+        for (int i = p.vocab + tid; i < p.dz_cols; i += kRingThreads) drow[i] = from_f32<TG>(0.f);
       warp_arrives(&sh.gradient_done[side]);
     }
     on_side ^= 1u << side;
@@ -349,7 +372,8 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
 }
 
 template <typename TG, bool GRAD, int POW>
-__device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, const Params& p, float c, float c1) {
+__device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, const Params& p, const Place& at, float c,
+                                            float c1) {
   const int lane = threadIdx.x & 31;
   const float scale = p.scale != nullptr ? *p.scale : 1.f;
   int turn = 0;
@@ -379,21 +403,46 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     }
     if (GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, sh, p.status)) return;
     if (!r.live) {
-      if (lane == 0) p.loss[r.row] = 0.f;
+      if (lane == 0 && at.rank == 0) p.loss[r.row] = 0.f;
       warp_arrives(&sh.side_free[side]);
       continue;
     }
-    // the rest's sums, relative to its own reference
-    const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
-    const float rest_top = warp_max(w.z);
+    // this CTA's part, to every CTA of the row
+    {
+      const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
+      const float most = warp_max(w.z);
+      const Ref mine(most == -CUDART_INF_F ? 0.f : most, c), of(w.z == -CUDART_INF_F ? 0.f : w.z, c);
+      const float sum = warp_sum(w.sum != 0.f ? w.sum * exp2f(mine.log2_of(of, c)) : 0.f);
+      const float sum1 =
+          POW != 0 ? warp_sum(w.sum1 != 0.f
+                                  ? w.sum1 * exp2f(rows::ref_at_one<POW>(mine).log2_of(rows::ref_at_one<POW>(of), c1))
+                                  : 0.f)
+                   : 0.f;
+      const Part part{most, sum, sum1, L, L1};
+      if (p.parts > 1) {
+        if (lane < p.parts) {
+          *rows::cg::this_cluster().map_shared_rank(&sh.part[side][at.rank], lane) = part;
+          mbar_arrive_at(&sh.part_ready[side], lane);
+        }
+        if (!warp_waits<true>(&sh.part_ready[side], (on_side >> side) & 1, sh, p.status)) return;
+      } else {
+        if (lane == 0) sh.part[side][0] = part;
+        __syncwarp();
+      }
+    }
+    // the rest's sums, relative to its own reference; every CTA computes the same
+    const Part w = lane < p.parts ? sh.part[side][lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0.f};
+    const float rest_top = warp_max(w.ref);
     const Ref own(rest_top != -CUDART_INF_F ? rest_top : r.list_top, c), own1 = rows::ref_at_one<POW>(own);
-    const Ref of(w.z == -CUDART_INF_F ? 0.f : w.z, c);
+    const Ref of(w.ref == -CUDART_INF_F ? 0.f : w.ref, c);
     const float S = warp_sum(w.sum != 0.f ? w.sum * exp2f(own.log2_of(of, c)) : 0.f);
     const float S1 =
         POW != 0 ? warp_sum(w.sum1 != 0.f ? w.sum1 * exp2f(own1.log2_of(rows::ref_at_one<POW>(of), c1)) : 0.f) : 0.f;
+    L = warp_sum(w.list);
+    if (POW != 0) L1 = warp_sum(w.list1);
     // the row's reference: the larger of the rest's and the list's
-    const Ref ref(listed > 0.f && r.list_top > own.z ? r.list_top : own.z, c), ref1 = rows::ref_at_one<POW>(ref);
-    if (listed > 0.f) {
+    const Ref ref(L != 0.f && r.list_top > own.z ? r.list_top : own.z, c), ref1 = rows::ref_at_one<POW>(ref);
+    if (L != 0.f) {
       L *= exp2f(ref.log2_of(list_ref, c));
       if (POW != 0) L1 *= exp2f(ref1.log2_of(list_ref1, c1));
     }
@@ -418,12 +467,14 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     }
     const float log2_total = log2f(total);
     float kl = 0.f;
-    for (int i = lane; i < p.k; i += 32) {
-      const float logq = (ref.log2_of(list[i].z, c) - log2_total) * CUDART_LN2_F;
-      if (list[i].p != 0.f) kl += list[i].p * (list[i].logp - logq);
+    if (at.rank == 0) {
+      for (int i = lane; i < p.k; i += 32) {
+        const float logq = (ref.log2_of(list[i].z, c) - log2_total) * CUDART_LN2_F;
+        if (list[i].p != 0.f) kl += list[i].p * (list[i].logp - logq);
+      }
+      kl = warp_sum(kl);
     }
-    kl = warp_sum(kl);
-    if (lane == 0) {
+    if (lane == 0 && at.rank == 0) {
       if (m > 0.f)  // log q_rest from its parts where the probability itself leaves fp32's range
         kl += m * (f > 1e-30f ? logf(m / (S * f * inv_sum))
                               : logf(m) - (logf(S) + (own.z - ref.z) * p.inv_tau - logf(total)));
@@ -448,7 +499,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
         if (ce != 0.f) g += ce * (exp2f(ref1.log2_of(list[i].z, c1)) * inv_sum1 - (col == r.target ? 1.f : 0.f));
         drow[col] = from_f32<TG>(g);
       }
-      if (lane == 0 && ce != 0.f && !r.target_listed) {
+      if (lane == 0 && ce != 0.f && !r.target_listed && r.target_here) {
         float g = rows::fast_exp2(own.log2_of(r.target_logit, c)) * A - ce;
         if (POW != 0) g += rows::fast_exp2(own1.log2_of(r.target_logit, c1)) * B;
         drow[r.target] = from_f32<TG>(g);
@@ -479,40 +530,83 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
       mbar_init(&sh.sums_ready[i], kRingWarps);
       mbar_init(&sh.scalars_ready[i], 1);
       mbar_init(&sh.gradient_done[i], kRingWarps);
+      mbar_init(&sh.part_ready[i], p.parts);
     }
     sh.stop = 0;
     fence_mbar_init();
   }
-  __syncthreads();
+  rows::cg::cluster_group cluster = rows::cg::this_cluster();
+  if (p.parts > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  const Place at{p.parts > 1 ? static_cast<int>(cluster.block_rank()) : 0, blockIdx.x / p.parts, gridDim.x / p.parts};
   const float c = p.inv_tau * CUDART_L2E_F, c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
   const int warp = threadIdx.x >> 5;
   if (warp < kRingWarps) {
-    consume<TZ, TG, GRAD, POW>(z, dz, sm, sh, p, c, c1);
+    consume<TZ, TG, GRAD, POW>(z, dz, sm, sh, p, at, c, c1);
   } else if (warp == kProducer) {
-    if ((threadIdx.x & 31) == 0) produce(z, sm, sh, p);
+    if ((threadIdx.x & 31) == 0) produce(z, sm, sh, p, at);
   } else if (warp == kLister) {
-    list_rows(z, lists, sh, p);
+    list_rows(z, lists, sh, p, at);
   } else if (warp == kPatcher) {
     patch_stages(sm, lists, sh, p);
   } else {
-    finish_rows<TG, GRAD, POW>(dz, lists, sh, p, c, c1);
+    finish_rows<TG, GRAD, POW>(dz, lists, sh, p, at, c, c1);
   }
+  if (p.parts > 1) {  // no CTA leaves while another may still write to it
+    __syncwarp();
+    cluster.sync();
+  }
+}
+
+// Clusters of this kernel that the device runs at one time (asked once for each kernel, size and shared memory).
+int active_clusters(const void* kernel, const cudaLaunchConfig_t& cfg, int parts) {
+  static std::mutex lock;
+  static std::map<std::tuple<int, const void*, int, size_t>, int> known;
+  int device = 0;
+  TTB_CUDA_CHECK(cudaGetDevice(&device));
+  const std::lock_guard<std::mutex> guard(lock);
+  auto [it, fresh] = known.try_emplace({device, kernel, parts, cfg.dynamicSmemBytes}, 0);
+  if (fresh) TTB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&it->second, kernel, &cfg));
+  return it->second < 1 ? 1 : it->second;
 }
 
 }  // namespace
 
 bool loss_by_ring(const DistillArgs& a, const Params& params, int pow, cudaStream_t stream) {
-  constexpr size_t kLeastSlice = 16 * 1024;            // below, several rows per SM hide each other's latencies
-  constexpr size_t kMostBytes = 112 * 1024;            // two CTAs on an SM
-  const size_t slice = static_cast<size_t>(params.per) * 16;
-  const size_t smem = slice + kSides * static_cast<size_t>(a.k) * sizeof(Listed);
-  if (slice < kLeastSlice || smem + sizeof(Shared) + 1024 > kMostBytes || a.rows < 4LL * num_sms()) return false;
+  constexpr size_t kLeastSlice = 16 * 1024;  // below, several rows per SM hide each other's latencies
+  constexpr size_t kMostBytes = 113 * 1024;  // two CTAs on an SM
+  const int E = 16 / scalar_bytes(a.z_type);
+  const int total = static_cast<int>((a.vocab + 2LL * (E - 1)) / E);  // the most vectors a row can touch
   Params p = params;
   p.rows = a.rows;
+  size_t smem = 0;
+  for (p.parts = 1; p.parts <= rows::kMaxParts; ++p.parts) {
+    p.per = (total + p.parts - 1) / p.parts;
+    smem = static_cast<size_t>(p.per) * 16 + kSides * static_cast<size_t>(a.k) * sizeof(Listed);
+    if (smem + sizeof(Shared) + 1024 <= kMostBytes) break;
+  }
+  if (p.parts > rows::kMaxParts || static_cast<size_t>(p.per) * 16 < kLeastSlice || a.rows * p.parts < 4LL * num_sms())
+    return false;
   auto launch = [&](auto kernel, auto* z, auto* dz) {
     TTB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    kernel<<<2 * num_sms(), kThreads, smem, stream>>>(z, dz, p);
-    TTB_CUDA_CHECK(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * num_sms());
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    if (p.parts > 1) {
+      cfg.gridDim.x = p.parts;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      cfg.gridDim.x = p.parts * active_clusters(reinterpret_cast<const void*>(kernel), cfg, p.parts);
+    }
+    TTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, z, dz, p));
   };
   with_kernel_types(a, [&](const auto* z, auto* dz) {
     using TZ = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;

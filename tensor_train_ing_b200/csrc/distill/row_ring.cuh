@@ -1,11 +1,12 @@
-// A row of logits in the shared memory of a CTA whose warps have roles: `kRingThreads` consumer threads work on rows
-// that other warps bring in and finish.
+// A row of logits in the shared memory of a CTA, or of the CTAs of a cluster, whose warps have roles: `kRingThreads` consumer
+// threads work on rows that other warps bring in and finish.
 //
 // A row is cut into 16-byte vectors counted from the 16-byte boundary at or below its first element, so that
 // rows at any element offset are copied in whole aligned vectors; the at most two vectors that reach over the
-// row's ends are its edges and are read from global memory element by element.  Consumer thread t works on the whole
-// vectors lo + t, lo + t + kRingThreads, ...  They arrive in kStages bulk copies with a barrier each, and a stage's memory is
-// given to the CTA's next row as soon as the last pass over it is done.
+// row's ends are its edges and are read from global memory element by element.  CTA `rank` of a row has the vectors from
+// rank * per on, and its consumer thread t works on the whole vectors lo + t, lo + t + kRingThreads, ... of them.  They arrive in
+// kStages bulk copies with a barrier each, and a stage's memory is given to the CTA's next row as soon as the last pass
+// over it is done.
 #pragma once
 
 #include "row_slice.cuh"
@@ -20,39 +21,43 @@ template <typename T>
 struct Span {
   static constexpr int kVec = 16 / static_cast<int>(sizeof(T));
   const T* row;
-  int columns;
-  int first;   // column of vector 0 (negative where that vector starts before the row)
-  int lo, hi;  // the whole vectors: [lo, hi)
+  int first;   // column of the CTA's vector 0 (negative where that vector starts before the row)
+  int lo, hi;  // its whole vectors: [lo, hi)
+  int c0, c1;  // its columns: [c0, c1)
   int off;     // elements between the 16-byte boundary and the row's first element
   int rounds;  // whole vectors that every thread has; the threads below hi - lo - rounds * threads have one more
   int stage;   // rounds per stage
 
-  __device__ __forceinline__ Span(const T* r, int cols) {
+  __device__ __forceinline__ Span(const T* r, int cols, int rank, int per) {
     constexpr int E = kVec;
     row = r;
     off = static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
-    const int nv = (off + cols + E - 1) / E;
-    columns = cols;
-    first = -off;
-    lo = off > 0 ? 1 : 0;
-    hi = max(lo, nv * E - off > cols ? nv - 1 : nv);
+    const int total = (off + cols + E - 1) / E;
+    const int v0 = min(rank * per, total);
+    const int nv = min(per, total - v0);
+    first = v0 * E - off;
+    c0 = min(cols, max(0, first));
+    c1 = max(c0, min(cols, first + nv * E));
+    lo = first < 0 ? 1 : 0;
+    hi = max(lo, first + nv * E > cols ? nv - 1 : nv);
     rounds = (hi - lo) / kRingThreads;
     stage = rounds / kStages + 1;
   }
-  __device__ __forceinline__ int vector_of(int col) const { return (col + off) / kVec; }
-  // The stage that brings a column, or kStages for an edge column.
+  __device__ __forceinline__ bool holds(int col) const { return col >= c0 && col < c1; }
+  // The stage that brings one of the CTA's columns, or kStages for an edge column.
   __device__ __forceinline__ int stage_of(int col) const {
-    const int v = vector_of(col);
+    const int v = (col - first) / kVec;
     return v >= lo && v < hi ? (v - lo) / (stage * kRingThreads) : kStages;
   }
   // Edge columns have slots 0..7 (before the first whole vector) and 8..15 (after the last); -1 for no column.
   __device__ __forceinline__ int edge_slot(int col) const {
-    return col < first + lo * kVec ? col : 8 + col - (first + hi * kVec);
+    const int head = min(c1, first + lo * kVec);
+    return col < head ? col - c0 : 8 + col - max(head, first + hi * kVec);
   }
   __device__ __forceinline__ int edge_column(int slot) const {
-    const int head = min(columns, first + lo * kVec), tail = max(head, first + hi * kVec);
-    const int col = slot < 8 ? slot : tail + slot - 8;
-    return slot < 8 ? (col < head ? col : -1) : (col < columns ? col : -1);
+    const int head = min(c1, first + lo * kVec), tail = max(head, first + hi * kVec);
+    const int col = slot < 8 ? c0 + slot : tail + slot - 8;
+    return col < (slot < 8 ? head : c1) ? col : -1;
   }
   // One thread: starts the copy of stage g into `sm`.
   __device__ __forceinline__ void load_stage(T* sm, uint64_t* bars, int g) const {

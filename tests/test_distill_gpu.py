@@ -268,14 +268,15 @@ def test_loss_of_strided_and_misaligned_rows(dtype, offset, ld):
     _check_loss(z, ids.long(), t, lse, None, 1.0, 1.0, 0.0, 1.0)
 
 
-# Many rows of logits that one CTA holds: the persistent kernel.  Its CTAs take several rows each, with and without
+# Many long rows: the persistent kernel, of single CTAs and of clusters.  These take several rows each, with and without
 # left-out ones between them; odd widths and offsets give rows with edges on either side.
 @pytest.mark.parametrize("dtype,v,ld,offset", [(BF16, 8192, 8192, 0), (BF16, 9001, 9001, 3), (F16, 20011, 20032, 1),
-                                               (F32, 4100, 4100, 0), (F32, 12345, 12345, 2), (BF16, 50257, 50257, 0)])
+                                               (F32, 4100, 4100, 0), (F32, 12345, 12345, 2), (BF16, 50257, 50257, 0),
+                                               (F32, 50257, 50257, 1), (F32, 131072, 131072, 0), (F16, 200003, 200003, 5)])
 @pytest.mark.parametrize("k,rest,tau,ce", [(1, False, 1.0, 0.0), (40, True, 2.0, 0.5), (200, True, 1.5, 0.25),
                                            (64, False, 4.0, 0.5)])
 def test_loss_of_many_rows(dtype, v, ld, offset, k, rest, tau, ce):
-    n = 601 if v > 30000 else 1201
+    n = 601 if v > 9500 else 1201
     z = _logits(n, v, dtype, v + k, ld=ld, offset=offset)
     ids, t, lse = _teacher(z, k, F32, k, rest, tau)
     ids[5:9] = -1
