@@ -272,8 +272,8 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
 }
 
 template <typename TZ, typename TG, bool GRAD, int POW>
-__device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Shared& sh, const Params& p,
-                                        const Place& at, float c, float c1) {
+__device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const Listed* lists, Shared& sh,
+                                        const Params& p, const Place& at, float c, float c1) {
   constexpr int E = Span<TZ>::kVec;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int turn = 0;
@@ -294,16 +294,36 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
     const float edge_z = edge >= 0 ? to_f32(s.row[edge]) : 0.f;
 
     rows::Sums<POW> sums(c);
+    bool sure = false;  // all threads of the warp have a reference: batches are added without looking for one
 #pragma unroll 1
     for (int g = 0; g < kStages; ++g) {
       if (!warp_waits(&sh.ready[g], turn & 1, sh, p.status)) return;
-      s.for_stage(sm, g, [&](const auto& u, int) {
-        sums.see(rows::max_of<TZ>(u), c);
-        sums.template add_batch<TZ>(u, c);
-      });
+      if (sure) {
+        s.for_stage(sm, g, [&](const auto& u, int) { sums.template add_vectors<TZ, false>(u, c); });
+      } else {
+        s.for_stage(sm, g, [&](const auto& u, int) {
+          sums.see(rows::max_of<TZ>(u), c);
+          sums.template add_batch<TZ>(u, c);
+        });
+        sure = __all_sync(0xffffffffu, sums.set && !sums.ref.far);
+      }
       if (!GRAD) warp_arrives(&sh.empty[g]);
     }
-    if (edge >= 0 && !((sh.row[side].edges >> tid) & 1u)) sums.add_one(edge_z, c);
+    const bool counted = edge >= 0 && !((sh.row[side].edges >> tid) & 1u);
+    if (counted) sums.add_one(edge_z, c);
+    if (sums.overflowed()) {  // rare: logits 80 tau above a thread's first ones, infinities, NaN
+      const Listed* list = lists + side * p.k;
+      sums = rows::Sums<POW>(c);
+      for (int v = s.lo + tid; v < s.hi; v += kRingThreads) {
+        for (int e = 0; e < E; ++e) {
+          const int col = s.first + v * E + e;
+          bool out = false;
+          for (int i = 0; i < p.k; ++i) out |= list[i].col == col;
+          if (!out) sums.add_one(to_f32(s.row[col]), c);
+        }
+      }
+      if (counted) sums.add_one(edge_z, c);
+    }
     const rows::WarpSum mine = rows::warp_total<POW>(sums, c, c1);
     if (lane == 0) sh.sums[side][warp] = mine;
     warp_arrives(&sh.sums_ready[side]);
@@ -371,6 +391,28 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, Share
   }
 }
 
+__device__ __forceinline__ float2 warp_sum2(float2 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float a = __shfl_xor_sync(0xffffffffu, v.x, o), b = __shfl_xor_sync(0xffffffffu, v.y, o);
+    v.x += a;
+    v.y += b;
+  }
+  return v;
+}
+// The lanes' sums relative to the largest of their references, which `top` becomes.
+template <int POW>
+__device__ __forceinline__ float2 relative_sums(float& top, float sum, float sum1, float c, float c1) {
+  const Ref of(top == -CUDART_INF_F ? 0.f : top, c);
+  top = warp_max(top);
+  const Ref to(top == -CUDART_INF_F ? 0.f : top, c);
+  if (sum != 0.f) sum *= rows::fast_exp2(to.log2_of(of, c));
+  if (POW != 0 && sum1 != 0.f)
+    sum1 *= rows::fast_exp2(rows::ref_at_one<POW>(to).log2_of(rows::ref_at_one<POW>(of), c1));
+  if (POW == 0) return make_float2(warp_sum(sum), 0.f);
+  return warp_sum2(make_float2(sum, sum1));
+}
+
 template <typename TG, bool GRAD, int POW>
 __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, const Params& p, const Place& at, float c,
                                             float c1) {
@@ -407,54 +449,42 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       warp_arrives(&sh.side_free[side]);
       continue;
     }
-    // this CTA's part, to every CTA of the row
-    {
-      const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
-      const float most = warp_max(w.z);
-      const Ref mine(most == -CUDART_INF_F ? 0.f : most, c), of(w.z == -CUDART_INF_F ? 0.f : w.z, c);
-      const float sum = warp_sum(w.sum != 0.f ? w.sum * exp2f(mine.log2_of(of, c)) : 0.f);
-      const float sum1 =
-          POW != 0 ? warp_sum(w.sum1 != 0.f
-                                  ? w.sum1 * exp2f(rows::ref_at_one<POW>(mine).log2_of(rows::ref_at_one<POW>(of), c1))
-                                  : 0.f)
-                   : 0.f;
-      const Part part{most, sum, sum1, L, L1};
-      if (p.parts > 1) {
-        if (lane < p.parts) {
-          *rows::cg::this_cluster().map_shared_rank(&sh.part[side][at.rank], lane) = part;
-          mbar_arrive_at(&sh.part_ready[side], lane);
-        }
-        if (!warp_waits<true>(&sh.part_ready[side], (on_side >> side) & 1, sh, p.status)) return;
-      } else {
-        if (lane == 0) sh.part[side][0] = part;
-        __syncwarp();
+    // The unlisted columns' sums, relative to one reference: of this CTA, then of the row.  The consumers wait for what
+    // follows, so independent sums go through the lanes together and quotients are the hardware's (2 ulp).
+    const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
+    float rest_top = w.z;
+    float2 S2 = relative_sums<POW>(rest_top, w.sum, w.sum1, c, c1);
+    if (p.parts > 1) {
+      const Part part{rest_top, S2.x, S2.y, L, L1};
+      if (lane < p.parts) {
+        *rows::cg::this_cluster().map_shared_rank(&sh.part[side][at.rank], lane) = part;
+        mbar_arrive_at(&sh.part_ready[side], lane);
       }
+      if (!warp_waits<true>(&sh.part_ready[side], (on_side >> side) & 1, sh, p.status)) return;
+      const Part q = lane < p.parts ? sh.part[side][lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0.f};
+      rest_top = q.ref;
+      S2 = relative_sums<POW>(rest_top, q.sum, q.sum1, c, c1);
+      const float2 L2 = warp_sum2(make_float2(q.list, q.list1));
+      L = L2.x;
+      L1 = L2.y;
     }
-    // the rest's sums, relative to its own reference; every CTA computes the same
-    const Part w = lane < p.parts ? sh.part[side][lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0.f};
-    const float rest_top = warp_max(w.ref);
+    const float S = S2.x, S1 = S2.y;
     const Ref own(rest_top != -CUDART_INF_F ? rest_top : r.list_top, c), own1 = rows::ref_at_one<POW>(own);
-    const Ref of(w.ref == -CUDART_INF_F ? 0.f : w.ref, c);
-    const float S = warp_sum(w.sum != 0.f ? w.sum * exp2f(own.log2_of(of, c)) : 0.f);
-    const float S1 =
-        POW != 0 ? warp_sum(w.sum1 != 0.f ? w.sum1 * exp2f(own1.log2_of(rows::ref_at_one<POW>(of), c1)) : 0.f) : 0.f;
-    L = warp_sum(w.list);
-    if (POW != 0) L1 = warp_sum(w.list1);
     // the row's reference: the larger of the rest's and the list's
     const Ref ref(L != 0.f && r.list_top > own.z ? r.list_top : own.z, c), ref1 = rows::ref_at_one<POW>(ref);
-    if (L != 0.f) {
+    if (L != 0.f && ref.z != r.list_top) {
       L *= exp2f(ref.log2_of(list_ref, c));
       if (POW != 0) L1 *= exp2f(ref1.log2_of(list_ref1, c1));
     }
     const bool same = ref.z == own.z;
     const float f = same ? 1.f : exp2f(ref.log2_of(own, c)), f1 = same ? 1.f : exp2f(ref1.log2_of(own1, c1));
     const float total = S * f + L, total1 = POW != 0 ? S1 * f1 + L1 : total;
-    const float inv_sum = 1.f / total, inv_sum1 = 1.f / total1;
+    const float inv_sum = __fdividef(1.f, total), inv_sum1 = POW != 0 ? __fdividef(1.f, total1) : inv_sum;
     // a list that names every column leaves no rest, whatever rounding says
     const float m = p.k >= p.vocab && static_cast<int>(listed) >= p.vocab ? 0.f : r.rest;
     const float mass = r.mass + m;
     float A = mass != 0.f ? mass * f * inv_sum : 0.f;
-    if (m > 0.f && S > 0.f) A -= m / S;
+    if (m > 0.f && S > 0.f) A -= __fdividef(m, S);
     A *= scale * p.kd * p.tau;
     float B = p.ce != 0.f ? scale * p.ce * f1 * inv_sum1 : 0.f;
     if (POW == 0) {  // one exponential serves both terms
@@ -544,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
   const float c = p.inv_tau * CUDART_L2E_F, c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
   const int warp = threadIdx.x >> 5;
   if (warp < kRingWarps) {
-    consume<TZ, TG, GRAD, POW>(z, dz, sm, sh, p, at, c, c1);
+    consume<TZ, TG, GRAD, POW>(z, dz, sm, lists, sh, p, at, c, c1);
   } else if (warp == kProducer) {
     if ((threadIdx.x & 31) == 0) produce(z, sm, sh, p, at);
   } else if (warp == kLister) {

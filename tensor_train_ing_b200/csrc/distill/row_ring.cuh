@@ -70,20 +70,14 @@ struct Span {
       mbar_arrive(&bars[g]);
     }
   }
-  // f(vectors, first vector number) over the thread's vectors of stage g: two (threads apart) at a time, then one.
+  // f(vector, its number) over the thread's vectors of stage g.  One at a time: the passes are long straight code, and
+  // a second copy of them for pairs of vectors costs more in instruction fetches than it gains.
   template <typename F>
   __device__ __forceinline__ void for_stage(const T* sm, int g, F&& f) const {
-    const int step = kRingThreads, end = min((g + 1) * stage, rounds);
-    int i = g * stage, v = lo + threadIdx.x + i * step;
-    for (; i + 2 <= end; i += 2, v += 2 * step) {
-      uint4 u[2] = {*reinterpret_cast<const uint4*>(sm + v * kVec),
-                    *reinterpret_cast<const uint4*>(sm + (v + step) * kVec)};
-      f(u, v);
-    }
-    // the stage's odd round, and in the stage that has it the round that only some threads have
-    const int last = min((g + 1) * stage, rounds + 1);
-    for (; i < last && v < hi; ++i, v += step) {
-      uint4 u[1] = {*reinterpret_cast<const uint4*>(sm + v * kVec)};
+    const int last = min(hi, lo + (g + 1) * stage * kRingThreads);
+#pragma unroll 1
+    for (int v = lo + static_cast<int>(threadIdx.x) + g * stage * kRingThreads; v < last; v += kRingThreads) {
+      const uint4 u[1] = {*reinterpret_cast<const uint4*>(sm + v * kVec)};
       f(u, v);
     }
   }
@@ -124,8 +118,10 @@ __device__ __forceinline__ float max_of(const uint4 (&u)[N]) {
 }
 
 // A thread's running sums of exp((z - ref) / tau) and, for POW > 0, exp(z - ref), over whatever it has seen.  The
-// reference is the largest logit of its first batch and moves only when a batch exceeds it by more than 2^40, so
-// that almost no batch rescales anything and no sum can overflow.
+// reference is the largest logit of its first batch that has one.  While `see` is called before every batch it moves when a
+// batch exceeds it by more than 2^40, so that no sum can overflow; batches added without have no maximum to take, which
+// is a fifth of the work and a branch that keeps the next batch's loads and exponentials from starting, but may overflow
+// where a logit exceeds the reference by more than 2^120: then `overflowed`, and the sums have to be taken again.
 template <int POW>
 struct Sums {
   Ref ref, ref1;
@@ -188,6 +184,7 @@ struct Sums {
     else
       add<false>(pair, 0, c);
   }
+  __device__ __forceinline__ bool overflowed() const { return !(sum() < CUDART_INF_F) || !(sum1() < CUDART_INF_F); }
   __device__ __forceinline__ float sum() const { return (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y); }
   __device__ __forceinline__ float sum1() const { return (acc1[0].x + acc1[0].y) + (acc1[1].x + acc1[1].y); }
 };
