@@ -28,6 +28,9 @@ using rows::Span;
 using rows::kRingThreads;
 using rows::kRingWarps;
 using rows::kStages;
+using rows::wait_for;
+using rows::warp_arrives;
+using rows::warp_waits;
 
 constexpr int kThreads = 512;
 constexpr int kProducer = kRingWarps, kLister = kRingWarps + 1, kPatcher = kRingWarps + 2, kFinisher = kRingWarps + 3;
@@ -74,33 +77,6 @@ struct Shared {
   int stop;
 };
 
-// Whether the barrier's phase completed; false when it, or a wait of another role, ran out.
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool wait_for(uint64_t* bar, int parity, Shared& sh, uint32_t* status) {
-  const auto test = [&] { return CLUSTER ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity); };
-  bool ok = test();
-  if (!ok) {
-    const long long t0 = clock64();
-    while (!(ok = test())) {
-      if (*reinterpret_cast<volatile int*>(&sh.stop) != 0) break;
-      if (clock64() - t0 > kWaitLimitCycles) {
-        record_error(status, kErrTimeoutProducer);
-        *reinterpret_cast<volatile int*>(&sh.stop) = 1;
-        break;
-      }
-    }
-  }
-  return ok;
-}
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool warp_waits(uint64_t* bar, int parity, Shared& sh, uint32_t* status) {
-  return __all_sync(0xffffffffu, wait_for<CLUSTER>(bar, parity, sh, status));
-}
-__device__ __forceinline__ void warp_arrives(uint64_t* bar) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-
 // The row's CTA this one is, and the rows its cluster takes.
 struct Place {
   int rank;
@@ -124,7 +100,7 @@ __device__ __forceinline__ void produce(const TZ* z, TZ* sm, Shared& sh, const P
     if (!now) continue;
     const Span<TZ> s(z + row * p.ldz, p.vocab, at.rank, p.per);
     for (int g = 0; g < kStages && ok; ++g) {
-      if (turn > 0) ok = wait_for(&sh.empty[g], (turn - 1) & 1, sh, p.status);
+      if (turn > 0) ok = wait_for(&sh.empty[g], (turn - 1) & 1, &sh.stop, p.status);
       if (ok) s.load_stage(sm, sh.full, g);
     }
     ++turn;
@@ -140,7 +116,7 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
   int n = 0;
   for (long long row = at.row0;; row += at.step, ++n) {
     const int side = n % kSides;
-    if (n >= kSides && !warp_waits(&sh.side_free[side], (n / kSides - 1) & 1, sh, p.status)) return;
+    if (n >= kSides && !warp_waits(&sh.side_free[side], (n / kSides - 1) & 1, &sh.stop, p.status)) return;
     Row& r = sh.row[side];
     if (row >= p.rows) {
       if (lane == 0) r.row = -1;
@@ -242,12 +218,12 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
   int turn = 0;
   for (int n = 0;; ++n) {
     const int side = n % kSides;
-    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, sh, p.status)) return;
+    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, &sh.stop, p.status)) return;
     Row& r = sh.row[side];
     if (r.row < 0) return;
     Listed* list = lists + side * p.k;
     for (int g = 0; g < kStages && r.live; ++g) {
-      if (!warp_waits(&sh.full[g], turn & 1, sh, p.status)) return;
+      if (!warp_waits(&sh.full[g], turn & 1, &sh.stop, p.status)) return;
       // Entries that share a column agree on one: the slot holds the number of its last writer until that one puts
       // -inf there (no number has -inf's bits).  Element e of the row lies at e + off from the slice's start.
       for (int i = lane; i < p.k; i += 32)
@@ -280,7 +256,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
   unsigned on_side = 0;  // bit s: the parity of the live rows side s has had
   for (int n = 0;; ++n) {
     const int side = n % kSides;
-    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, sh, p.status)) return;
+    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, &sh.stop, p.status)) return;
     const long long row = sh.row[side].row;
     if (row < 0) return;
     TG* drow = GRAD ? dz + row * p.lddz : nullptr;
@@ -297,7 +273,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
     bool sure = false;  // all threads of the warp have a reference: batches are added without looking for one
 #pragma unroll 1
     for (int g = 0; g < kStages; ++g) {
-      if (!warp_waits(&sh.ready[g], turn & 1, sh, p.status)) return;
+      if (!warp_waits(&sh.ready[g], turn & 1, &sh.stop, p.status)) return;
       if (sure) {
         s.for_stage(sm, g, [&](const auto& u, int) { sums.template add_vectors<TZ, false>(u, c); });
       } else {
@@ -329,7 +305,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
     warp_arrives(&sh.sums_ready[side]);
 
     if (GRAD) {
-      if (!warp_waits(&sh.scalars_ready[side], (on_side >> side) & 1, sh, p.status)) return;
+      if (!warp_waits(&sh.scalars_ready[side], (on_side >> side) & 1, &sh.stop, p.status)) return;
       const Scalars k = sh.scalars[side];
       const Ref from(k.at, c), from1 = rows::ref_at_one<POW>(from);
       const auto gradient = [&](float2 q, auto far) {
@@ -406,9 +382,8 @@ __device__ __forceinline__ float2 relative_sums(float& top, float sum, float sum
   const Ref of(top == -CUDART_INF_F ? 0.f : top, c);
   top = warp_max(top);
   const Ref to(top == -CUDART_INF_F ? 0.f : top, c);
-  if (sum != 0.f) sum *= rows::fast_exp2(to.log2_of(of, c));
-  if (POW != 0 && sum1 != 0.f)
-    sum1 *= rows::fast_exp2(rows::ref_at_one<POW>(to).log2_of(rows::ref_at_one<POW>(of), c1));
+  sum = rows::rescaled(sum, to.log2_of(of, c));
+  if (POW != 0) sum1 = rows::rescaled(sum1, rows::ref_at_one<POW>(to).log2_of(rows::ref_at_one<POW>(of), c1));
   if (POW == 0) return make_float2(warp_sum(sum), 0.f);
   return warp_sum2(make_float2(sum, sum1));
 }
@@ -422,17 +397,17 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
   unsigned on_side = 0;  // bit s: the parity of the live rows side s has had
   for (int n = 0;; ++n) {
     const int side = n % kSides;
-    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, sh, p.status)) return;
+    if (!warp_waits(&sh.list_ready[side], (n / kSides) & 1, &sh.stop, p.status)) return;
     const Row& r = sh.row[side];
     if (r.row < 0) return;
     Listed* list = lists + side * p.k;
     // The list's sums, each column once, relative to its largest logit.  With a gradient, whose consumers wait for this
     // warp, already while they sum the last stage (they then cannot run past that stage's phase; without one they can).
-    if (!GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, sh, p.status)) return;
+    if (!GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, &sh.stop, p.status)) return;
     const Ref list_ref(r.list_top, c), list_ref1 = rows::ref_at_one<POW>(list_ref);
     float L = 0.f, L1 = 0.f, listed = 0.f;
     if (r.live) {
-      if (GRAD && !warp_waits(&sh.ready[kStages - 1], turn & 1, sh, p.status)) return;
+      if (GRAD && !warp_waits(&sh.ready[kStages - 1], turn & 1, &sh.stop, p.status)) return;
       for (int i = lane; i < p.k; i += 32) {
         if (!list[i].owner) continue;
         L += exp2f(list_ref.log2_of(list[i].z, c));
@@ -443,7 +418,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       if (POW != 0) L1 = warp_sum(L1);
       listed = warp_sum(listed);
     }
-    if (GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, sh, p.status)) return;
+    if (GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, &sh.stop, p.status)) return;
     if (!r.live) {
       if (lane == 0 && at.rank == 0) p.loss[r.row] = 0.f;
       warp_arrives(&sh.side_free[side]);
@@ -460,7 +435,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
         *rows::cg::this_cluster().map_shared_rank(&sh.part[side][at.rank], lane) = part;
         mbar_arrive_at(&sh.part_ready[side], lane);
       }
-      if (!warp_waits<true>(&sh.part_ready[side], (on_side >> side) & 1, sh, p.status)) return;
+      if (!warp_waits<true>(&sh.part_ready[side], (on_side >> side) & 1, &sh.stop, p.status)) return;
       const Part q = lane < p.parts ? sh.part[side][lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0.f};
       rest_top = q.ref;
       S2 = relative_sums<POW>(rest_top, q.sum, q.sum1, c, c1);
@@ -513,7 +488,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       p.loss[r.row] = scale * loss;
     }
     if (GRAD) {
-      if (!warp_waits(&sh.gradient_done[side], (on_side >> side) & 1, sh, p.status)) return;
+      if (!warp_waits(&sh.gradient_done[side], (on_side >> side) & 1, &sh.stop, p.status)) return;
       TG* drow = dz + r.row * p.lddz;
       const float kd = scale * p.kd * p.tau, ce = scale * p.ce;
       for (int i = lane; i < p.k; i += 32) {

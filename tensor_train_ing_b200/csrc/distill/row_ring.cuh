@@ -83,6 +83,34 @@ struct Span {
   }
 };
 
+// Whether the barrier's phase completed; false when it, or a wait of another role (`stop`, in shared memory), ran
+// out.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_for(uint64_t* bar, int parity, volatile int* stop, uint32_t* status) {
+  const auto test = [&] { return CLUSTER ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity); };
+  bool ok = test();
+  if (!ok) {
+    const long long t0 = clock64();
+    while (!(ok = test())) {
+      if (*stop != 0) break;
+      if (clock64() - t0 > kWaitLimitCycles) {
+        record_error(status, kErrTimeoutProducer);
+        *stop = 1;
+        break;
+      }
+    }
+  }
+  return ok;
+}
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_waits(uint64_t* bar, int parity, volatile int* stop, uint32_t* status) {
+  return __all_sync(0xffffffffu, wait_for<CLUSTER>(bar, parity, stop, status));
+}
+__device__ __forceinline__ void warp_arrives(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 // The elements of a vector as pairs.
 template <typename T>
 __device__ __forceinline__ void to_pairs(const uint4& u, float2 (&p)[Span<T>::kVec / 2]) {
@@ -133,7 +161,7 @@ struct Sums {
   }
   __device__ __forceinline__ void move(float logit, float c) {
     const Ref next(logit, c), next1 = ref_at_one<POW>(next);
-    if (set) {
+    if (set && sum() < CUDART_INF_F) {  // an infinite sum stays one (times a factor that underflows it would be NaN)
       const float2 f = both(fast_exp2(next.log2_of(ref, c)));
       acc[0] = mul2(acc[0], f);
       acc[1] = mul2(acc[1], f);
@@ -189,6 +217,11 @@ struct Sums {
   __device__ __forceinline__ float sum1() const { return (acc1[0].x + acc1[0].y) + (acc1[1].x + acc1[1].y); }
 };
 
+// sum 2^log2; nothing, and infinity, stay what they are.
+__device__ __forceinline__ float rescaled(float sum, float log2) {
+  return sum != 0.f && sum < CUDART_INF_F ? sum * fast_exp2(log2) : sum;
+}
+
 // What a warp's threads have summed, relative to one reference (lane 0 has the sums).
 struct WarpSum {
   float z;  // the reference logit; -inf where the warp has seen no finite logit
@@ -200,13 +233,13 @@ __device__ __forceinline__ WarpSum warp_total(const Sums<POW>& s, float c, float
   w.z = warp_max(s.set ? s.ref.z : -CUDART_INF_F);
   const Ref ref(w.z == -CUDART_INF_F ? 0.f : w.z, c);
   w.sum = s.sum();
-  if (w.sum != 0.f) w.sum *= fast_exp2(ref.log2_of(s.ref, c));
+  w.sum = rescaled(w.sum, ref.log2_of(s.ref, c));
   w.sum = warp_sum(w.sum);
   w.sum1 = 0.f;
   if (POW != 0) {
     const Ref ref1 = ref_at_one<POW>(ref);
     w.sum1 = s.sum1();
-    if (w.sum1 != 0.f) w.sum1 *= fast_exp2(ref1.log2_of(s.ref1, c1));
+    w.sum1 = rescaled(w.sum1, ref1.log2_of(s.ref1, c1));
     w.sum1 = warp_sum(w.sum1);
   }
   return w;

@@ -10,36 +10,14 @@
 // 64-bit key, so the result does not depend on the order of collection.  Rows with so many elements at the bound that
 // the list overflows (ties, rows almost all -inf), and rows with NaN, find the k-th largest key bit by bit.
 #include "../common/host.h"
-#include "distill_api.h"
-#include "row_slice.cuh"
+#include "top_common.cuh"
 
 namespace ttb {
 namespace {
 
 using rows::Slice;
 namespace cg = cooperative_groups;
-
-constexpr int kCapacity = 640;  // collected elements: about 1.7 times the largest k
-
-// Monotone whole number of a float: larger for larger values, -0 = +0, NaN above all.
-__device__ __forceinline__ uint32_t ordered(float v) {
-  if (v != v) return 0xFFFFFFFFu;
-  const uint32_t u = __float_as_uint(v + 0.f);
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float from_ordered(uint32_t o) {
-  return __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
-}
-__device__ __forceinline__ unsigned long long key_of(float v, int col) {
-  return (static_cast<unsigned long long>(ordered(v)) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(col));
-}
-
-// The lowest bit of ordered(v) that values of type T can set (16-bit types widen to floats with zero tails).
-template <typename T>
-constexpr int lowest_bit() {
-  if (std::is_same_v<T, float>) return 0;
-  return std::is_same_v<T, __half> ? 13 : 16;
-}
+using namespace top;
 
 struct Shared {
   uint64_t bars[rows::kStages];
@@ -63,40 +41,6 @@ __device__ __forceinline__ int block_count(int v, int* red) {
   for (int i = 1; i < blockDim.x / 32; ++i) t += red[i];
   __syncthreads();
   return t;
-}
-
-// A value that at least r and, where the values allow it, few more than r of the block's thread maxima reach
-// (0 where fewer than r threads have elements).  One warp; the common leading bits are skipped.
-template <typename T>
-__device__ __forceinline__ uint32_t find_bound(const uint32_t* maxima, int threads, int r) {
-  constexpr int kMost = rows::kMaxThreads / 32;
-  const int lane = threadIdx.x & 31, each = threads / 32;
-  uint32_t m[kMost];
-  uint32_t all = 0xFFFFFFFFu, any = 0u;
-#pragma unroll
-  for (int i = 0; i < kMost; ++i) {
-    m[i] = i < each ? maxima[i * 32 + lane] : 0u;
-    if (i < each) {
-      all &= m[i];
-      any |= m[i];
-    }
-  }
-  all = __reduce_and_sync(0xffffffffu, all);
-  any = __reduce_or_sync(0xffffffffu, any);
-  const uint32_t differ = all ^ any;
-  if (differ == 0 || r > threads) return r > threads ? 0u : all;
-  const int top = 31 - __clz(differ);
-  uint32_t bound = top == 31 ? 0u : all & ~((2u << top) - 1u);
-  for (int bit = top; bit >= lowest_bit<T>(); --bit) {
-    const uint32_t trial = bound | (1u << bit);
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < kMost; ++i) c += m[i] >= trial;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (c >= r) bound = trial;
-    if (c >= r && c <= r + r / 8) break;  // close enough: a higher bound would only shorten the list a little
-  }
-  return bound;
 }
 
 template <typename T>
@@ -311,6 +255,7 @@ void top_logits(const TopLogitsArgs& a, cudaStream_t stream) {
   TTB_CHECK(a.k >= 1 && a.k <= kTopLogitsMaxK && a.k <= a.vocab, "top logits: k must be between 1 and min(256, columns)");
   TTB_CHECK(logits_row_fits(a.vocab, a.type), "top logits: the rows are too long");
   if (a.rows == 0) return;
+  if (top_logits_by_ring(a, stream)) return;
   rows::Plan p = rows::plan_rows(a.rows, a.vocab, scalar_bytes(a.type));
   while (p.threads < rows::kMaxThreads && p.threads < 4 * ((a.k + p.parts - 1) / p.parts)) p.threads *= 2;
   TTB_CHECK(a.rows * p.parts <= 0x7FFFFFFFLL, "top logits: too many rows");

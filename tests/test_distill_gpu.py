@@ -120,6 +120,26 @@ def test_infinities_and_nan(v, dtype):
     _check_top(z, 12)
 
 
+# Many long rows: the persistent kernel
+@pytest.mark.parametrize("dtype,v,ld,offset", [(BF16, 16384, 16384, 0), (BF16, 20001, 20001, 3), (F16, 50257, 50304, 0),
+                                               (F32, 8200, 8200, 0), (F32, 12345, 12345, 2), (F32, 131072, 131072, 0),
+                                               (F16, 300007, 300007, 5)])
+@pytest.mark.parametrize("k", [1, 64, 256])
+def test_top_logits_of_many_rows(dtype, v, ld, offset, k):
+    n = 1501 if v < 30000 else 601
+    z = _logits(n, v, dtype, v + k, ld=ld, offset=offset)
+    z[3] = 0  # ties throughout
+    z[4] = float("-inf")
+    z[5, 100:] = float("-inf")
+    z[6, 7] = float("nan")
+    z[7] = torch.finfo(dtype).min
+    z[8, ::3] = z[8].max() + 1  # more ties at the top than any list holds
+    z[9, [0, v - 1]] = 50.0  # the ends of the row
+    z[10, 5] = float("inf")
+    z[n - 1] = torch.arange(v, device="cuda").to(dtype)
+    _check_top(z, k, tau=1.5)
+
+
 def test_top_logits_of_a_peaked_thread():
     """All large logits in the vectors one thread reads: the bound from thread maxima is then far too low."""
     z = _logits(3, 30000, F32, 2)
