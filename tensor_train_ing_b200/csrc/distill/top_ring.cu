@@ -3,8 +3,8 @@
 //   consumers   stream the rows through a ring of chunks, one after the other without a pause: sums of exponentials and,
 //               for every quarter of a row, the largest element of each thread
 //   producer    keeps the ring full
-//   collectors  behind the consumers: find a bound below the row's k-th largest element from the maxima, read the few
-//               threads' vectors that can reach it again (from L2), rank what is found, write it out
+//   collectors  behind the consumers, a row each: find a bound below the row's k-th largest element from the maxima, read
+//               the few threads' vectors that can reach it again (from L2), rank what is found, write it out
 //
 // No row is kept, so its length does not matter.  8192 rows of 50257 bf16 logits, the top 64, took 264 us with a row per
 // CTA (two CTAs of an SM waiting through the bound, the collection and the ranking of each row) and {CHUNK} us here; 2048 rows of
@@ -26,13 +26,13 @@ using rows::warp_waits;
 
 constexpr int kThreads = 512;
 constexpr int kProducer = kRingWarps, kCollector = kRingWarps + 1;
-constexpr int kTeam = kThreads - 32 * kCollector;  // collector threads
-constexpr int kRounds = 3;                          // vectors of a chunk per consumer thread
+constexpr int kCollectors = kThreads / 32 - kCollector;
+constexpr int kRounds = 2;                          // vectors of a chunk per consumer thread
 constexpr int kChunkVectors = kRounds * kRingThreads;
 constexpr int kSlots = 4;
 constexpr int kParts = 4;  // a row's quarters
 constexpr int kGroups = kParts * kRingThreads;
-constexpr int kSides = 3;  // rows between their sums and their end at one time
+constexpr int kSides = 5;  // rows between their sums and their end at one time
 static_assert(kGroups == 16 * 3 * 32);
 
 struct Shared {
@@ -40,13 +40,9 @@ struct Shared {
   uint64_t sums_ready[kSides], side_free[kSides];
   uint32_t maxima[kSides][kGroups];
   rows::WarpSum sums[kSides][kRingWarps];
-  unsigned long long list[kCapacity];
-  unsigned short hit[kGroups];
-  uint32_t bound;
-  float total;  // the row's sum relative to top
-  float top;
-  int hits, taken;
-  int red[kTeam / 32], ok[kTeam / 32];
+  unsigned long long list[kCollectors][kCapacity];
+  unsigned short hit[kCollectors][kGroups];
+  int taken[kCollectors];
   int stop;
 };
 
@@ -121,95 +117,69 @@ __device__ __forceinline__ void consume(const T* z, long long ldz, long long row
   }
 }
 
-__device__ __forceinline__ void team_barrier() { named_barrier(1, kTeam); }
-
-__device__ __forceinline__ int team_count(int v, int* red, int warp) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) red[warp] = v;
-  team_barrier();
-  int t = 0;
-#pragma unroll
-  for (int i = 0; i < kTeam / 32; ++i) t += red[i];
-  team_barrier();
-  return t;
-}
-
 template <typename T>
 __device__ __forceinline__ void collect(const T* z, long long ldz, long long rows_n, int vocab, int k, float inv_tau,
                                         T* values, int* ids, float* lse, Shared& sh, float c, uint32_t* status) {
   constexpr int E = Span<T>::kVec;
-  const int t = threadIdx.x - 32 * kCollector, lane = t & 31, warp = t >> 5;
+  const int lane = threadIdx.x & 31, me = (threadIdx.x >> 5) - kCollector;
+  unsigned long long* list = sh.list[me];
+  unsigned short* hit_list = sh.hit[me];
+  int& taken = sh.taken[me];
   const auto take = [&](float value, int col) {
-    const int to = atomicAdd(&sh.taken, 1);
-    if (to < kCapacity) sh.list[to] = key_of(value, col);
+    const int to = atomicAdd(&taken, 1);
+    if (to < kCapacity) list[to] = key_of(value, col);
   };
-  int n = 0;
-  for (long long row = blockIdx.x; row < rows_n; row += gridDim.x, ++n) {
+  int n = me;
+  for (long long row = blockIdx.x + static_cast<long long>(me) * gridDim.x; row < rows_n;
+       row += static_cast<long long>(kCollectors) * gridDim.x, n += kCollectors) {
     const int side = n % kSides;
-    const bool ok = warp_waits(&sh.sums_ready[side], (n / kSides) & 1, &sh.stop, status);
-    if (lane == 0) sh.ok[warp] = ok;
-    if (t == 0) sh.hits = sh.taken = 0;
-    team_barrier();
-    bool all_ok = true;
-#pragma unroll
-    for (int i = 0; i < kTeam / 32; ++i) all_ok &= sh.ok[i] != 0;
-    if (!all_ok) return;  // the whole team: none is left at its barrier
+    if (!warp_waits(&sh.sums_ready[side], (n / kSides) & 1, &sh.stop, status)) return;
+    if (lane == 0) taken = 0;
+    __syncwarp();
     const Span<T> s(z + row * ldz, vocab, 0, 1 << 30);
-    if (warp == 0) {
-      const uint32_t bound = find_bound<T, 3>(sh.maxima[side], kGroups, k);
-      if (lane == 0) sh.bound = bound;
-    } else if (warp == 1) {
-      const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
-      const float top = warp_max(w.z);
-      const rows::Ref ref(top == -CUDART_INF_F ? 0.f : top, c), of(w.z == -CUDART_INF_F ? 0.f : w.z, c);
-      const float total = warp_sum(rows::rescaled(w.sum, ref.log2_of(of, c)));
-      if (lane == 0) {
-        sh.total = total;
-        sh.top = ref.z;
-        lse[row] = ref.far ? ref.z * inv_tau + logf(total) : (ref.r + log2f(total)) * CUDART_LN2_F;
-      }
-    }
-    team_barrier();
-    const uint32_t bound = sh.bound;
+    const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
+    const float top = warp_max(w.z);
+    const rows::Ref ref(top == -CUDART_INF_F ? 0.f : top, c), of(w.z == -CUDART_INF_F ? 0.f : w.z, c);
+    const float sum = warp_sum(rows::rescaled(w.sum, ref.log2_of(of, c)));
+    if (lane == 0) lse[row] = ref.far ? ref.z * inv_tau + logf(sum) : (ref.r + log2f(sum)) * CUDART_LN2_F;
+    const uint32_t bound = find_bound<T, 3>(sh.maxima[side], kGroups, k);
     // NaN, or no bound: the k-th largest element is searched bit by bit
-    bool search = sh.total != sh.total || bound <= ordered(-CUDART_INF_F);
+    bool search = sum != sum || bound <= ordered(-CUDART_INF_F);
     if (!search) {
       const float least = from_ordered(bound);
-      for (int g = t; g < kGroups; g += kTeam) {
+      int hits = 0;
+      for (int g = lane; g < kGroups; g += 32) {
         const bool hit = sh.maxima[side][g] >= bound;
         const unsigned who = __ballot_sync(0xffffffffu, hit);
-        if (who == 0) continue;
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&sh.hits, __popc(who));
-        at = __shfl_sync(0xffffffffu, at, 0);
-        if (hit) sh.hit[at + __popc(who & ((1u << lane) - 1u))] = static_cast<unsigned short>(g);
+        if (hit) hit_list[hits + __popc(who & ((1u << lane) - 1u))] = static_cast<unsigned short>(g);
+        hits += __popc(who);
       }
-      const int edge = t < 16 ? s.edge_column(t) : -1;
+      const int edge = lane < 16 ? s.edge_column(lane) : -1;
       if (edge >= 0) {
         const float v = to_f32(s.row[edge]);
         if (v >= least) take(v, edge);
       }
-      team_barrier();
-      // `lanes` threads look through a group's vectors, two groups at a time so that their reads overlap
+      __syncwarp();
+      // `lanes` lanes look through a group's vectors, four groups at a time so that their reads overlap
+      constexpr int U = 4;
       const int chunks = chunks_of(s), each = (chunks + kParts - 1) / kParts, rounds = each * kRounds;
-      const int lanes = rounds <= 8 ? 8 : rounds <= 16 ? 16 : 32, teams = kTeam / lanes;
-      const int hits = sh.hits, in = t % lanes;
-      for (int h = t / lanes; h < hits; h += 2 * teams) {
-        for (int j = in; j < rounds; j += lanes) {
-          uint4 u[2];
-          int first[2];
-          bool have[2];
+      const int lanes = rounds <= 8 ? 8 : rounds <= 16 ? 16 : 32, teams = 32 / lanes;
+      for (int h = lane / lanes; h < hits; h += U * teams) {
+        for (int j = lane % lanes; j < rounds; j += lanes) {
+          uint4 u[U];
+          int first[U];
+          bool have[U];
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
+          for (int b = 0; b < U; ++b) {
             const int hit = h + b * teams;
-            const int g = hit < hits ? sh.hit[hit] : 0, part = g / kRingThreads, who = g % kRingThreads;
+            const int g = hit < hits ? hit_list[hit] : 0, part = g / kRingThreads, who = g % kRingThreads;
             const int v = s.lo + (part * rounds + j) * kRingThreads + who;
             have[b] = hit < hits && v < s.hi;
             first[b] = s.first + v * E;
             if (have[b]) u[b] = __ldg(reinterpret_cast<const uint4*>(s.row + first[b]));
           }
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
+          for (int b = 0; b < U; ++b) {
             if (!have[b]) continue;
             float2 q[E / 2];
             rows::to_pairs<T>(u[b], q);
@@ -221,10 +191,11 @@ __device__ __forceinline__ void collect(const T* z, long long ldz, long long row
           }
         }
       }
-      team_barrier();
-      search = sh.taken > kCapacity;
+      __syncwarp();
+      search = taken > kCapacity;
     }
-    int total = sh.taken;
+    int total = taken;
+    __syncwarp();
     if (search) {
       const int col_bits = 32 - __clz(vocab);  // the column's upper bits are ones in every key
       unsigned long long kth = 0;
@@ -235,29 +206,29 @@ __device__ __forceinline__ void collect(const T* z, long long ldz, long long row
           continue;
         }
         int m = 0;
-        for (int col = t; col < vocab; col += kTeam) m += key_of(to_f32(s.row[col]), col) >= trial;
-        if (team_count(m, sh.red, warp) >= k) kth = trial;
+#pragma unroll 8
+        for (int col = lane; col < vocab; col += 32) m += key_of(to_f32(s.row[col]), col) >= trial;
+        if (__reduce_add_sync(0xffffffffu, m) >= k) kth = trial;
       }
-      if (t == 0) sh.taken = 0;
-      team_barrier();
-      for (int col = t; col < vocab; col += kTeam) {
+      if (lane == 0) taken = 0;
+      __syncwarp();
+      for (int col = lane; col < vocab; col += 32) {
         const float v = to_f32(s.row[col]);
         if (key_of(v, col) >= kth) take(v, col);
       }
-      team_barrier();
+      __syncwarp();
       total = k;
     }
-    for (int i = t; i < total; i += kTeam) {
-      const unsigned long long key = sh.list[i];
+    for (int i = lane; i < total; i += 32) {
+      const unsigned long long key = list[i];
       int place = 0;
-      for (int j = 0; j < total; ++j) place += sh.list[j] > key;
+      for (int j = 0; j < total; ++j) place += list[j] > key;
       if (place < k) {
         values[row * k + place] = from_f32<T>(from_ordered(static_cast<uint32_t>(key >> 32)));
         ids[row * k + place] = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key));
       }
     }
-    team_barrier();  // the list and the counters may be used again
-    if (t == 0) mbar_arrive(&sh.side_free[side]);
+    warp_arrives(&sh.side_free[side]);
   }
 }
 
