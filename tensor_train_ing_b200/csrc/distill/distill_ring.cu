@@ -52,6 +52,7 @@ struct Row {  // what the lister says about a row
   int live, target;
   float mass, rest, target_logit, list_top;
   unsigned edges;  // listed edge columns, by slot
+  float edge[16];  // the edge columns' logits, by slot
   int first;       // column of the slice's first element
   int repeats, target_listed;
   int target_here;  // the CTA has the target's column
@@ -161,6 +162,8 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
       has_target |= col >= 0 && col == target;
     }
     const float target_logit = p.ce != 0.f ? to_f32(s.row[target]) : 0.f;
+    const int edge = lane < 16 ? s.edge_column(lane) : -1;
+    if (edge >= 0) r.edge[lane] = to_f32(s.row[edge]);
     present = __any_sync(0xffffffffu, present);
     has_target = __any_sync(0xffffffffu, has_target);
     top = warp_max(top);
@@ -267,7 +270,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
     }
     const Span<TZ> s(z + row * p.ldz, p.vocab, at.rank, p.per);
     const int edge = tid < 16 ? s.edge_column(tid) : -1;
-    const float edge_z = edge >= 0 ? to_f32(s.row[edge]) : 0.f;
+    const float edge_z = edge >= 0 ? sh.row[side].edge[tid] : 0.f;
 
     rows::Sums<POW> sums(c);
     bool sure = false;  // all threads of the warp have a reference: batches are added without looking for one

@@ -111,6 +111,22 @@ __device__ __forceinline__ void warp_arrives(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+// A load that is issued where it stands (the compiler would move a plain one to its use, where its latency shows).
+template <typename T>
+__device__ __forceinline__ T load_early(const T* p) {
+  T v;
+  if constexpr (sizeof(T) == 4) {
+    uint32_t u;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(u) : "l"(p));
+    v = *reinterpret_cast<const T*>(&u);
+  } else {
+    unsigned short u;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(u) : "l"(p));
+    v = *reinterpret_cast<const T*>(&u);
+  }
+  return v;
+}
+
 // The elements of a vector as pairs.
 template <typename T>
 __device__ __forceinline__ void to_pairs(const uint4& u, float2 (&p)[Span<T>::kVec / 2]) {
@@ -124,6 +140,29 @@ __device__ __forceinline__ void to_pairs(const uint4& u, float2 (&p)[Span<T>::kV
     unpack2<T>(u.w, p[3].x, p[3].y);
   }
 }
+
+// The running maximum of vectors (NaN left out): 16-bit types keep one for each half of a word.
+template <typename T>
+struct RunningMax {
+  uint32_t packed;
+  float wide;
+  __device__ __forceinline__ RunningMax() : packed(0), wide(-__builtin_huge_valf()) {
+    if constexpr (sizeof(T) == 2) packed = pack2<T>(-CUDART_INF_F, -CUDART_INF_F);
+  }
+  __device__ __forceinline__ void take(const uint4& u) {
+    if constexpr (sizeof(T) == 4)
+      wide = fmaxf(wide, fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                               fmaxf(__uint_as_float(u.z), __uint_as_float(u.w))));
+    else
+      packed = max2<T>(packed, max2<T>(max2<T>(u.x, u.y), max2<T>(u.z, u.w)));
+  }
+  __device__ __forceinline__ float get() const {
+    if constexpr (sizeof(T) == 4) return wide;
+    float a, b;
+    unpack2<T>(packed, a, b);
+    return fmaxf(a, b);
+  }
+};
 
 // The largest element of some vectors (NaN left out).
 template <typename T, int N>

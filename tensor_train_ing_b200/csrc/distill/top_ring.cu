@@ -27,13 +27,14 @@ using rows::warp_waits;
 constexpr int kThreads = 512;
 constexpr int kProducer = kRingWarps, kCollector = kRingWarps + 1;
 constexpr int kCollectors = kThreads / 32 - kCollector;
-constexpr int kRounds = 2;                          // vectors of a chunk per consumer thread
+constexpr int kRounds = 5;                          // vectors of a chunk per consumer thread
 constexpr int kChunkVectors = kRounds * kRingThreads;
-constexpr int kSlots = 4;
+constexpr int kSlots = 2;
 constexpr int kParts = 4;  // a row's quarters
 constexpr int kGroups = kParts * kRingThreads;
-constexpr int kSides = 5;  // rows between their sums and their end at one time
+constexpr int kSides = 4;  // rows between their sums and their end at one time
 static_assert(kGroups == 16 * 3 * 32);
+constexpr int kMostHits = 768;  // groups at the bound that are looked through; more (ties) are searched
 
 struct Shared {
   uint64_t full[kSlots], empty[kSlots];
@@ -41,7 +42,7 @@ struct Shared {
   uint32_t maxima[kSides][kGroups];
   rows::WarpSum sums[kSides][kRingWarps];
   unsigned long long list[kCollectors][kCapacity];
-  unsigned short hit[kCollectors][kGroups];
+  unsigned short hit[kCollectors][kMostHits];
   int taken[kCollectors];
   int stop;
 };
@@ -82,35 +83,50 @@ __device__ __forceinline__ void consume(const T* z, long long ldz, long long row
     const int side = n % kSides;
     const Span<T> s(z + row * ldz, vocab, 0, 1 << 30);
     const int edge = tid < 16 ? s.edge_column(tid) : -1;
-    const float edge_z = edge >= 0 ? to_f32(s.row[edge]) : 0.f;
+    const float edge_z = edge >= 0 ? to_f32(rows::load_early(s.row + edge)) : 0.f;
     if (n >= kSides && !warp_waits(&sh.side_free[side], (n / kSides - 1) & 1, &sh.stop, status)) return;
     const int chunks = chunks_of(s), each = (chunks + kParts - 1) / kParts;
     rows::Sums<0> sums(c);
+    bool sure = false;  // all threads of the warp have a reference: vectors are added without looking for one
     int chunk = 0;
 #pragma unroll 1
     for (int part = 0; part < kParts; ++part) {
-      float mx = -CUDART_INF_F;
-      bool any = false;
+      rows::RunningMax<T> mx;
+      const bool any = s.lo + part * each * kChunkVectors + tid < s.hi;
 #pragma unroll 1
       for (const int end = min(chunks, (part + 1) * each); chunk < end; ++chunk, ++q) {
         const unsigned slot = q % kSlots;
         if (!warp_waits(&sh.full[slot], (q / kSlots) & 1, &sh.stop, status)) return;
-        const int have = s.hi - s.lo - chunk * kChunkVectors;
+        const int have = min(s.hi - s.lo - chunk * kChunkVectors, kChunkVectors);
         const T* at = sm + slot * kChunkVectors * Span<T>::kVec;
+        if (sure) {
 #pragma unroll 1
-        for (int i = tid; i < min(have, kChunkVectors); i += kRingThreads) {
-          const uint4 u[1] = {*reinterpret_cast<const uint4*>(at + i * Span<T>::kVec)};
-          const float top = rows::max_of<T>(u);
-          mx = fmaxf(mx, top);
-          any = true;
-          sums.see(top, c);
-          sums.template add_batch<T>(u, c);
+          for (int i = tid; i < have; i += kRingThreads) {
+            const uint4 u[1] = {*reinterpret_cast<const uint4*>(at + i * Span<T>::kVec)};
+            mx.take(u[0]);
+            sums.template add_vectors<T, false>(u, c);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = tid; i < have; i += kRingThreads) {
+            const uint4 u[1] = {*reinterpret_cast<const uint4*>(at + i * Span<T>::kVec)};
+            mx.take(u[0]);
+            sums.see(rows::max_of<T>(u), c);
+            sums.template add_batch<T>(u, c);
+          }
+          sure = __all_sync(0xffffffffu, sums.set && !sums.ref.far);
         }
         warp_arrives(&sh.empty[slot]);
       }
-      sh.maxima[side][part * kRingThreads + tid] = any ? ordered(mx) : 0u;
+      sh.maxima[side][part * kRingThreads + tid] = any ? ordered(mx.get()) : 0u;
     }
     if (edge >= 0) sums.add_one(edge_z, c);
+    if (sums.overflowed()) {  // rare: logits 80 tau above a thread's first ones, infinities, NaN
+      sums = rows::Sums<0>(c);
+      for (int v = s.lo + tid; v < s.hi; v += kRingThreads)
+        for (int e = 0; e < Span<T>::kVec; ++e) sums.add_one(to_f32(s.row[s.first + v * Span<T>::kVec + e]), c);
+      if (edge >= 0) sums.add_one(edge_z, c);
+    }
     const rows::WarpSum mine = rows::warp_total<0>(sums, c, c);
     if (lane == 0) sh.sums[side][warp] = mine;
     warp_arrives(&sh.sums_ready[side]);
@@ -151,9 +167,12 @@ __device__ __forceinline__ void collect(const T* z, long long ldz, long long row
       for (int g = lane; g < kGroups; g += 32) {
         const bool hit = sh.maxima[side][g] >= bound;
         const unsigned who = __ballot_sync(0xffffffffu, hit);
-        if (hit) hit_list[hits + __popc(who & ((1u << lane) - 1u))] = static_cast<unsigned short>(g);
+        const int to = hits + __popc(who & ((1u << lane) - 1u));
+        if (hit && to < kMostHits) hit_list[to] = static_cast<unsigned short>(g);
         hits += __popc(who);
       }
+      search = hits > kMostHits;
+      hits = min(hits, kMostHits);
       const int edge = lane < 16 ? s.edge_column(lane) : -1;
       if (edge >= 0) {
         const float v = to_f32(s.row[edge]);
@@ -192,7 +211,7 @@ __device__ __forceinline__ void collect(const T* z, long long ldz, long long row
         }
       }
       __syncwarp();
-      search = taken > kCapacity;
+      search |= taken > kCapacity;
     }
     int total = taken;
     __syncwarp();
