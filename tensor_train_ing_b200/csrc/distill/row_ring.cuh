@@ -141,26 +141,16 @@ __device__ __forceinline__ void to_pairs(const uint4& u, float2 (&p)[Span<T>::kV
   }
 }
 
-// The running maximum of vectors (NaN left out): 16-bit types keep one for each half of a word.
-template <typename T>
-struct RunningMax {
-  uint32_t packed;
-  float wide;
-  __device__ __forceinline__ RunningMax() : packed(0), wide(-__builtin_huge_valf()) {
-    if constexpr (sizeof(T) == 2) packed = pack2<T>(-CUDART_INF_F, -CUDART_INF_F);
-  }
-  __device__ __forceinline__ void take(const uint4& u) {
-    if constexpr (sizeof(T) == 4)
-      wide = fmaxf(wide, fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
-                               fmaxf(__uint_as_float(u.z), __uint_as_float(u.w))));
-    else
-      packed = max2<T>(packed, max2<T>(max2<T>(u.x, u.y), max2<T>(u.z, u.w)));
-  }
-  __device__ __forceinline__ float get() const {
-    if constexpr (sizeof(T) == 4) return wide;
-    float a, b;
-    unpack2<T>(packed, a, b);
-    return fmaxf(a, b);
+// Over vectors (NaN left out): the largest element, the number of a vector that has it, and the largest element of all
+// other vectors (or the same, where two vectors share it).
+struct Leaders {
+  float most, next;
+  int where;
+  __device__ __forceinline__ Leaders() : most(-__builtin_huge_valf()), next(-__builtin_huge_valf()), where(0) {}
+  __device__ __forceinline__ void take(float vector_max, int number) {
+    next = fmaxf(next, fminf(vector_max, most));
+    if (vector_max > most) where = number;
+    most = fmaxf(most, vector_max);
   }
 };
 

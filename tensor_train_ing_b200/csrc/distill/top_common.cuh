@@ -67,6 +67,23 @@ __device__ __forceinline__ uint32_t find_bound(const uint32_t* maxima, int count
   return bound;
 }
 
+// The same over maxima left in shared memory, one for one: slower, and closer where r is no small part of the count.
+template <typename T>
+__device__ __noinline__ uint32_t find_close_bound(const uint32_t* maxima, int count, int r) {
+  const int lane = threadIdx.x & 31;
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= lowest_bit<T>(); --bit) {
+    const uint32_t trial = bound | (1u << bit);
+    int c = 0;
+#pragma unroll 8
+    for (int i = lane; i < count; i += 32) c += maxima[i] >= trial;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= r) bound = trial;
+    if (c >= r && c <= r + r / 16) break;
+  }
+  return bound;
+}
+
 // The kernel for many long rows (top_ring.cu); false where it does not apply.
 bool top_logits_by_ring(const TopLogitsArgs& a, cudaStream_t stream);
 
