@@ -293,7 +293,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
     if (sums.overflowed()) {  // rare: logits 80 tau above a thread's first ones, infinities, NaN
       const Listed* list = lists + side * p.k;
       sums = rows::Sums<POW>(c);
-      for (int v = s.lo + tid; v < s.hi; v += kRingThreads) {
+      for (int v = tid < s.lo ? tid + kRingThreads : tid; v < s.hi; v += kRingThreads) {
         for (int e = 0; e < E; ++e) {
           const int col = s.first + v * E + e;
           bool out = false;

@@ -4,9 +4,9 @@
 // A row is cut into 16-byte vectors counted from the 16-byte boundary at or below its first element, so that
 // rows at any element offset are copied in whole aligned vectors; the at most two vectors that reach over the
 // row's ends are its edges and are read from global memory element by element.  CTA `rank` of a row has the vectors from
-// rank * per on, and its consumer thread t works on the whole vectors lo + t, lo + t + kRingThreads, ... of them.  They arrive in
-// kStages bulk copies with a barrier each, and a stage's memory is given to the CTA's next row as soon as the last pass
-// over it is done.
+// rank * per on, and its consumer thread t works on the whole ones among the vectors t, t + kRingThreads, ... of them.  They
+// arrive in kStages bulk copies with a barrier each, and a stage's memory is given to the CTA's next row as soon as the
+// last pass over it is done: a stage is therefore the same vectors of the slice in every row, whatever the row's offset.
 #pragma once
 
 #include "row_slice.cuh"
@@ -25,8 +25,7 @@ struct Span {
   int lo, hi;  // its whole vectors: [lo, hi)
   int c0, c1;  // its columns: [c0, c1)
   int off;     // elements between the 16-byte boundary and the row's first element
-  int rounds;  // whole vectors that every thread has; the threads below hi - lo - rounds * threads have one more
-  int stage;   // rounds per stage
+  int stage;   // vectors per stage, a multiple of kRingThreads
 
   __device__ __forceinline__ Span(const T* r, int cols, int rank, int per) {
     constexpr int E = kVec;
@@ -40,14 +39,13 @@ struct Span {
     c1 = max(c0, min(cols, first + nv * E));
     lo = first < 0 ? 1 : 0;
     hi = max(lo, first + nv * E > cols ? nv - 1 : nv);
-    rounds = (hi - lo) / kRingThreads;
-    stage = rounds / kStages + 1;
+    stage = (per + kStages * kRingThreads - 1) / (kStages * kRingThreads) * kRingThreads;
   }
   __device__ __forceinline__ bool holds(int col) const { return col >= c0 && col < c1; }
   // The stage that brings one of the CTA's columns, or kStages for an edge column.
   __device__ __forceinline__ int stage_of(int col) const {
     const int v = (col - first) / kVec;
-    return v >= lo && v < hi ? (v - lo) / (stage * kRingThreads) : kStages;
+    return v >= lo && v < hi ? v / stage : kStages;
   }
   // Edge columns have slots 0..7 (before the first whole vector) and 8..15 (after the last); -1 for no column.
   __device__ __forceinline__ int edge_slot(int col) const {
@@ -61,8 +59,7 @@ struct Span {
   }
   // One thread: starts the copy of stage g into `sm`.
   __device__ __forceinline__ void load_stage(T* sm, uint64_t* bars, int g) const {
-    const int a = lo + g * stage * kRingThreads;
-    const int b = min(hi, a + stage * kRingThreads);
+    const int a = max(lo, g * stage), b = min(hi, (g + 1) * stage);
     if (a < b) {
       mbar_arrive_expect_tx(&bars[g], (b - a) * 16);
       bulk_load(sm + a * kVec, row + first + a * kVec, (b - a) * 16, &bars[g]);
@@ -74,9 +71,11 @@ struct Span {
   // a second copy of them for pairs of vectors costs more in instruction fetches than it gains.
   template <typename F>
   __device__ __forceinline__ void for_stage(const T* sm, int g, F&& f) const {
-    const int last = min(hi, lo + (g + 1) * stage * kRingThreads);
+    const int last = min(hi, (g + 1) * stage);
+    int v = g * stage + static_cast<int>(threadIdx.x);
+    if (v < lo) v += kRingThreads;
 #pragma unroll 1
-    for (int v = lo + static_cast<int>(threadIdx.x) + g * stage * kRingThreads; v < last; v += kRingThreads) {
+    for (; v < last; v += kRingThreads) {
       const uint4 u[1] = {*reinterpret_cast<const uint4*>(sm + v * kVec)};
       f(u, v);
     }

@@ -337,6 +337,23 @@ def test_non_finite_rows_among_many():
     assert a == _ops().distillation_loss(flat, ids, t, lse, reduction="none")[10]
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logits_far_above_a_threads_first_ones(dtype):
+    """Late logits so far above the first that sums relative to these overflow; in many rows and in few."""
+    for n in (700, 5):
+        z = _logits(n, 40009, dtype, 54)
+        ids, t, lse = _teacher(z, 8, F32, 55, True, 1.0)
+        z[::2, 30000:30100] += 300.0
+        z[1, 39000] = 400.0
+        kept = z[3, ids[3].long()].clone()
+        z[3, :20000] = float("-inf")
+        z[3, ids[3].long()] = kept  # a listed column at -inf makes the row's loss infinite
+        _check_loss(z, ids, t, lse, None, 1.0)
+        y = _targets(n, 40009, ids, 56)
+        _check_loss(z, ids, t, lse, y, 2.0, 1.0, 0.5)
+        _check_top(z, 8)
+
+
 def test_types_of_the_list_mix():
     z = _logits(8, 3000, BF16, 6)
     for t_dtype in (F32, BF16, F16):
