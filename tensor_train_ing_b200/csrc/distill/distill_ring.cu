@@ -583,7 +583,9 @@ int active_clusters(const void* kernel, const cudaLaunchConfig_t& cfg, int parts
 }  // namespace
 
 bool loss_by_ring(const DistillArgs& a, const Params& params, int pow, cudaStream_t stream) {
-  constexpr size_t kLeastSlice = 16 * 1024;  // below, several rows per SM hide each other's latencies
+  // Shorter rows go a CTA each, several to an SM.  Measured with 8288 rows, 64 listed: 32 KB (16384 bf16) 135 us here and
+  // 100 us there, with gradient 193 and 154; 64 KB (32768 bf16) 157 and 197, 249 and 282; (16384 fp32) 131 and 199, 229 and 264.
+  constexpr size_t kLeastSlice = 48 * 1024;
   constexpr size_t kMostBytes = 113 * 1024;  // two CTAs on an SM
   const int E = 16 / scalar_bytes(a.z_type);
   const int total = static_cast<int>((a.vocab + 2LL * (E - 1)) / E);  // the most vectors a row can touch

@@ -122,8 +122,8 @@ def test_infinities_and_nan(v, dtype):
 
 # Many long rows: the persistent kernel
 @pytest.mark.parametrize("dtype,v,ld,offset", [(BF16, 16384, 16384, 0), (BF16, 20001, 20001, 3), (F16, 50257, 50304, 0),
-                                               (F32, 8200, 8200, 0), (F32, 12345, 12345, 2), (F32, 131072, 131072, 0),
-                                               (F16, 300007, 300007, 5)])
+                                               (F32, 8200, 8200, 0), (F32, 30001, 30001, 2), (F32, 131072, 131072, 0),
+                                               (BF16, 60003, 60003, 3), (F16, 300007, 300007, 5)])
 @pytest.mark.parametrize("k", [1, 64, 256])
 def test_top_logits_of_many_rows(dtype, v, ld, offset, k):
     n = 1501 if v < 30000 else 601
@@ -291,7 +291,8 @@ def test_loss_of_strided_and_misaligned_rows(dtype, offset, ld):
 # Many long rows: the persistent kernel, of single CTAs and of clusters.  These take several rows each, with and without
 # left-out ones between them; odd widths and offsets give rows with edges on either side.
 @pytest.mark.parametrize("dtype,v,ld,offset", [(BF16, 8192, 8192, 0), (BF16, 9001, 9001, 3), (F16, 20011, 20032, 1),
-                                               (F32, 4100, 4100, 0), (F32, 12345, 12345, 2), (BF16, 50257, 50257, 0),
+                                               (F32, 4100, 4100, 0), (F32, 16001, 16001, 2), (BF16, 50257, 50257, 0),
+                                               (BF16, 30011, 30011, 3), (F16, 40009, 40064, 5), (F32, 20480, 20480, 0),
                                                (F32, 50257, 50257, 1), (F32, 131072, 131072, 0), (F16, 200003, 200003, 5)])
 @pytest.mark.parametrize("k,rest,tau,ce", [(1, False, 1.0, 0.0), (40, True, 2.0, 0.5), (200, True, 1.5, 0.25),
                                            (64, False, 4.0, 0.5)])
@@ -311,19 +312,19 @@ def test_loss_of_many_rows(dtype, v, ld, offset, k, rest, tau, ce):
 
 
 def test_every_row_of_many_left_out():
-    z = _logits(800, 9001, BF16, 50)
+    z = _logits(800, 30011, BF16, 50)
     ids, t, lse = _teacher(z, 8, F32, 51, True, 1.0)
     _check_loss(z, ids, t, lse, torch.full((800,), -100, device="cuda"))
 
 
 def test_non_finite_rows_among_many():
-    z = _logits(700, 9001, F32, 52)
+    z = _logits(700, 20011, F32, 52)
     ids, t, lse = _teacher(z, 8, F32, 53, True, 1.0)
     clean = _ops().distillation_loss(z, ids, t, lse, reduction="none")
     bad = torch.zeros(700, dtype=torch.bool, device="cuda")
     bad[[3, 299, 699]] = True
     zz = z.clone()
-    zz[3, 1], zz[299, 9000], zz[699, 4000] = float("nan"), float("nan"), float("inf")
+    zz[3, 1], zz[299, 20010], zz[699, 4000] = float("nan"), float("nan"), float("inf")
     rows = _ops().distillation_loss(zz, ids, t, lse, reduction="none")
     assert torch.equal(rows[~bad], clean[~bad]) and not torch.isfinite(rows[bad]).any()
     low = z.clone()
