@@ -70,10 +70,11 @@ struct Part {  // what one CTA of the row's knows of its columns: sums at tau an
 
 struct Shared {
   uint64_t full[kStages], ready[kStages], empty[kStages];
-  uint64_t list_ready[kSides], side_free[kSides], sums_ready[kSides], scalars_ready[kSides], gradient_done[kSides], part_ready[kSides];
+  uint64_t list_ready[kSides], side_free[kSides], sums_ready[kSides], scalars_ready[kSides], gradient_done[kSides];
+  uint64_t part_ready[2];
   Row row[kSides];
   Scalars scalars[kSides];
-  Part part[kSides][rows::kMaxParts];
+  Part part[2][rows::kMaxParts];
   rows::WarpSum sums[kSides][kRingWarps];
   int stop;
 };
@@ -273,18 +274,18 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
     const float edge_z = edge >= 0 ? sh.row[side].edge[tid] : 0.f;
 
     rows::Sums<POW> sums(c);
-    bool sure = false;  // all threads of the warp have a reference: batches are added without looking for one
+    bool sure = false;  // all threads of the warp have a reference: vectors are added without looking for one
 #pragma unroll 1
     for (int g = 0; g < kStages; ++g) {
       if (!warp_waits(&sh.ready[g], turn & 1, &sh.stop, p.status)) return;
       if (sure) {
-        s.for_stage(sm, g, [&](const auto& u, int) { sums.template add_vectors<TZ, false>(u, c); });
+        s.for_stage(sm, g, [&](const uint4& u, int) { sums.template add_vector<TZ, false>(u, c); });
       } else {
-        s.for_stage(sm, g, [&](const auto& u, int) {
+        s.for_stage(sm, g, [&](const uint4& u, int) {
           sums.see(rows::max_of<TZ>(u), c);
-          sums.template add_batch<TZ>(u, c);
+          sums.template add_seen<TZ>(u, c);
         });
-        sure = __all_sync(0xffffffffu, sums.set && !sums.ref.far);
+        sure = sums.settle(c);
       }
       if (!GRAD) warp_arrives(&sh.empty[g]);
     }
@@ -294,12 +295,12 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
       const Listed* list = lists + side * p.k;
       sums = rows::Sums<POW>(c);
       for (int v = tid < s.lo ? tid + kRingThreads : tid; v < s.hi; v += kRingThreads) {
-        for (int e = 0; e < E; ++e) {
-          const int col = s.first + v * E + e;
-          bool out = false;
-          for (int i = 0; i < p.k; ++i) out |= list[i].col == col;
-          if (!out) sums.add_one(to_f32(s.row[col]), c);
-        }
+        const int col = s.first + v * E;
+        unsigned out = 0;  // bit e: element e is listed
+        for (int i = 0; i < p.k; ++i)
+          if (const unsigned e = list[i].col - col; e < E) out |= 1u << e;
+        for (int e = 0; e < E; ++e)
+          if (!((out >> e) & 1u)) sums.add_one(to_f32(s.row[col + e]), c);
       }
       if (counted) sums.add_one(edge_z, c);
     }
@@ -326,26 +327,22 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
               ? (reinterpret_cast<uintptr_t>(drow) & 15) / sizeof(TG) == static_cast<uintptr_t>(s.off)
               : s.off == 0 && (reinterpret_cast<uintptr_t>(drow) & (E * sizeof(TG) - 1)) == 0;
       const auto stage = [&](int g, auto far) {
-        s.for_stage(sm, g, [&](const auto& u, int v) {
-          constexpr int N = sizeof(u) / sizeof(uint4);
+        s.for_stage(sm, g, [&](const uint4& u, int v) {
+          float2 q[E / 2];
+          rows::to_pairs<TZ>(u, q);
+          float out[E];
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            float2 q[E / 2];
-            rows::to_pairs<TZ>(u[i], q);
-            float out[E];
+          for (int j = 0; j < E / 2; ++j) {
+            const float2 o = gradient(q[j], far);
+            out[2 * j] = o.x;
+            out[2 * j + 1] = o.y;
+          }
+          TG* to = drow + s.first + v * E;
+          if (same_vectors) {
+            store_vec<E>(to, out);
+          } else {
 #pragma unroll
-            for (int j = 0; j < E / 2; ++j) {
-              const float2 o = gradient(q[j], far);
-              out[2 * j] = o.x;
-              out[2 * j + 1] = o.y;
-            }
-            TG* to = drow + s.first + (v + i * kRingThreads) * E;
-            if (same_vectors) {
-              store_vec<E>(to, out);
-            } else {
-#pragma unroll
-              for (int j = 0; j < E; ++j) to[j] = from_f32<TG>(out[j]);
-            }
+            for (int j = 0; j < E; ++j) to[j] = from_f32<TG>(out[j]);
           }
         });
       };
@@ -433,13 +430,16 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     float rest_top = w.z;
     float2 S2 = relative_sums<POW>(rest_top, w.sum, w.sum1, c, c1);
     if (p.parts > 1) {
+      // Two places by turns of live rows: a CTA writes a place again only after the turn between, for which every CTA
+      // has arrived after it read this one.
       const Part part{rest_top, S2.x, S2.y, L, L1};
+      const int place = turn & 1;
       if (lane < p.parts) {
-        *rows::cg::this_cluster().map_shared_rank(&sh.part[side][at.rank], lane) = part;
-        mbar_arrive_at(&sh.part_ready[side], lane);
+        *rows::cg::this_cluster().map_shared_rank(&sh.part[place][at.rank], lane) = part;
+        mbar_arrive_at(&sh.part_ready[place], lane);
       }
-      if (!warp_waits<true>(&sh.part_ready[side], (on_side >> side) & 1, &sh.stop, p.status)) return;
-      const Part q = lane < p.parts ? sh.part[side][lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0.f};
+      if (!warp_waits<true>(&sh.part_ready[place], (turn >> 1) & 1, &sh.stop, p.status)) return;
+      const Part q = lane < p.parts ? sh.part[place][lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0.f};
       rest_top = q.ref;
       S2 = relative_sums<POW>(rest_top, q.sum, q.sum1, c, c1);
       const float2 L2 = warp_sum2(make_float2(q.list, q.list1));
@@ -538,8 +538,8 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
       mbar_init(&sh.sums_ready[i], kRingWarps);
       mbar_init(&sh.scalars_ready[i], 1);
       mbar_init(&sh.gradient_done[i], kRingWarps);
-      mbar_init(&sh.part_ready[i], p.parts);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.part_ready[i], p.parts);
     sh.stop = 0;
     fence_mbar_init();
   }

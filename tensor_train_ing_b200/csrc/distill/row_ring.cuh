@@ -75,10 +75,7 @@ struct Span {
     int v = g * stage + static_cast<int>(threadIdx.x);
     if (v < lo) v += kRingThreads;
 #pragma unroll 1
-    for (; v < last; v += kRingThreads) {
-      const uint4 u[1] = {*reinterpret_cast<const uint4*>(sm + v * kVec)};
-      f(u, v);
-    }
+    for (; v < last; v += kRingThreads) f(*reinterpret_cast<const uint4*>(sm + v * kVec), v);
   }
 };
 
@@ -153,30 +150,23 @@ struct Leaders {
   }
 };
 
-// The largest element of some vectors (NaN left out).
-template <typename T, int N>
-__device__ __forceinline__ float max_of(const uint4 (&u)[N]) {
+// The largest element of a vector (NaN left out).
+template <typename T>
+__device__ __forceinline__ float max_of(const uint4& u) {
   if constexpr (sizeof(T) == 4) {
-    float m = -CUDART_INF_F;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u[i].x), __uint_as_float(u[i].y)),
-                         fmaxf(__uint_as_float(u[i].z), __uint_as_float(u[i].w))));
-    return m;
+    return fmaxf(fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                       fmaxf(__uint_as_float(u.z), __uint_as_float(u.w))), -CUDART_INF_F);
   } else {
-    uint32_t m = max2<T>(max2<T>(u[0].x, u[0].y), max2<T>(u[0].z, u[0].w));
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = max2<T>(m, max2<T>(max2<T>(u[i].x, u[i].y), max2<T>(u[i].z, u[i].w)));
     float a, b;
-    unpack2<T>(m, a, b);
+    unpack2<T>(max2<T>(max2<T>(u.x, u.y), max2<T>(u.z, u.w)), a, b);
     return fmaxf(fmaxf(a, b), -CUDART_INF_F);  // two NaN halves give -inf
   }
 }
 
 // A thread's running sums of exp((z - ref) / tau) and, for POW > 0, exp(z - ref), over whatever it has seen.  The
-// reference is the largest logit of its first batch that has one.  While `see` is called before every batch it moves when a
-// batch exceeds it by more than 2^40, so that no sum can overflow; batches added without have no maximum to take, which
-// is a fifth of the work and a branch that keeps the next batch's loads and exponentials from starting, but may overflow
+// reference is the largest logit of its first vector that has one.  While `see` is called before every vector it moves when
+// one exceeds it by more than 2^40, so that no sum can overflow; vectors added without have no maximum to take, which
+// is a fifth of the work and a branch that keeps the next one's loads and exponentials from starting, but may overflow
 // where a logit exceeds the reference by more than 2^120: then `overflowed`, and the sums have to be taken again.
 template <int POW>
 struct Sums {
@@ -208,6 +198,12 @@ struct Sums {
   __device__ __forceinline__ void see(float top, float c) {
     if ((!set || ref.log2_of(top, c) > 40.f) && fabsf(top) < CUDART_INF_F) move(top, c);
   }
+  // Whether vectors may be added without `see` from here on: all of the warp's threads have ordinary references.  One far
+  // below the warp's largest (a thread whose first vectors are masked) moves there, so that it will not overflow.
+  __device__ __forceinline__ bool settle(float c) {
+    see(warp_max(set ? ref.z : -CUDART_INF_F), c);
+    return __all_sync(0xffffffffu, set && !ref.far);
+  }
   template <bool FAR>
   __device__ __forceinline__ void add(float2 z, int i, float c) {
     const float2 e = exp2_pair(log2_pair<FAR>(z, both(c), both(FAR ? -ref.z : -ref.r)));
@@ -215,22 +211,19 @@ struct Sums {
     if constexpr (POW == 2) acc1[i & 1] = fma2(e, e, acc1[i & 1]);
     if constexpr (POW == 1 || POW == 4) acc1[i & 1] = add2(acc1[i & 1], at_one<POW, FAR>(e, z, ref1));
   }
-  template <typename T, bool FAR, int N>
-  __device__ __forceinline__ void add_vectors(const uint4 (&u)[N], float c) {
+  template <typename T, bool FAR>
+  __device__ __forceinline__ void add_vector(const uint4& u, float c) {
+    float2 q[Span<T>::kVec / 2];
+    to_pairs<T>(u, q);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      float2 q[Span<T>::kVec / 2];
-      to_pairs<T>(u[n], q);
-#pragma unroll
-      for (int i = 0; i < Span<T>::kVec / 2; ++i) add<FAR>(q[i], i, c);
-    }
+    for (int i = 0; i < Span<T>::kVec / 2; ++i) add<FAR>(q[i], i, c);
   }
-  template <typename T, int N>
-  __device__ __forceinline__ void add_batch(const uint4 (&u)[N], float c) {
+  template <typename T>
+  __device__ __forceinline__ void add_seen(const uint4& u, float c) {
     if (ref.far)
-      add_vectors<T, true>(u, c);
+      add_vector<T, true>(u, c);
     else
-      add_vectors<T, false>(u, c);
+      add_vector<T, false>(u, c);
   }
   __device__ __forceinline__ void add_one(float z, float c) {
     see(z, c);

@@ -105,20 +105,20 @@ __device__ __forceinline__ void consume(const T* z, long long ldz, long long row
         if (sure) {
 #pragma unroll 1
           for (int i = tid; i < have; i += kRingThreads) {
-            const uint4 u[1] = {*reinterpret_cast<const uint4*>(at + i * Span<T>::kVec)};
+            const uint4 u = *reinterpret_cast<const uint4*>(at + i * Span<T>::kVec);
             lead.take(rows::max_of<T>(u), number++);
-            sums.template add_vectors<T, false>(u, c);
+            sums.template add_vector<T, false>(u, c);
           }
         } else {
 #pragma unroll 1
           for (int i = tid; i < have; i += kRingThreads) {
-            const uint4 u[1] = {*reinterpret_cast<const uint4*>(at + i * Span<T>::kVec)};
+            const uint4 u = *reinterpret_cast<const uint4*>(at + i * Span<T>::kVec);
             const float top = rows::max_of<T>(u);
             lead.take(top, number++);
             sums.see(top, c);
-            sums.template add_batch<T>(u, c);
+            sums.template add_seen<T>(u, c);
           }
-          sure = __all_sync(0xffffffffu, sums.set && !sums.ref.far);
+          sure = sums.settle(c);
         }
         warp_arrives(&sh.empty[slot]);
       }

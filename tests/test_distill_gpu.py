@@ -338,6 +338,30 @@ def test_non_finite_rows_among_many():
     assert a == _ops().distillation_loss(flat, ids, t, lse, reduction="none")[10]
 
 
+@pytest.mark.parametrize("keep", [1, 2, 5])
+def test_clusters_that_leave_out_most_rows(keep):
+    z = _logits(1200, 50257, F32, 57)
+    ids, t, lse = _teacher(z, 16, F32, 58, True, 2.0)
+    y = _targets(1200, 50257, ids, 59)
+    stride = torch.arange(1200, device="cuda") // 100  # rows of one cluster lie about a hundred apart
+    y[(stride % 6) >= keep] = -100
+    _check_loss(z, ids, t, lse, y, 2.0, 1.0, 0.5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [-1e4, -3e38, float("-inf")])
+def test_rows_masked_at_their_start(dtype, low):
+    z = _logits(700, 40009, dtype, 60)
+    ids, t, lse = _teacher(z[:, 9000:].contiguous(), 8, F32, 61, True, 1.0)
+    ids = torch.where(ids >= 0, ids + 9000, ids)
+    z[:, :9000] = low
+    y = torch.where(ids[:, 0] >= 0, ids[:, 0].long(), 30000)
+    y[::3] = 20000
+    _check_loss(z, ids, t, lse, y, 2.0, 1.0, 0.5)
+    _check_loss(z, ids, t, lse, None, 1.0)
+    _check_top(z, 8)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_logits_far_above_a_threads_first_ones(dtype):
     """Late logits so far above the first that sums relative to these overflow; in many rows and in few."""
