@@ -380,7 +380,7 @@ __device__ __forceinline__ float2 warp_sum2(float2 v) {
 template <int POW>
 __device__ __forceinline__ float2 relative_sums(float& top, float sum, float sum1, float c, float c1) {
   const Ref of(top == -CUDART_INF_F ? 0.f : top, c);
-  top = warp_max(top);
+  top = rows::lanes_max(top);
   const Ref to(top == -CUDART_INF_F ? 0.f : top, c);
   sum = rows::rescaled(sum, to.log2_of(of, c));
   if (POW != 0) sum1 = rows::rescaled(sum1, rows::ref_at_one<POW>(to).log2_of(rows::ref_at_one<POW>(of), c1));

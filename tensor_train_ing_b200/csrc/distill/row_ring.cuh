@@ -123,6 +123,12 @@ __device__ __forceinline__ T load_early(const T* p) {
   return v;
 }
 
+// The largest of the lanes' values (none NaN), in one instruction.
+__device__ __forceinline__ float lanes_max(float v) {
+  asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+  return v;
+}
+
 // The elements of a vector as pairs.
 template <typename T>
 __device__ __forceinline__ void to_pairs(const uint4& u, float2 (&p)[Span<T>::kVec / 2]) {
@@ -201,7 +207,7 @@ struct Sums {
   // Whether vectors may be added without `see` from here on: all of the warp's threads have ordinary references.  One far
   // below the warp's largest (a thread whose first vectors are masked) moves there, so that it will not overflow.
   __device__ __forceinline__ bool settle(float c) {
-    see(warp_max(set ? ref.z : -CUDART_INF_F), c);
+    see(lanes_max(set ? ref.z : -CUDART_INF_F), c);
     return __all_sync(0xffffffffu, set && !ref.far);
   }
   template <bool FAR>
@@ -251,7 +257,7 @@ struct WarpSum {
 template <int POW>
 __device__ __forceinline__ WarpSum warp_total(const Sums<POW>& s, float c, float c1) {
   WarpSum w;
-  w.z = warp_max(s.set ? s.ref.z : -CUDART_INF_F);
+  w.z = lanes_max(s.set ? s.ref.z : -CUDART_INF_F);
   const Ref ref(w.z == -CUDART_INF_F ? 0.f : w.z, c);
   w.sum = s.sum();
   w.sum = rescaled(w.sum, ref.log2_of(s.ref, c));
