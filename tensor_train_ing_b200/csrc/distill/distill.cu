@@ -17,6 +17,10 @@
 // same (0), e^2 or e^4 for the temperatures 2 and 4 (a product is cheaper than a second exponential: the
 // special-function unit gives 16 a cycle and SM, and two more per element would bound 16-bit logits), else (1) by
 // another exponential.
+//
+// Few rows, and rows shorter than the persistent kernel's.  Bound by what a row waits for: its copy, the list, and the three
+// barriers between maximum, sums and gradient, filled only by the SM's other CTAs.  8288 rows of 16384 bf16 logits, 64 listed:
+// 100 us for the loss (42 us for the bytes), 154 us with the gradient (83 us).
 #include "../common/host.h"
 #include "distill_common.cuh"
 

@@ -212,9 +212,11 @@ __global__ void __launch_bounds__(kThreads) layer_norm_bwd_kernel(
 constexpr int kMaxSlots = 8;
 
 // Elements of a row a thread holds.  What a warp does once per row (sums across lanes and warps, waiting for the slot)
-// costs as much as about 20 elements per lane, so few warps with much of a row each beat many with little: the forward at
-// 2048 columns took 61 us with 8 elements (2450 instructions per row) and {FWD} us with 32; the backward, which also
-// holds its columns' sums, {BWD8} us with 8 and {BWD} us with 16.
+// costs as much as about 20 elements per lane, so few warps with much of a row each beat many with little.  16384 rows
+// of 2048 fp32 columns to bf16 (bytes alone: 31 us): the forward took 61 us with 8 elements a thread, 46 us with 32 and 41 us
+// with 64.  The backward also holds its columns' sums of dw and db, so 128 registers end at 24 elements: 78 us with
+// 8, 66 us with 16, 61 us with 24 (51 us for its bytes); 8192 rows of 6144 bf16 columns 81 us (46 us).  It is bound by each
+// row's chain of loads, sums across warps and stores, of which an SM has two (6144 columns) or four (2048) under way.
 constexpr int kFwdPerThread = 64, kBwdPerThread = 24;
 constexpr int kFwdBlocks = 1, kBwdBlocks = 1;  // of 512 threads that fit an SM then
 
