@@ -293,7 +293,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
     }
     const bool counted = edge >= 0 && !((sh.row[side].edges >> tid) & 1u);
     if (counted) sums.add_one(edge_z, c);
-    if (sums.overflowed()) {  // rare: logits 80 tau above a thread's first ones, infinities, NaN
+    if (sums.overflowed()) {  // rare: logits 40 tau above a thread's first ones, infinities, NaN
       const Listed* list = lists + side * p.k;
       sums = rows::Sums<POW>(c);
       for (int v = tid < s.lo ? tid + kRingThreads : tid; v < s.hi; v += kRingThreads) {

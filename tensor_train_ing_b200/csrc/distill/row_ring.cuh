@@ -171,9 +171,15 @@ __device__ __forceinline__ float max_of(const uint4& u) {
 
 // A thread's running sums of exp((z - ref) / tau) and, for POW > 0, exp(z - ref), over whatever it has seen.  The
 // reference is the largest logit of its first vector that has one.  While `see` is called before every vector it moves when
-// one exceeds it by more than 2^40, so that no sum can overflow; vectors added without have no maximum to take, which
-// is a fifth of the work and a branch that keeps the next one's loads and exponentials from starting, but may overflow
-// where a logit exceeds the reference by more than 2^120: then `overflowed`, and the sums have to be taken again.
+// one exceeds it by more than 2^40; vectors added without have no maximum to take, which is a fifth of the work and a
+// branch that keeps the next one's loads and exponentials from starting, but their sums may grow past kSafeSum: then
+// `overflowed`, and the sums have to be taken again.
+//
+// kSafeSum lies far below the largest fp32 number because of what is made of the sums.  The sums of 384 threads and 8 CTAs
+// add up to less than 2^72; 1 / sum, times a loss scale and a weight, stays a normal number and its quotient in the range
+// of the fast division (denominators up to 2^126); and a sum that another's larger reference scales by less
+// than 2^-126, that is to zero, is below 2^-54 of that other's.
+constexpr float kSafeSum = 1.152921504606846976e18f;  // 2^60
 template <int POW>
 struct Sums {
   Ref ref, ref1;
@@ -239,7 +245,7 @@ struct Sums {
     else
       add<false>(pair, 0, c);
   }
-  __device__ __forceinline__ bool overflowed() const { return !(sum() < CUDART_INF_F) || !(sum1() < CUDART_INF_F); }
+  __device__ __forceinline__ bool overflowed() const { return !(sum() < kSafeSum) || !(sum1() < kSafeSum); }
   __device__ __forceinline__ float sum() const { return (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y); }
   __device__ __forceinline__ float sum1() const { return (acc1[0].x + acc1[0].y) + (acc1[1].x + acc1[1].y); }
 };

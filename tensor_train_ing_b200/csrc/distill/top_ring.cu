@@ -127,7 +127,7 @@ __device__ __forceinline__ void consume(const T* z, long long ldz, long long row
       sh.others[side][part * kRingThreads + tid] = (ordered(lead.next) & 0xFFFF0000u) | static_cast<uint32_t>(lead.where);
     }
     if (edge >= 0) sums.add_one(edge_z, c);
-    if (sums.overflowed()) {  // rare: logits 80 tau above a thread's first ones, infinities, NaN
+    if (sums.overflowed()) {  // rare: logits 40 tau above a thread's first ones, infinities, NaN
       sums = rows::Sums<0>(c);
       for (int v = s.lo + tid; v < s.hi; v += kRingThreads)
         for (int e = 0; e < Span<T>::kVec; ++e) sums.add_one(to_f32(s.row[s.first + v * Span<T>::kVec + e]), c);
