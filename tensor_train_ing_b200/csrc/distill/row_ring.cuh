@@ -171,9 +171,9 @@ __device__ __forceinline__ float max_of(const uint4& u) {
 
 // A thread's running sums of exp((z - ref) / tau) and, for POW > 0, exp(z - ref), over whatever it has seen.  The
 // reference is the largest logit of its first vector that has one.  While `see` is called before every vector it moves when
-// one exceeds it by more than 2^40; vectors added without have no maximum to take, which is a fifth of the work and a
-// branch that keeps the next one's loads and exponentials from starting, but their sums may grow past kSafeSum: then
-// `overflowed`, and the sums have to be taken again.
+// one exceeds it by more than 2^40, at the temperature or at 1, so that no element adds more to either sum.  Vectors added
+// without have no maximum to take, which is a fifth of the work and a branch that keeps the next one's loads and
+// exponentials from starting, but their sums may grow past kSafeSum: then `overflowed`, and the sums have to be taken again.
 //
 // kSafeSum lies far below the largest fp32 number because of what is made of the sums.  The sums of 384 threads and 8 CTAs
 // add up to less than 2^72; 1 / sum, times a loss scale and a weight, stays a normal number and its quotient in the range
@@ -206,9 +206,14 @@ struct Sums {
     ref1 = next1;
     set = true;
   }
+  // 40, as an exponent at the temperature: an exponential at 1 has tau times the exponent (tau = log2(e) / c).
+  __device__ __forceinline__ static float most_above(float c) {
+    if (POW == 0) return 40.f;
+    return POW == 1 ? 40.f * fminf(1.f, c * CUDART_LN2_F) : 40.f / POW;
+  }
   // before adding logits of which `top` is the largest
   __device__ __forceinline__ void see(float top, float c) {
-    if ((!set || ref.log2_of(top, c) > 40.f) && fabsf(top) < CUDART_INF_F) move(top, c);
+    if ((!set || ref.log2_of(top, c) > most_above(c)) && fabsf(top) < CUDART_INF_F) move(top, c);
   }
   // Whether vectors may be added without `see` from here on: all of the warp's threads have ordinary references.  One far
   // below the warp's largest (a thread whose first vectors are masked) moves there, so that it will not overflow.

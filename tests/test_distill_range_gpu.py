@@ -27,7 +27,8 @@ def _masked_rows(n, dtype, seed):
 # 700 rows go to the persistent kernels (CTAs of their own for bf16, clusters for fp32), 91 to those of few rows
 @pytest.mark.parametrize("n", [700, 91])
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("tau,ce", [(1.0, 0.0), (1.0, 0.5), (0.5, 0.5), (1.5, 0.5), (2.0, 0.5), (4.0, 0.0)])
+@pytest.mark.parametrize("tau,ce", [(1.0, 0.0), (1.0, 0.5), (0.5, 0.5), (1.5, 0.5), (2.0, 0.5), (3.5, 0.5), (4.0, 0.0),
+                                    (4.0, 0.5), (8.0, 0.5), (30.0, 0.5)])
 def test_finite_masks_at_every_depth(n, dtype, tau, ce):
     z = _masked_rows(n, dtype, 70)
     ids, t, lse = _teacher(z, 12, F32, 71, True, tau)
