@@ -335,8 +335,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
       S = 0.f;
       for (int q = 0; q < parts; ++q)
         if (sh.again_part[q].rest != 0.f) S += sh.again_part[q].rest * exp2f(own.log2_of(sh.again_part[q].ref, c));
-      // (natural units: c times the type's lowest value is no fp32 number)
-      finish(own, S, logf(S) + (own.z - top.z) * p.inv_tau - logf(total));
+      finish(own, S, logf(S) + top.log_of(own, c, p.inv_tau) - logf(total));
     }
     __syncthreads();
   }

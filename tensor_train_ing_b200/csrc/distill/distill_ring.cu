@@ -487,7 +487,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     if (lane == 0 && at.rank == 0) {
       if (m > 0.f)  // log q_rest from its parts where the probability itself leaves fp32's range
         kl += m * (f > 1e-30f ? logf(m / (S * f * inv_sum))
-                              : logf(m) - (logf(S) + (own.z - ref.z) * p.inv_tau - logf(total)));
+                              : logf(m) - (logf(S) + ref.log_of(own, c, p.inv_tau) - logf(total)));
       float loss = p.kd != 0.f ? p.kd * p.tau * p.tau * kl : 0.f;
       if (p.ce != 0.f) loss += p.ce * (log2f(total1) - ref1.log2_of(r.target_logit, c1)) * CUDART_LN2_F;
       p.loss[r.row] = scale * loss;

@@ -176,22 +176,29 @@ __device__ __forceinline__ void load_pairs(const Slice<T>& s, int v, float2 (&p)
 
 // Exponentials are taken as powers of two of z c - r, c = log2(e) / tau, in one fused multiply-add: r is the fp32
 // number nearest to (largest logit) c, and everything about a row is kept relative to 2^r, so r's rounding
-// cancels.  Where the largest logit is so large in size that the product could overflow (rows at the type's lowest value), z is
-// instead compared with the logit itself first.
+// cancels.  That takes an r whose rounding is small itself: at a product of 2^24 it is up to 1/2, and at 2^34 (a row
+// masked with -1e10) it would be an exponent of 512.  From 2^24 on, at the temperature or at 1, z is instead compared with the logit
+// itself first, and everything is relative to exp(logit / tau).
 struct Ref {
   float z, r;  // the reference logit and z c
-  bool far;    // |z c| is no ordinary number
+  bool far;    // compared by logits
   __device__ __forceinline__ Ref() {}
   __device__ __forceinline__ Ref(float zmax, float c) {
     z = isfinite(zmax) ? zmax : 0.f;
-    far = !(fabsf(z * c) < 1e30f);
+    far = !(fabsf(z) * fmaxf(c, CUDART_L2E_F) < 16777216.f);
     r = z * c;
   }
   // log2 of exp((v - reference) / tau)
   __device__ __forceinline__ float log2_of(float v, float c) const { return far ? (v - z) * c : fmaf(v, c, -r); }
-  // ... of another reference, of the same row and so of the same kind or infinitely far below
+  // log2 of exp(logit / tau) over what the reference stands for, exactly
+  __device__ __forceinline__ float excess(float c) const { return far ? 0.f : fmaf(z, c, -r); }
+  // log2 of another reference, of the same row, over this one
   __device__ __forceinline__ float log2_of(const Ref& o, float c) const {
-    return far || o.far ? (o.z - z) * c : o.r - r;
+    return far || o.far ? fmaf(o.z - z, c, excess(c) - o.excess(c)) : o.r - r;
+  }
+  // the natural logarithm of the same (c times the type's lowest value is no fp32 number)
+  __device__ __forceinline__ float log_of(const Ref& o, float c, float inv_tau) const {
+    return fmaf(o.z - z, inv_tau, (excess(c) - o.excess(c)) * CUDART_LN2_F);
   }
 };
 
@@ -205,8 +212,8 @@ __device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(fast_
 // The reference at temperature 1 that goes with `ref` at tau: with e^POW for the exponentials, exactly POW times it.
 template <int POW>
 __device__ __forceinline__ Ref ref_at_one(const Ref& ref) {
-  if constexpr (POW == 1) return Ref(ref.z, CUDART_L2E_F);
   Ref r = ref;
+  if constexpr (POW == 1) r.r = ref.z * CUDART_L2E_F;
   if constexpr (POW > 1) r.r = POW * ref.r;
   return r;
 }
