@@ -10,8 +10,8 @@
 //     exp((z_j - R) / tau) A + exp(z_j - R) B,
 //     A = scale kd tau ((P + m) / T - m / S),  S, T = sums of exp((z - R) / tau) over the rest and the row
 //     B = scale ce / T1,                       T1 = sum of exp(z - R) over the row
-// and the few listed columns and the target are written after the others.  Should S vanish in fp32 because the rest lies
-// far below the list, it is summed again relative to the rest's own largest logit.
+// and the few listed columns and the target are written after the others.  Where the rest lies so far below the list that S or
+// much of it vanishes in fp32, it is summed again relative to the rest's own largest logit.
 //
 // POW: how exp(z - R) of the cross-entropy follows from e = exp((z - R) / tau) of the divergence: not needed or the
 // same (0), e^2 or e^4 for the temperatures 2 and 4 (a product is cheaper than a second exponential: the
@@ -35,6 +35,10 @@ using distill::zero_row;
 
 using rows::Slice;
 namespace cg = cooperative_groups;
+
+// Below this the rest's sum is taken again relative to its own largest logit.  Exponentials vanish below 2^-126; of a sum
+// of 2^-64 and more what vanished is less than 2^-62 an element, less than 2^-42 in all.
+constexpr float kLeastRestSum = 5.421010862427522e-20f;  // 2^-64
 
 struct Part {  // what one CTA knows of its slice; sums are relative to its references at tau and at 1
   rows::Ref ref, ref1;
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     total1 = POW != 0 ? S1 + L1 : total;
     // a list that names every column leaves no rest, whatever rounding says
     m = p.k >= p.vocab && all_listed >= p.vocab ? 0.f : sh.rest;
-    const bool again = m > 0.f && S < 1e-30f;
+    const bool again = m > 0.f && S < kLeastRestSum;
     if (lane == 0) sh.again = again;
     if (!again) finish(top, S, logf(S / total));
   }

@@ -134,3 +134,17 @@ def test_only_the_listed_logits_are_not_masked(n, dtype, tau):
     listed = tau * (q * (p.sum(1) + m)[:, None] - p)
     tol = tau * 64 * U * (1 + 20) * (q + p) + half * listed.abs()
     assert ((got.gather(1, ids.long()).double() - listed).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [700, 3])
+def test_a_rest_far_below_the_list(n):
+    """The unlisted logits' mass lies e^-68.9 below the list's largest logit, one column of it far above the others, whose
+    exponentials relative to the list vanish in fp32 (2^-126) although they are a thousandth of that mass."""
+    v = 131072
+    z = torch.full((n, v), -87.45, device="cuda")
+    z[:, 70000] = -68.95
+    ids = torch.tensor([[0, 5, 131071]], dtype=torch.int32, device="cuda").repeat(n, 1)
+    z[:, ids[0].long()] = torch.tensor([0.0, -1.0, -2.0], device="cuda")
+    t = torch.tensor([[1.0, 0.5, 0.0]], device="cuda").repeat(n, 1)
+    lse = torch.logsumexp(t, 1) + 0.3
+    _compare(z, z, ids, t, lse, None, 1.0, 1.0, 0.0)
