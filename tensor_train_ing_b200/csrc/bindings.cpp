@@ -310,6 +310,31 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x, const Tens
 // ops/_ext.py adds them to those of the bindings).
 std::atomic<int64_t> autograd_launches{0};
 
+// The history of gradients that the nodes below return while a graph of the backward is recorded (create_graph): it leads to
+// all that they depend on, and refuses to be differentiated.  Without it such gradients would count as constants.
+struct FirstDerivativeOnly : torch::autograd::Node {
+  FirstDerivativeOnly(const char* op, torch::autograd::edge_list&& inputs) : Node(std::move(inputs)), op(op) {}
+  torch::autograd::variable_list apply(torch::autograd::variable_list&&) override {
+    TORCH_CHECK(false, op, ": its kernels form no second derivative");
+  }
+  const char* op;
+};
+void refuse_second_derivative(const char* op, const Tensor& incoming, torch::autograd::variable_list& gradients) {
+  if (!at::GradMode::is_enabled()) return;
+  const auto node = torch::autograd::get_current_node();
+  TORCH_CHECK(node != nullptr, op, ": a backward that records a graph outside the autograd engine");
+  torch::autograd::edge_list inputs = node->next_edges();
+  if (incoming.requires_grad()) inputs.push_back(torch::autograd::impl::gradient_edge(incoming));
+  const std::shared_ptr<torch::autograd::Node> history(new FirstDerivativeOnly(op, std::move(inputs)),
+                                                       torch::autograd::deleteNode);
+  for (Tensor& g : gradients)
+    if (g.defined()) torch::autograd::create_gradient_edge(g, history);
+}
+
+void refuse_tangent(const char* op, const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), op, ": its kernels form no forward-mode derivative");
+}
+
 // layer_norm with its backward as a node of the graph.  Node and call are C++: at small sizes the time of a call is the
 // host's, and a Python autograd function costs more of it than both kernels.
 struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
@@ -329,13 +354,18 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     if (dy.size(1) > 1 && dy.stride(1) != 1) dy = dy.contiguous();
     const auto r = layer_norm_bwd(dy, saved[0], saved[1], saved[2]);
     if (saved[0].size(0) > 0) autograd_launches += 2;
-    return {r[0], r[1], ctx->saved_data["bias"].toBool() ? r[2] : Tensor(), Tensor(), Tensor()};
+    torch::autograd::variable_list out{r[0], r[1], ctx->saved_data["bias"].toBool() ? r[2] : Tensor(), Tensor(), Tensor()};
+    refuse_second_derivative("layer_norm", grads[0], out);
+    return out;
   }
 };
 
 // x [N, d] -> y [N, d], differentiable where gradients are recorded.
 Tensor layer_norm(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& b, double eps,
                   torch::ScalarType out) {
+  refuse_tangent("layer_norm", x);
+  refuse_tangent("layer_norm", w);
+  if (b.has_value()) refuse_tangent("layer_norm", *b);
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (b.has_value() && b->requires_grad())))
     return LayerNormNode::apply(x, w, b, eps, static_cast<int64_t>(out));
   return layer_norm_fwd(x, w, b, eps, out, false)[0];
@@ -463,6 +493,7 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
     if (dz.size(0) > 0) autograd_launches += 1;
     torch::autograd::variable_list out(10);
     out[0] = dz;
+    refuse_second_derivative("distillation_loss", grads[0], out);
     return out;
   }
 };
@@ -471,6 +502,7 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
 Tensor distillation(const Tensor& z, const Tensor& ids, const Tensor& t, const c10::optional<Tensor>& teacher_lse,
                     const c10::optional<Tensor>& targets, double tau, double kd, double ce,
                     const c10::optional<Tensor>& scale, bool total) {
+  refuse_tangent("distillation_loss", z);
   if (at::GradMode::is_enabled() && z.requires_grad())
     return DistillNode::apply(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, total);
   const Tensor loss = distill_loss(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, c10::nullopt);

@@ -24,7 +24,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     x's), dense.  Statistics and sums are fp32; the result is rounded once.  Runs on the current stream.
 
     Differentiable with respect to ``x``, ``weight`` and ``bias``: the backward reads ``x`` again with the forward's
-    per-row mean and rstd, and sums the weight and bias gradients in a fixed order (the same inputs give the same bits)."""
+    per-row mean and rstd, and sums the weight and bias gradients in a fixed order (the same inputs give the same bits).
+    Second derivatives and forward-mode tangents are refused (``models.normalization.LayerNorm.plain`` has them)."""
     if not x.is_cuda:
         raise ValueError("layer_norm: x must be a CUDA tensor (models.normalization.LayerNorm has the CPU form)")
     out_dtype = x.dtype if out_dtype is None else out_dtype

@@ -619,3 +619,32 @@ def test_refusals():
         with pytest.raises(kind, match=text):
             call()
     assert torch.isfinite(d.distillation_loss(z, ids, t))  # refused calls leave the context usable
+
+
+# The loss forms first derivatives.  A second one, or a tangent, is refused and never left out of a sum.
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_second_derivatives_are_refused(reduction, dtype):
+    z = _logits(6, 900, dtype, 32).requires_grad_(True)
+    ids, t, lse = _teacher(z, 6, F32, 33, True, 1.0)
+    s = torch.ones((), device="cuda", requires_grad=True)
+    loss = lambda: _ops().distillation_loss(z, ids, t, lse, reduction=reduction).sum()  # noqa: E731
+    (want,) = torch.autograd.grad(loss(), z)
+    for leaf in (z, s):
+        first = loss()
+        (g,) = torch.autograd.grad(first * s, z, create_graph=True)
+        assert torch.equal(g, want)
+        for objective in (g.float().square().sum(), first.detach() * s + z.sum() + g.float().square().sum()):
+            with pytest.raises(RuntimeError, match="distillation_loss.*second derivative"):
+                torch.autograd.grad(objective, leaf, retain_graph=True, allow_unused=True)
+
+
+@pytest.mark.parametrize("record", [False, True])
+def test_tangents_are_refused(record):
+    import torch.autograd.forward_ad as fwd
+    z = _logits(6, 900, F32, 34)
+    ids, t, lse = _teacher(z, 6, F32, 35, True, 1.0)
+    with fwd.dual_level():
+        dual = fwd.make_dual(z.requires_grad_(record), torch.ones_like(z))
+        with pytest.raises(RuntimeError, match="distillation_loss.*forward-mode"):
+            _ops().distillation_loss(dual, ids, t, lse)

@@ -199,3 +199,45 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="bias"):
         _layer_norm(x, w, w.cpu())
     assert torch.isfinite(_layer_norm(x, w)).all()  # refused calls leave the context usable
+
+
+# The backward kernels form first derivatives.  A second one, or a tangent, is refused and never left out of a sum.
+@pytest.mark.parametrize("learned", ["x", "w", "b", "xwb"])
+def test_second_derivatives_are_refused(learned):
+    x, w, b, dy = _inputs(5, 96, torch.float32, torch.float32)
+    leaves = [t.requires_grad_(True) for name, t in zip("xwb", (x, w, b)) if name in learned]
+    want = torch.autograd.grad((_layer_norm(x, w, b) * dy).sum(), leaves)
+    y = _layer_norm(x, w, b)
+    grads = torch.autograd.grad((y * dy).sum(), leaves, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(grads, want))  # the first derivative itself is as ever
+    penalty = sum(g.square().sum() for g in grads)
+    for objective in (penalty, y.sum() + penalty):  # with and without another way to the inputs
+        with pytest.raises(RuntimeError, match="layer_norm.*second derivative"):
+            torch.autograd.grad(objective, leaves, retain_graph=True, allow_unused=True)
+    objective = y.square().sum()
+    objective.backward(create_graph=True)
+    assert all(torch.isfinite(t.grad).all() for t in leaves)
+    for t in leaves:
+        t.grad = None
+
+
+def test_a_factor_that_is_learned_gets_no_silent_gradient():
+    x, w, b, dy = _inputs(5, 96, torch.float32, torch.float32)
+    x.requires_grad_(True)
+    s = torch.ones((), device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad((_layer_norm(x, w, b) * dy * s).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="layer_norm.*second derivative"):
+        torch.autograd.grad(g.sum(), s, allow_unused=True)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("record", [False, True])
+def test_tangents_are_refused(which, record):
+    import torch.autograd.forward_ad as fwd
+    args = list(_inputs(4, 64, torch.float32, torch.float32)[:3])
+    if record:
+        args = [t.requires_grad_(True) for t in args]
+    with fwd.dual_level():
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="layer_norm.*forward-mode"):
+            _layer_norm(*args)
