@@ -416,10 +416,10 @@ class LinearDistillFn(torch.autograd.Function):
     KEEP_BYTES = 8 << 30
 
     @staticmethod
-    def forward(ctx, x, targets, ids, t, lse, group, V, alpha, chunk, tau, kd, ce, scale, weight):
+    def forward(ctx, x, targets, ids, t, lse, group, V, alpha, chunk, tau, kd, ce, scale, record, weight):
         w16 = group.bf16()
         N, Vp = x.shape[0], w16.shape[0]
-        grad = any(ctx.needs_input_grad)
+        grad = record and any(ctx.needs_input_grad)
         keep = grad and N * Vp * 2 <= LinearDistillFn.KEEP_BYTES
         dz = torch.empty(N, Vp, device=x.device, dtype=torch.bfloat16) if keep else None
         total = torch.zeros((), device=x.device, dtype=torch.float32)
@@ -465,7 +465,7 @@ class LinearDistillFn(torch.autograd.Function):
                 _mm(part.t(), x[s:e], out, c=out, alpha=alpha, beta=beta if s == 0 else 1.0)
 
         (gw,) = group.sink_grad(compute)
-        return (dx,) + (None,) * 12 + (gw,)
+        return (dx,) + (None,) * 13 + (gw,)
 
 
 def linear_distillation(x, targets, group, V, teacher, alpha=1.0, chunk=8192, scale=None):
@@ -477,7 +477,8 @@ def linear_distillation(x, targets, group, V, teacher, alpha=1.0, chunk=8192, sc
     return LinearDistillFn.apply(x.contiguous(), targets.contiguous().view(-1), teacher.ids.reshape(n, k).contiguous(),
                                  teacher.values.reshape(n, k).contiguous(), lse, group, int(V), float(alpha), int(chunk),
                                  float(teacher.temperature), float(teacher.kd_weight), float(teacher.ce_weight),
-                                 scale.detach().reshape(1).float() if scale is not None else None, group.params[0])
+                                 scale.detach().reshape(1).float() if scale is not None else None,
+                                 torch.is_grad_enabled(), group.params[0])  # inside, neither says whether to record
 
 
 def linear_cross_entropy(x, targets, group, V, alpha=1.0, chunk=8192):

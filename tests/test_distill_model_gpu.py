@@ -117,3 +117,27 @@ def test_example_distils_on_the_gpu():
         report = run_distill(steps=25, teacher_steps=40, rows=8, device="cuda")
     assert report["student_ce_after"] < report["student_ce_before"] - 0.2
     assert {"layer_norm", "top_logits", "distill_loss", "autograd"} <= set(c.by_name)
+
+
+def test_evaluation_forms_no_gradient():
+    """Without recorded gradients the loss needs its logits chunk and little else: 2 x 2000 rows of 4096 columns would be
+    33 MB of 16-bit gradients."""
+    model = _model(vocab_size=4000, padded_vocab=4096, loss_chunk_tokens=100)
+    idx, y, teacher = _batch(B=2, T=2000)
+    with torch.no_grad():
+        model(idx, targets=y, reduction="sum", teacher=teacher)  # caches of the weights
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        x = torch.randn(4000, 256, device="cuda").bfloat16()
+        from tensor_train_ing_b200.ops import fused
+        from tensor_train_ing_b200.ops.weights import group_for
+        group = group_for(model, "unembed", [model.unembed.weight])
+        torch.cuda.reset_peak_memory_stats()
+        loss = fused.linear_distillation(x, y.reshape(-1), group, 4000, teacher, 1.0, 100)
+        peak = torch.cuda.max_memory_allocated() - base
+    assert peak < 12 << 20, peak
+    x.requires_grad_(True)
+    again = fused.linear_distillation(x, y.reshape(-1), group, 4000, teacher, 1.0, 100)
+    assert torch.equal(loss, again.detach())
+    (dx,) = torch.autograd.grad(again, x)
+    assert dx.shape == x.shape and dx.any()
