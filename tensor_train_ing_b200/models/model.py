@@ -405,9 +405,10 @@ class TensorLM(nn.Module):
         if targets is None:
             logits = self.unembed(x)[..., :self.cfg.vocab_size]
             return logits * self.logit_multiplier if self.cfg.width_scaling_base else logits
-        if teacher is not None:
-            logits, loss = None, self._distill(x, targets, teacher, scale)
-        else:
-            logits, loss = self._loss(x, targets)
         n = (targets != -100).sum()
+        if teacher is not None:
+            from ..ops.distill import factor_of
+            loss = self._distill(x, targets, teacher, factor_of(scale, n, reduction))
+            return (None, loss, n) if reduction == "sum" else (None, loss)
+        logits, loss = self._loss(x, targets)
         return (logits, loss, n) if reduction == "sum" else (logits, loss / n.clamp_min(1))

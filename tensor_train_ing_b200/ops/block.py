@@ -18,6 +18,7 @@ import torch.nn as nn
 from ..models.attention import rope_inv_freq, row_scale_vector
 from ..models.normalization import GroupRMSNorm, LaggedRMS, LayerNorm, RMSNorm, SpectralLinear, TaperRMS
 from . import fused, norms
+from .distill import factor_of
 from .layer_norm import layer_norm
 from .weights import group_for, spectral_group_for
 
@@ -190,10 +191,11 @@ def model_forward(model, idx, ctx, targets, reduction, teacher=None, scale=None)
     ug = group_for(model, "unembed", [model.unembed.weight])
     alpha = model.logit_multiplier
     if teacher is not None:
-        chunk = cfg.loss_chunk_tokens or 8192
-        loss = fused.linear_distillation(h, targets.reshape(-1), ug, V, teacher, alpha, chunk, scale)
-        logits = None
-    elif targets is not None and cfg.loss_chunk_tokens > 0:
+        n = (targets != -100).sum()
+        loss = fused.linear_distillation(h, targets.reshape(-1), ug, V, teacher, alpha, cfg.loss_chunk_tokens or 8192,
+                                         factor_of(scale, n, reduction))
+        return (None, loss, n) if reduction == "sum" else (None, loss)
+    if targets is not None and cfg.loss_chunk_tokens > 0:
         loss = fused.linear_cross_entropy(h, targets.reshape(-1), ug, V, alpha, cfg.loss_chunk_tokens)
         logits = None
     else:

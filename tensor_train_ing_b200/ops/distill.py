@@ -51,6 +51,15 @@ class Teacher(NamedTuple):
         return self._replace(ids=part(self.ids), values=part(self.values), lse=part(self.lse))
 
 
+def factor_of(scale, count, reduction: str):
+    """The loss' ``scale`` for this reduction over ``count`` targets (a device tensor): a mean's division belongs into it, so
+    that a gradient of 16 bits is rounded once, after it."""
+    if reduction == "sum":
+        return scale
+    inverse = count.clamp_min(1).double().reciprocal()
+    return inverse if scale is None else inverse * scale.detach().reshape(())
+
+
 def _rows(logits: torch.Tensor, what: str) -> torch.Tensor:
     """The logits as [N, V] rows with a unit column stride (a view where there is one)."""
     if not logits.is_cuda:

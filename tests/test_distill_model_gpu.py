@@ -141,3 +141,23 @@ def test_evaluation_forms_no_gradient():
     assert torch.equal(loss, again.detach())
     (dx,) = torch.autograd.grad(again, x)
     assert dx.shape == x.shape and dx.any()
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_the_mean_is_the_sum_with_its_factor_inside(fused):
+    """reduction="mean" hands one over the count to the loss kernel, which rounds the gradient once, after it."""
+    model = _model()
+    model._force_reference = not fused
+    idx, y, teacher = _batch()
+    assert model.uses_fused_path(idx) == fused
+    for factor in (None, torch.tensor([0.7], device="cuda")):
+        n = (y != -100).sum().float().reshape(1)
+        loss, want = _run(model, idx, y, teacher, (1 if factor is None else factor) / n)
+        model.zero_grad(set_to_none=True)
+        _, mean = model(idx, targets=y, teacher=teacher, scale=factor)
+        mean.backward()
+        assert torch.equal(mean.detach(), loss)
+        for name, p in model.named_parameters():
+            assert torch.equal(p.grad, want[name]), name
+    _, none = model(idx, targets=torch.full_like(y, -100), teacher=teacher)
+    assert none == 0
