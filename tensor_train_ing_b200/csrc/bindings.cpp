@@ -398,10 +398,12 @@ std::vector<Tensor> top_logits(const Tensor& z, int64_t k, double tau) {
   return {values, ids, lse};
 }
 
-// (loss [N] fp32, dz or an undefined tensor).  dz is given (its columns past V are zeroed) or not wanted.
+// (loss [N] fp32, dz or an undefined tensor).  dz is given (its columns past V are zeroed) or not wanted.  factor: one number
+// or one per row that multiplies loss and gradient besides; a single 1 leaves dz as it is and the loss unset.
 Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c10::optional<Tensor>& teacher_lse,
                     const c10::optional<Tensor>& targets, double tau, double kd, double ce,
-                    const c10::optional<Tensor>& scale, const c10::optional<Tensor>& dz) {
+                    const c10::optional<Tensor>& scale, const c10::optional<Tensor>& dz,
+                    const c10::optional<Tensor>& factor = c10::nullopt) {
   check_rows(z, "logits", z);
   const c10::cuda::CUDAGuard guard(z.device());
   const int64_t N = z.size(0), V = z.size(1), K = ids.size(-1);
@@ -421,6 +423,7 @@ Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c
                 "targets must be dense int64 [rows] on the logits' device");
   TORCH_CHECK(ce == 0.0 || targets.has_value(), "the cross-entropy term needs targets");
   if (scale.has_value()) check_f32_vector(*scale, "scale", 1, z);
+  if (factor.has_value()) check_f32_vector(*factor, "factor", factor->numel() == 1 ? 1 : N, z);
   auto loss = torch::empty({N}, z.options().dtype(torch::kFloat32));
   ttb::DistillArgs a{};
   a.z = z.data_ptr();
@@ -439,6 +442,8 @@ Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c
   a.kd = static_cast<float>(kd);
   a.ce = static_cast<float>(ce);
   a.scale = scale.has_value() ? scale->data_ptr<float>() : nullptr;
+  a.factor = factor.has_value() ? factor->data_ptr<float>() : nullptr;
+  a.factor_step = factor.has_value() && factor->numel() > 1 ? 1 : 0;
   a.loss = loss.data_ptr<float>();
   if (dz.has_value()) {
     check_rows(*dz, "dz", z);
@@ -471,7 +476,10 @@ Tensor gradient_like(const Tensor& z) {
 }
 
 // distill_loss with its gradient formed in the same pass over the logits and kept instead of them; the backward
-// multiplies it by the incoming factor in place, so it can run once.
+// multiplies it by the incoming factor in place, so it can run once.  A factor other than 1 then rounds bf16 a second time (another
+// 2^-9 of the value), which costs less than keeping the logits.  fp16 has no exponents for that: a loss scaler's factor
+// would come after most of the gradient was rounded to zero.  Its logits are kept too, and a factor other than 1 forms the
+// gradient once more from them.
 struct DistillNode : torch::autograd::Function<DistillNode> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& z, const Tensor& ids, const Tensor& t,
                         const c10::optional<Tensor>& teacher_lse, const c10::optional<Tensor>& targets, double tau,
@@ -480,16 +488,31 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
     Tensor dz = gradient_like(z);
     Tensor loss = distill_loss(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, dz);
     ctx->saved_data["dz"] = dz;
+    if (z.scalar_type() == torch::kFloat16) {
+      ctx->save_for_backward({z, ids, t, teacher_lse.value_or(Tensor()), targets.value_or(Tensor()),
+                              scale.value_or(Tensor())});
+      ctx->saved_data["tau"] = tau;
+      ctx->saved_data["kd"] = kd;
+      ctx->saved_data["ce"] = ce;
+    }
     return total ? loss.sum() : loss;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView guard;
     auto& kept = ctx->saved_data["dz"];
     TORCH_CHECK(kept.isTensor(), "distillation_loss: the gradient was handed out by an earlier backward");
     Tensor dz = kept.toTensor();
     kept = c10::IValue();
-    scale_rows_(dz, grads[0].contiguous());
+    const Tensor factor = grads[0].contiguous();
+    if (saved.empty()) {
+      scale_rows_(dz, factor);
+    } else {
+      const auto given = [](const Tensor& q) { return q.defined() ? c10::optional<Tensor>(q) : c10::nullopt; };
+      distill_loss(saved[0], saved[1], saved[2], given(saved[3]), given(saved[4]), ctx->saved_data["tau"].toDouble(),
+                   ctx->saved_data["kd"].toDouble(), ctx->saved_data["ce"].toDouble(), given(saved[5]), dz, factor);
+    }
     if (dz.size(0) > 0) autograd_launches += 1;
     torch::autograd::variable_list out(10);
     out[0] = dz;
@@ -1039,7 +1062,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("z"), py::arg("k"), py::arg("tau"));
   m.def("distill_loss", &distill_loss, "distillation loss of each row and, into dz, its gradient", py::arg("z"),
         py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),
-        py::arg("ce"), py::arg("scale"), py::arg("dz"));
+        py::arg("ce"), py::arg("scale"), py::arg("dz"),
+        py::arg("factor") = py::none());
   m.def("scale_rows_", &scale_rows_, "rows of dz times their factor, in place", py::arg("dz"), py::arg("g"));
   m.def("distillation", &distillation, "distillation loss of rows or their sum, differentiable", py::arg("z"),
         py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),

@@ -29,7 +29,10 @@ namespace {
 
 using distill::get_mark;
 using distill::Params;
+using distill::nothing_to_do;
 using distill::put_mark;
+using distill::scale_of;
+using distill::scale_of_all;
 using distill::teacher_logit;
 using distill::zero_row;
 
@@ -75,6 +78,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   constexpr int E = Slice<TZ>::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
+  if (nothing_to_do(p)) return;  // the same for the whole grid
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = p.parts, rank = parts > 1 ? cluster.block_rank() : 0;
   const long long row = blockIdx.x / parts;
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   float S = 0.f, total = 0.f, total1 = 0.f, m = 0.f;
   // What the gradient needs, and the loss, from the rest's sum relative to `at` and the logarithm of the rest's probability.
   auto finish = [&](const rows::Ref& at, float rest_sum, float log_rest) {
-    const float scale = p.scale != nullptr ? *p.scale : 1.f;
+    const float scale = scale_of(p, scale_of_all(p), row);
     const float mass = sh.mass + m;
     const rows::Ref at1 = rows::ref_at_one<POW>(at);
     if (lane == 0) {
@@ -386,7 +390,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   if (rank == parts - 1)
     for (int i = p.vocab + tid; i < p.dz_cols; i += blockDim.x) drow[i] = from_f32<TG>(0.f);
   __syncthreads();
-  const float scale = p.scale != nullptr ? *p.scale : 1.f;
+  const float scale = scale_of(p, scale_of_all(p), row);
   const float kd = scale * p.kd * p.tau, ce = scale * p.ce;
   for (int i = tid; i < p.k; i += blockDim.x) {
     if (!list[i].owner) continue;
@@ -453,6 +457,8 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   p.teacher_lse = a.teacher_lse;
   p.targets = a.targets;
   p.scale = a.scale;
+  p.factor = a.factor;
+  p.factor_step = a.factor_step;
   p.loss = a.loss;
   p.ldz = a.ldz;
   p.lddz = a.lddz;

@@ -58,6 +58,10 @@ struct DistillArgs {
   const long long* targets;   // [rows] or null; a negative target leaves its row out
   float tau, kd, ce;
   const float* scale;  // device scalar or null (1)
+  // What multiplies row r besides: factor[r * factor_step], or null (1).  A single factor (step 0) of 1 leaves loss and dz as
+  // they are: they hold the answer already.
+  const float* factor;
+  int factor_step;
   float* loss;         // [rows]
   void* dz;            // null: no gradient.  [rows, dz_cols], rows lddz apart; columns past vocab are written as zeros
   long long lddz;

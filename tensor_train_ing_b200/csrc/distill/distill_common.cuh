@@ -18,6 +18,8 @@ struct Params {
   const float* teacher_lse;
   const long long* targets;
   const float* scale;
+  const float* factor;
+  int factor_step;
   float* loss;
   long long ldz, lddz;
   uint32_t* status;
@@ -27,6 +29,15 @@ __device__ __forceinline__ float teacher_logit(const Params& p, long long i) {
   if (p.t_type == ScalarType::kF32) return static_cast<const float*>(p.t)[i];
   if (p.t_type == ScalarType::kBF16) return to_f32(static_cast<const __nv_bfloat16*>(p.t)[i]);
   return to_f32(static_cast<const __half*>(p.t)[i]);
+}
+
+__device__ __forceinline__ bool nothing_to_do(const Params& p) {
+  return p.factor != nullptr && p.factor_step == 0 && *p.factor == 1.f;
+}
+// What multiplies a row's loss and gradient, `scale` being what multiplies all rows'.
+__device__ __forceinline__ float scale_of_all(const Params& p) { return p.scale != nullptr ? *p.scale : 1.f; }
+__device__ __forceinline__ float scale_of(const Params& p, float scale, long long row) {
+  return p.factor != nullptr ? scale * p.factor[row * p.factor_step] : scale;
 }
 
 // The smem element a listed column's slot holds while entries compete for it, as bits of a finite value.

@@ -394,7 +394,7 @@ template <typename TG, bool GRAD, int POW>
 __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, const Params& p, const Place& at, float c,
                                             float c1) {
   const int lane = threadIdx.x & 31;
-  const float scale = p.scale != nullptr ? *p.scale : 1.f;
+  const float all_scale = scale_of_all(p);
   int turn = 0;
   unsigned on_side = 0;  // bit s: the parity of the live rows side s has had
   for (int n = 0;; ++n) {
@@ -426,6 +426,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       warp_arrives(&sh.side_free[side]);
       continue;
     }
+    const float scale = scale_of(p, all_scale, r.row);
     // The unlisted columns' sums, relative to one reference: of this CTA, then of the row.  The consumers wait for what
     // follows, so independent sums go through the lanes together and quotients are the hardware's (2 ulp).
     const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
@@ -528,6 +529,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
   __shared__ Shared sh;
   TZ* sm = reinterpret_cast<TZ*>(smem);
   auto* lists = reinterpret_cast<Listed*>(smem + static_cast<size_t>(p.per) * 16);
+  if (nothing_to_do(p)) return;  // the same for the whole grid
   if (threadIdx.x == 0) {
     for (int g = 0; g < kStages; ++g) {
       mbar_init(&sh.full[g], 1);

@@ -146,7 +146,8 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     to the logits' type, so that ``backward()`` has nothing left to do.
 
     Differentiable with respect to ``logits`` alone, once: the forward forms the gradient in the same pass over the
-    logits and keeps it instead of them; the backward multiplies it by the incoming factor in place.  Second derivatives
+    logits and keeps it instead of them; the backward multiplies it by the incoming factor in place (fp16 logits are kept as
+    well, and a factor other than 1, a loss scaler's for instance, takes another pass over them).  Second derivatives
     and forward-mode tangents are refused (``distillation_loss_reference`` has them).  A teacher's mass outside its
     list at or below 2^-20 counts as none (that is what rounding leaves of 1 - sum p)."""
     if not temperature > 0:

@@ -648,3 +648,27 @@ def test_tangents_are_refused(record):
         dual = fwd.make_dual(z.requires_grad_(record), torch.ones_like(z))
         with pytest.raises(RuntimeError, match="distillation_loss.*forward-mode"):
             _ops().distillation_loss(dual, ids, t, lse)
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("n,v", [(6, 3001), (700, 50257), (6, 50257)])
+def test_factors_reach_an_fp16_gradient_before_it_is_rounded(n, v, reduction):
+    """What a loss scaler does: the loss is one over many tokens, the factor arrives in the backward.  The rounding to fp16
+    comes after both, so nothing of the gradient is lost below 2^-25."""
+    z = _logits(n, v, F16, 36, ld=v + 7)
+    ids, t, lse = _teacher(z, 9, F32, 37, True, 2.0)
+    y = _targets(n, v, ids, 38)
+    weights = torch.ones(n, device="cuda") if reduction == "sum" else \
+        torch.tensor([1.0, 0.5, -3.0], device="cuda").repeat(n // 3 + 1)[:n]
+    scale, factor = 2.0 ** -17, 49152.0
+    zz = z.detach().requires_grad_(True)
+    loss = _ops().distillation_loss(zz, ids, t, lse, y, temperature=2.0, ce_weight=0.5, scale=scale, reduction=reduction)
+    objective = factor * (loss if reduction == "sum" else (loss * weights).sum())
+    (got,) = torch.autograd.grad(objective, zz, retain_graph=True)
+    _, grad, _, gtol = _reference(z, ids, t, lse, y, 2.0, 1.0, 0.5, scale * factor)
+    grad, gtol = grad * weights[:, None], gtol * weights.abs()[:, None].clamp_min(1)
+    bad = (got.double() - grad).abs() > gtol
+    assert got.dtype == F16 and not bad.any(), (bad.nonzero()[:5], got[bad][:5], grad[bad][:5], gtol[bad][:5])
+    assert (got != 0).float().mean() > 0.3  # most of it would be zero without the factor
+    with pytest.raises(RuntimeError, match="earlier backward"):
+        torch.autograd.grad(objective, zz)
