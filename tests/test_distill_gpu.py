@@ -672,3 +672,32 @@ def test_factors_reach_an_fp16_gradient_before_it_is_rounded(n, v, reduction):
     assert (got != 0).float().mean() > 0.3  # most of it would be zero without the factor
     with pytest.raises(RuntimeError, match="earlier backward"):
         torch.autograd.grad(objective, zz)
+
+
+def _direct(z, ids, t, lse, y, tau, kd, ce, scale, dz):
+    from tensor_train_ing_b200.ops._ext import lib
+    return lib().distill_loss(z, ids, t, lse, y, tau, kd, ce, torch.full((1,), scale, device="cuda"), dz)
+
+
+# What the trainer calls: fp32 logits cut from a padded buffer, a bf16 gradient as wide as that buffer.
+@pytest.mark.parametrize("n,v,ld,offset", [(601, 50257, 50304, 0), (601, 50257, 50257, 1), (601, 131071, 131072, 0),
+                                           (1201, 16385, 16448, 0), (1201, 20000, 20032, 4), (40, 50257, 50304, 0),
+                                           (3, 500, 512, 2), (9, 4097, 4104, 3)])
+@pytest.mark.parametrize("k,rest,tau,ce", [(1, False, 1.0, 0.0), (40, True, 2.0, 0.5), (64, True, 1.5, 0.25),
+                                           (64, False, 4.0, 0.5)])
+def test_fp32_logits_with_a_bf16_gradient(n, v, ld, offset, k, rest, tau, ce):
+    z = _logits(n, v, F32, v + k, ld=ld, offset=offset)
+    ids, t, lse = _teacher(z, k, F32, k, rest, tau)
+    y = _targets(n, v, ids, 5)
+    y[torch.rand(n, device="cuda", generator=_gen(6)) < 0.3] = -100
+    y[0], y[1] = 0, v - 1
+    loss, grad, tol, gtol = _reference(z, ids, t, lse, y, tau, 0.9, ce, 0.5)
+    gtol = gtol + HALF_ULP[BF16] * 1.01 * grad.abs()
+    for width, skip in ((ld, 0), (v, 0), (ld + 5, 1)):  # the buffer's width, the logits', rows off 16 bytes
+        flat = torch.full((n * width + 1,), float("nan"), device="cuda", dtype=BF16)
+        dz = flat[skip:skip + n * width].view(n, width)
+        rows = _direct(z, ids, t, lse, y, tau, 0.9, ce, 0.5, dz)
+        assert ((rows.double() - loss).abs() <= tol).all()
+        bad = ~((dz[:, :v].double() - grad).abs() <= gtol)
+        assert not bad.any(), (bad.nonzero()[:5], dz[:, :v][bad][:5], grad[bad][:5], gtol[bad][:5])
+        assert not dz[:, v:].any() and flat[:skip].isnan().all() and flat[skip + n * width:].isnan().all()
