@@ -27,6 +27,7 @@
 namespace ttb {
 namespace {
 
+using distill::first_of_column;
 using distill::get_mark;
 using distill::Params;
 using distill::nothing_to_do;
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   const rows::Ref ref(mx, c), ref1 = rows::ref_at_one<POW>(ref);
 
   // Take the listed logits out of the slice.  Entries that share a column agree on one: the slot holds the number
-  // of its last writer until that one puts -inf there (no number has -inf's bits).
+  // of its last writer until that one puts -inf there (no number has -inf's bits).  Where any do, the first stands for the column.
   for (int i = tid; i < p.k; i += blockDim.x)
     if (list[i].col >= 0 && s.holds(list[i].col)) put_mark(s.sm + (list[i].col - s.first), i);
   __syncthreads();
@@ -178,6 +179,10 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     if (owner && p.k >= p.vocab) atomicAdd(&sh.listed, 1);  // only such a list can name every column
   }
   __syncthreads();
+  if (sh.repeats) {
+    for (int i = tid; i < p.k; i += blockDim.x)
+      if (list[i].col >= 0 && s.holds(list[i].col)) list[i].owner = first_of_column(list, i);
+  }
   if (parts > 1) cluster.barrier_wait();
 
   // sums over the slice and its listed columns, relative to the slice's largest logit

@@ -52,6 +52,15 @@ __device__ __forceinline__ int get_mark(const T* p) {
   else return *reinterpret_cast<const unsigned short*>(p);
 }
 
+// Whether no entry before i names entry i's column.  Which of several entries stands for a column decides where its exponential
+// is added; the competition for its slot has some winner, this one has the same in every run.
+template <typename E>
+__device__ __noinline__ bool first_of_column(const E* list, int i) {
+  for (int j = 0; j < i; ++j)
+    if (list[j].col == list[i].col) return false;
+  return true;
+}
+
 // Threads first, first + step, ... write the row's zeros: 16 bytes each between the ragged ends.
 template <typename T>
 __device__ __forceinline__ void zero_row(T* row, int cols, int first, int step) {

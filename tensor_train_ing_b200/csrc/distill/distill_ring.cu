@@ -114,6 +114,13 @@ __device__ __forceinline__ void produce(const TZ* z, TZ* sm, Shared& sh, const P
       if (turn > 0) mbar_wait(&sh.full[g], (turn - 1) & 1, p.status, kErrTimeoutProducer);
 }
 
+// One warp: of the stage's entries that share a column, the first stands for it.
+__device__ __noinline__ void settle_owners(Listed* list, int stage, Row& r, int k) {
+  for (int i = threadIdx.x & 31; i < k; i += 32)
+    if (list[i].stage == stage) list[i].owner = first_of_column(list, i);
+  r.repeats = 1;
+}
+
 template <typename TZ>
 __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh, const Params& p, const Place& at) {
   const int lane = threadIdx.x & 31;
@@ -207,13 +214,15 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
       r.target_here = target >= 0 && s.holds(static_cast<int>(target));
     }
     __syncwarp();
+    bool shared = false;
     for (int i = lane; i < p.k; i += 32) {  // edge columns are never in shared memory: they are settled here
       if (list[i].stage != kStages) continue;
       const unsigned bit = 1u << s.edge_slot(list[i].col);
       const bool owner = !(atomicOr(&r.edges, bit) & bit);
       list[i].owner = owner;
-      if (!owner) r.repeats = 1;
+      shared |= !owner;
     }
+    if (__any_sync(0xffffffffu, shared)) settle_owners(list, kStages, r, p.k);
     warp_arrives(&sh.list_ready[side]);
   }
 }
@@ -231,10 +240,11 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
     for (int g = 0; g < kStages && r.live; ++g) {
       if (!warp_waits(&sh.full[g], turn & 1, &sh.stop, p.status)) return;
       // Entries that share a column agree on one: the slot holds the number of its last writer until that one puts
-      // -inf there (no number has -inf's bits).  Element e of the row lies at e + off from the slice's start.
+      // -inf there (no number has -inf's bits).  Where any do, the first stands for the column.  Element e of the row lies at e + off from the slice's start.
       for (int i = lane; i < p.k; i += 32)
         if (list[i].stage == g) put_mark(sm + list[i].col - r.first, i);
       __syncwarp();
+      bool shared = false;
       for (int i = lane; i < p.k; i += 32) {
         if (list[i].stage != g) continue;
         TZ* slot = sm + list[i].col - r.first;
@@ -243,8 +253,9 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
         if (owner)
           *slot = rows::neg_inf<TZ>();
         else
-          r.repeats = 1;
+          shared = true;
       }
+      if (__any_sync(0xffffffffu, shared)) settle_owners(list, g, r, p.k);
       fence_proxy_async_smem();  // before the stage's next copy
       warp_arrives(&sh.ready[g]);
     }

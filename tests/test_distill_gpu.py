@@ -701,3 +701,23 @@ def test_fp32_logits_with_a_bf16_gradient(n, v, ld, offset, k, rest, tau, ce):
         bad = ~((dz[:, :v].double() - grad).abs() <= gtol)
         assert not bad.any(), (bad.nonzero()[:5], dz[:, :v][bad][:5], grad[bad][:5], gtol[bad][:5])
         assert not dz[:, v:].any() and flat[:skip].isnan().all() and flat[skip + n * width:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype,v,offset", [(F32, 20011, 1), (BF16, 50257, 3), (BF16, 901, 0)])
+@pytest.mark.parametrize("n", [700, 12])
+def test_columns_named_many_times_give_the_same_bits(n, dtype, v, offset):
+    z = _logits(n, v, dtype, 60, offset=offset)
+    ids, t, lse = _teacher(z, 300, F32, 61, True, 2.0)
+    some = torch.tensor([0, 1, v - 1, v // 2, v // 3, 257, 258], device="cuda", dtype=torch.int32)
+    ids = torch.where(torch.rand(n, 300, device="cuda", generator=_gen(62)) < 0.5, ids,
+                      some[torch.randint(0, 7, (n, 300), device="cuda", generator=_gen(63))])
+    lse = torch.logsumexp(t / 2.0, 1) + 0.2
+    y = _targets(n, v, ids, 64)
+    _check_loss(z, ids, t, lse, y, 2.0, 1.0, 0.5)
+    once = None
+    for _ in range(12):
+        zz = z.detach().requires_grad_(True)
+        rows = _ops().distillation_loss(zz, ids, t, lse, y, temperature=2.0, ce_weight=0.5, reduction="none")
+        got = rows.detach(), torch.autograd.grad(rows.sum(), zz)[0]
+        once = once or got
+        assert torch.equal(got[0], once[0]) and torch.equal(got[1], once[1])
