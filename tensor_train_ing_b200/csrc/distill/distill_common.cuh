@@ -55,7 +55,7 @@ __device__ __forceinline__ int get_mark(const T* p) {
 // Whether no entry before i names entry i's column.  Which of several entries stands for a column decides where its exponential
 // is added; the competition for its slot has some winner, this one has the same in every run.
 template <typename E>
-__device__ __noinline__ bool first_of_column(const E* list, int i) {
+__device__ __forceinline__ bool first_of_column(const E* list, int i) {
   for (int j = 0; j < i; ++j)
     if (list[j].col == list[i].col) return false;
   return true;

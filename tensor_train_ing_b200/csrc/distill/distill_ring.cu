@@ -114,13 +114,6 @@ __device__ __forceinline__ void produce(const TZ* z, TZ* sm, Shared& sh, const P
       if (turn > 0) mbar_wait(&sh.full[g], (turn - 1) & 1, p.status, kErrTimeoutProducer);
 }
 
-// One warp: of the stage's entries that share a column, the first stands for it.
-__device__ __noinline__ void settle_owners(Listed* list, int stage, Row& r, int k) {
-  for (int i = threadIdx.x & 31; i < k; i += 32)
-    if (list[i].stage == stage) list[i].owner = first_of_column(list, i);
-  r.repeats = 1;
-}
-
 template <typename TZ>
 __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh, const Params& p, const Place& at) {
   const int lane = threadIdx.x & 31;
@@ -214,15 +207,13 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
       r.target_here = target >= 0 && s.holds(static_cast<int>(target));
     }
     __syncwarp();
-    bool shared = false;
     for (int i = lane; i < p.k; i += 32) {  // edge columns are never in shared memory: they are settled here
       if (list[i].stage != kStages) continue;
       const unsigned bit = 1u << s.edge_slot(list[i].col);
       const bool owner = !(atomicOr(&r.edges, bit) & bit);
       list[i].owner = owner;
-      shared |= !owner;
+      if (!owner) r.repeats = 1;
     }
-    if (__any_sync(0xffffffffu, shared)) settle_owners(list, kStages, r, p.k);
     warp_arrives(&sh.list_ready[side]);
   }
 }
@@ -240,11 +231,10 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
     for (int g = 0; g < kStages && r.live; ++g) {
       if (!warp_waits(&sh.full[g], turn & 1, &sh.stop, p.status)) return;
       // Entries that share a column agree on one: the slot holds the number of its last writer until that one puts
-      // -inf there (no number has -inf's bits).  Where any do, the first stands for the column.  Element e of the row lies at e + off from the slice's start.
+      // -inf there (no number has -inf's bits).  Element e of the row lies at e + off from the slice's start.
       for (int i = lane; i < p.k; i += 32)
         if (list[i].stage == g) put_mark(sm + list[i].col - r.first, i);
       __syncwarp();
-      bool shared = false;
       for (int i = lane; i < p.k; i += 32) {
         if (list[i].stage != g) continue;
         TZ* slot = sm + list[i].col - r.first;
@@ -253,9 +243,8 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
         if (owner)
           *slot = rows::neg_inf<TZ>();
         else
-          shared = true;
+          r.repeats = 1;
       }
-      if (__any_sync(0xffffffffu, shared)) settle_owners(list, g, r, p.k);
       fence_proxy_async_smem();  // before the stage's next copy
       warp_arrives(&sh.ready[g]);
     }
@@ -266,7 +255,7 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
 
 template <typename TZ, typename TG, bool GRAD, int POW>
 __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const Listed* lists, Shared& sh,
-                                        const Params& p, const Place& at, float c, float c1) {
+                                        const Params& p, const Place& at, float c) {
   constexpr int E = Span<TZ>::kVec;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int turn = 0;
@@ -317,7 +306,7 @@ __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const
       }
       if (counted) sums.add_one(edge_z, c);
     }
-    const rows::WarpSum mine = rows::warp_total<POW>(sums, c, c1);
+    const rows::WarpSum mine = rows::warp_total<POW>(sums, c);
     if (lane == 0) sh.sums[side][warp] = mine;
     warp_arrives(&sh.sums_ready[side]);
 
@@ -391,12 +380,14 @@ __device__ __forceinline__ float2 warp_sum2(float2 v) {
 }
 // The lanes' sums relative to the largest of their references, which `top` becomes.
 template <int POW>
-__device__ __forceinline__ float2 relative_sums(float& top, float sum, float sum1, float c, float c1) {
+__device__ __forceinline__ float2 relative_sums(float& top, float sum, float sum1, float c) {
   const Ref of(top == -CUDART_INF_F ? 0.f : top, c);
   top = rows::lanes_max(top);
   const Ref to(top == -CUDART_INF_F ? 0.f : top, c);
-  sum = rows::rescaled(sum, to.log2_of(of, c));
-  if (POW != 0) sum1 = rows::rescaled(sum1, rows::ref_at_one<POW>(to).log2_of(rows::ref_at_one<POW>(of), c1));
+  const float step = to.log2_of(of, c);
+  sum = rows::rescaled(sum, step);
+  if (POW != 0)
+    sum1 = rows::rescaled(sum1, rows::log2_at_one<POW>(step, rows::ref_at_one<POW>(to), rows::ref_at_one<POW>(of)));
   if (POW == 0) return make_float2(warp_sum(sum), 0.f);
   return warp_sum2(make_float2(sum, sum1));
 }
@@ -421,11 +412,21 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     float L = 0.f, L1 = 0.f, listed = 0.f;
     if (r.live) {
       if (GRAD && !warp_waits(&sh.ready[kStages - 1], turn & 1, &sh.stop, p.status)) return;
-      for (int i = lane; i < p.k; i += 32) {
-        if (!list[i].owner) continue;
-        L += exp2f(list_ref.log2_of(list[i].z, c));
-        if (POW != 0) L1 += exp2f(list_ref1.log2_of(list[i].z, c1));
-        listed += 1.f;
+      const bool repeats = r.repeats;
+      const auto add_list = [&] {
+        for (int i = lane; i < p.k; i += 32) {
+          if (!list[i].owner) continue;
+          L += rows::fast_exp2(list_ref.log2_of(list[i].z, c));
+          if (POW != 0) L1 += rows::fast_exp2(list_ref1.log2_of(list[i].z, c1));
+          listed += 1.f;
+        }
+      };
+      add_list();
+      if (__builtin_expect(repeats, 0)) {  // which entry stands for a column decides where it is added: the first, in every run
+        for (int i = lane; i < p.k; i += 32)
+          if (list[i].stage >= 0) list[i].owner = first_of_column(list, i);
+        L = L1 = listed = 0.f;
+        add_list();
       }
       L = warp_sum(L);
       if (POW != 0) L1 = warp_sum(L1);
@@ -442,7 +443,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     // follows, so independent sums go through the lanes together and quotients are the hardware's (2 ulp).
     const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
     float rest_top = w.z;
-    float2 S2 = relative_sums<POW>(rest_top, w.sum, w.sum1, c, c1);
+    float2 S2 = relative_sums<POW>(rest_top, w.sum, w.sum1, c);
     if (p.parts > 1) {
       // Two places by turns of live rows: a CTA writes a place again only after the turn between, for which every CTA
       // has arrived after it read this one.
@@ -455,7 +456,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       if (!warp_waits<true>(&sh.part_ready[place], (turn >> 1) & 1, &sh.stop, p.status)) return;
       const Part q = lane < p.parts ? sh.part[place][lane] : Part{-CUDART_INF_F, 0.f, 0.f, 0.f, 0.f};
       rest_top = q.ref;
-      S2 = relative_sums<POW>(rest_top, q.sum, q.sum1, c, c1);
+      S2 = relative_sums<POW>(rest_top, q.sum, q.sum1, c);
       const float2 L2 = warp_sum2(make_float2(q.list, q.list1));
       L = L2.x;
       L1 = L2.y;
@@ -465,11 +466,13 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     // the row's reference: the larger of the rest's and the list's
     const Ref ref(L != 0.f && r.list_top > own.z ? r.list_top : own.z, c), ref1 = rows::ref_at_one<POW>(ref);
     if (L != 0.f && ref.z != r.list_top) {
-      L *= exp2f(ref.log2_of(list_ref, c));
-      if (POW != 0) L1 *= exp2f(ref1.log2_of(list_ref1, c1));
+      const float step = ref.log2_of(list_ref, c);
+      L *= rows::fast_exp2(step);
+      if (POW != 0) L1 *= rows::fast_exp2(rows::log2_at_one<POW>(step, ref1, list_ref1));
     }
     const bool same = ref.z == own.z;
-    const float f = same ? 1.f : exp2f(ref.log2_of(own, c)), f1 = same ? 1.f : exp2f(ref1.log2_of(own1, c1));
+    const float step = ref.log2_of(own, c), f = same ? 1.f : rows::fast_exp2(step),
+                f1 = same || POW == 0 ? f : rows::fast_exp2(rows::log2_at_one<POW>(step, ref1, own1));
     const float total = S * f + L, total1 = POW != 0 ? S1 * f1 + L1 : total;
     const float inv_sum = __fdividef(1.f, total), inv_sum1 = POW != 0 ? __fdividef(1.f, total1) : inv_sum;
     // a list that names every column leaves no rest, whatever rounding says
@@ -497,9 +500,8 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       kl = warp_sum(kl);
     }
     if (lane == 0 && at.rank == 0) {
-      if (m > 0.f)  // log q_rest from its parts where the probability itself leaves fp32's range
-        kl += m * (f > 1e-30f ? logf(m / (S * f * inv_sum))
-                              : logf(m) - (logf(S) + ref.log_of(own, c, p.inv_tau) - logf(total)));
+      // log q_rest from its parts: the probability itself may leave fp32's range
+      if (m > 0.f) kl += m * ((log2f(m) - log2f(S) + log2_total) * CUDART_LN2_F - ref.log_of(own, c, p.inv_tau));
       float loss = p.kd != 0.f ? p.kd * p.tau * p.tau * kl : 0.f;
       if (p.ce != 0.f) loss += p.ce * (log2f(total1) - ref1.log2_of(r.target_logit, c1)) * CUDART_LN2_F;
       p.loss[r.row] = scale * loss;
@@ -517,8 +519,8 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
           for (int j = 0; j < p.k; ++j)
             if (list[j].col == col) share += list[j].p;
         }
-        float g = kd != 0.f ? kd * (exp2f(ref.log2_of(list[i].z, c)) * inv_sum * mass - share) : 0.f;
-        if (ce != 0.f) g += ce * (exp2f(ref1.log2_of(list[i].z, c1)) * inv_sum1 - (col == r.target ? 1.f : 0.f));
+        float g = kd != 0.f ? kd * (rows::fast_exp2(ref.log2_of(list[i].z, c)) * inv_sum * mass - share) : 0.f;
+        if (ce != 0.f) g += ce * (rows::fast_exp2(ref1.log2_of(list[i].z, c1)) * inv_sum1 - (col == r.target ? 1.f : 0.f));
         drow[col] = from_f32<TG>(g);
       }
       if (lane == 0 && ce != 0.f && !r.target_listed && r.target_here) {
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
   const float c = p.inv_tau * CUDART_L2E_F, c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
   const int warp = threadIdx.x >> 5;
   if (warp < kRingWarps) {
-    consume<TZ, TG, GRAD, POW>(z, dz, sm, lists, sh, p, at, c, c1);
+    consume<TZ, TG, GRAD, POW>(z, dz, sm, lists, sh, p, at, c);
   } else if (warp == kProducer) {
     if ((threadIdx.x & 31) == 0) produce(z, sm, sh, p, at);
   } else if (warp == kLister) {

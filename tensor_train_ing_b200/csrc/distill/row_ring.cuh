@@ -169,6 +169,12 @@ __device__ __forceinline__ float max_of(const uint4& u) {
   }
 }
 
+// log2 of o1 over ref1, references at temperature 1, where `step` is that of the references at tau that they go with.
+template <int POW>
+__device__ __forceinline__ float log2_at_one(float step, const Ref& ref1, const Ref& o1) {
+  return POW == 1 ? ref1.log2_of(o1, CUDART_L2E_F) : POW * step;
+}
+
 // A thread's running sums of exp((z - ref) / tau) and, for POW > 0, exp(z - ref), over whatever it has seen.  The
 // reference is the largest logit of its first vector that has one.  While `see` is called before every vector it moves when
 // one exceeds it by more than 2^40, at the temperature or at 1, so that no element adds more to either sum.  Vectors added
@@ -192,12 +198,12 @@ struct Sums {
   __device__ __forceinline__ void move(float logit, float c) {
     const Ref next(logit, c), next1 = ref_at_one<POW>(next);
     if (set && sum() < CUDART_INF_F) {  // an infinite sum stays one (times a factor that underflows it would be NaN)
-      const float2 f = both(fast_exp2(next.log2_of(ref, c)));
+      const float step = next.log2_of(ref, c);
+      const float2 f = both(fast_exp2(step));
       acc[0] = mul2(acc[0], f);
       acc[1] = mul2(acc[1], f);
       if (POW != 0) {
-        const float c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
-        const float2 f1 = both(fast_exp2(next1.log2_of(ref1, c1)));
+        const float2 f1 = both(fast_exp2(log2_at_one<POW>(step, next1, ref1)));
         acc1[0] = mul2(acc1[0], f1);
         acc1[1] = mul2(acc1[1], f1);
       }
@@ -266,18 +272,18 @@ struct WarpSum {
   float sum, sum1;
 };
 template <int POW>
-__device__ __forceinline__ WarpSum warp_total(const Sums<POW>& s, float c, float c1) {
+__device__ __forceinline__ WarpSum warp_total(const Sums<POW>& s, float c) {
   WarpSum w;
   w.z = lanes_max(s.set ? s.ref.z : -CUDART_INF_F);
   const Ref ref(w.z == -CUDART_INF_F ? 0.f : w.z, c);
   w.sum = s.sum();
-  w.sum = rescaled(w.sum, ref.log2_of(s.ref, c));
+  const float step = ref.log2_of(s.ref, c);
+  w.sum = rescaled(w.sum, step);
   w.sum = warp_sum(w.sum);
   w.sum1 = 0.f;
   if (POW != 0) {
-    const Ref ref1 = ref_at_one<POW>(ref);
     w.sum1 = s.sum1();
-    w.sum1 = rescaled(w.sum1, ref1.log2_of(s.ref1, c1));
+    w.sum1 = rescaled(w.sum1, log2_at_one<POW>(step, ref_at_one<POW>(ref), s.ref1));
     w.sum1 = warp_sum(w.sum1);
   }
   return w;

@@ -192,10 +192,8 @@ struct Ref {
   __device__ __forceinline__ float log2_of(float v, float c) const { return far ? (v - z) * c : fmaf(v, c, -r); }
   // log2 of exp(logit / tau) over what the reference stands for, exactly
   __device__ __forceinline__ float excess(float c) const { return far ? 0.f : fmaf(z, c, -r); }
-  // log2 of another reference, of the same row, over this one
-  __device__ __forceinline__ float log2_of(const Ref& o, float c) const {
-    return far || o.far ? fmaf(o.z - z, c, excess(c) - o.excess(c)) : o.r - r;
-  }
+  // log2 of another reference, of the same row, over this one, whatever their kinds
+  __device__ __forceinline__ float log2_of(const Ref& o, float c) const { return excess(c) - o.log2_of(z, c); }
   // the natural logarithm of the same (c times the type's lowest value is no fp32 number)
   __device__ __forceinline__ float log_of(const Ref& o, float c, float inv_tau) const {
     return fmaf(o.z - z, inv_tau, (excess(c) - o.excess(c)) * CUDART_LN2_F);

@@ -133,7 +133,7 @@ __device__ __forceinline__ void consume(const T* z, long long ldz, long long row
         for (int e = 0; e < Span<T>::kVec; ++e) sums.add_one(to_f32(s.row[s.first + v * Span<T>::kVec + e]), c);
       if (edge >= 0) sums.add_one(edge_z, c);
     }
-    const rows::WarpSum mine = rows::warp_total<0>(sums, c, c);
+    const rows::WarpSum mine = rows::warp_total<0>(sums, c);
     if (lane == 0) sh.sums[side][warp] = mine;
     warp_arrives(&sh.sums_ready[side]);
   }
