@@ -585,16 +585,19 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
   }
 }
 
-// Clusters of this kernel that the device runs at one time (asked once for each kernel, size and shared memory).
+// Clusters of this kernel that the device runs at one time (asked once for each kernel, size and shared memory; an error leaves
+// nothing behind).
 int active_clusters(const void* kernel, const cudaLaunchConfig_t& cfg, int parts) {
   static std::mutex lock;
   static std::map<std::tuple<int, const void*, int, size_t>, int> known;
   int device = 0;
   TTB_CUDA_CHECK(cudaGetDevice(&device));
   const std::lock_guard<std::mutex> guard(lock);
-  auto [it, fresh] = known.try_emplace({device, kernel, parts, cfg.dynamicSmemBytes}, 0);
-  if (fresh) TTB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&it->second, kernel, &cfg));
-  return it->second < 1 ? 1 : it->second;
+  const std::tuple<int, const void*, int, size_t> key{device, kernel, parts, cfg.dynamicSmemBytes};
+  if (const auto it = known.find(key); it != known.end()) return it->second;
+  int clusters = 0;
+  TTB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg));
+  return known[key] = clusters < 1 ? 1 : clusters;
 }
 
 }  // namespace
