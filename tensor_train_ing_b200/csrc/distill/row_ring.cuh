@@ -195,10 +195,11 @@ struct Sums {
   __device__ __forceinline__ explicit Sums(float c) : ref(0.f, c), ref1(0.f, c), set(false) {
     acc[0] = acc[1] = acc1[0] = acc1[1] = both(0.f);
   }
-  __device__ __forceinline__ void move(float logit, float c) {
+  // to this logit, `above` the reference by so many powers of two
+  __device__ __forceinline__ void move(float logit, float above, float c) {
     const Ref next(logit, c), next1 = ref_at_one<POW>(next);
     if (set && sum() < CUDART_INF_F) {  // an infinite sum stays one (times a factor that underflows it would be NaN)
-      const float step = next.log2_of(ref, c);
+      const float step = next.excess(c) - above;
       const float2 f = both(fast_exp2(step));
       acc[0] = mul2(acc[0], f);
       acc[1] = mul2(acc[1], f);
@@ -219,7 +220,8 @@ struct Sums {
   }
   // before adding logits of which `top` is the largest
   __device__ __forceinline__ void see(float top, float c) {
-    if ((!set || ref.log2_of(top, c) > most_above(c)) && fabsf(top) < CUDART_INF_F) move(top, c);
+    const float above = ref.log2_of(top, c);
+    if ((!set || above > most_above(c)) && fabsf(top) < CUDART_INF_F) move(top, above, c);
   }
   // Whether vectors may be added without `see` from here on: all of the warp's threads have ordinary references.  One far
   // below the warp's largest (a thread whose first vectors are masked) moves there, so that it will not overflow.
