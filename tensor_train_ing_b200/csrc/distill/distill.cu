@@ -137,16 +137,17 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
       inv = 1.f / e;
       log_sum = logf(e);
     }
+    const bool empty = base == -CUDART_INF_F;  // the teacher's row has no logit at all: no mass, on the rest neither
     float mass = 0.f;
     for (int i = lane; i < p.k; i += 32) {
-      const float a = list[i].logp - base;
+      const float a = empty ? -CUDART_INF_F : list[i].logp - base;
       list[i].logp = a - log_sum;
       list[i].p = expf(a) * inv;
       mass += list[i].p;
     }
     mass = warp_sum(mass);
     if (lane == 0) {
-      const float rest = p.teacher_lse != nullptr && present > 0 ? 1.f - mass : 0.f;
+      const float rest = p.teacher_lse != nullptr && present > 0 && !empty ? 1.f - mass : 0.f;
       sh.mass = mass;
       sh.rest = rest > kDistillLeastRest ? rest : 0.f;
       sh.target_logit = target_logit;

@@ -183,16 +183,17 @@ __device__ __forceinline__ void list_rows(const TZ* z, Listed* lists, Shared& sh
       inv = 1.f / e;
       log_sum = logf(e);
     }
+    const bool empty = base == -CUDART_INF_F;  // the teacher's row has no logit at all: no mass, on the rest neither
     float mass = 0.f;
     for (int i = lane; i < p.k; i += 32) {
-      const float a = list[i].logp - base;
+      const float a = empty ? -CUDART_INF_F : list[i].logp - base;
       list[i].logp = a - log_sum;
       list[i].p = expf(a) * inv;
       mass += list[i].p;
     }
     mass = warp_sum(mass);
     if (lane == 0) {
-      const float rest = p.teacher_lse != nullptr && present ? 1.f - mass : 0.f;
+      const float rest = p.teacher_lse != nullptr && present && !empty ? 1.f - mass : 0.f;
       r.row = row;
       r.live = 1;
       r.target = static_cast<int>(target);

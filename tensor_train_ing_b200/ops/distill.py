@@ -139,7 +139,8 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     teacher, distinct columns in any order; an entry with a negative id is absent, and a row without entries
     has no divergence.  An id past the vocabulary is recorded in the status word (``ops._ext.check_status``)
     and counts as absent.  ``teacher_lse`` (...): the log-sum-exp of the teacher's whole row over the same
-    temperature (``top_logits(...).lse``); without it the teacher is renormalised over its list.
+    temperature (``top_logits(...).lse``); without it the teacher is renormalised over its list.  A row where it is -inf (the
+    teacher masked it throughout) has no divergence.
     ``targets`` (...) int64: rows with a negative target (-100) are left out entirely, loss and gradient zero;
     they are required when ``ce_weight`` is not 0.  ``scale`` (a number or a one-element tensor, e.g. one over
     the update's target count) multiplies loss and gradient inside the kernel, before the gradient is rounded
@@ -183,9 +184,9 @@ def distillation_loss_reference(logits: torch.Tensor, teacher_ids: torch.Tensor,
     there = (ids >= 0) & (ids < v)
     at = torch.where(there, ids, 0)
     a = (teacher_logits.reshape(n, -1).to(z.dtype) / temperature).masked_fill(~there, -math.inf)
-    top = a.amax(1)
-    some = there.any(1) & (top > -math.inf) if teacher_lse is None else there.any(1)
     norm = torch.logsumexp(a, 1) if teacher_lse is None else teacher_lse.reshape(n).to(z.dtype)
+    some = there.any(1) & (norm != -math.inf)
+    a = a.masked_fill(~some[:, None], -math.inf)
     logp = a - torch.where(some, norm, 0)[:, None]
     p = logp.exp()
     logq = torch.log_softmax(z / temperature, 1)

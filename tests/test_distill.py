@@ -200,3 +200,23 @@ def test_kernel_entry_points_refuse_cpu_tensors():
         layer_norm(z, torch.ones(8))
     with pytest.raises(ValueError, match="targets"):
         distill.distillation_loss_reference(z, torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, 1), ce_weight=1.0)
+
+
+def test_a_teacher_row_without_any_logit_has_no_divergence():
+    """A row masked throughout gives a list of -inf and a log-sum-exp of -inf: nothing to learn from it but its target."""
+    z = torch.randn(3, 30, dtype=torch.float64, generator=torch.Generator().manual_seed(6))
+    teacher = torch.randn(3, 30, dtype=torch.float64, generator=torch.Generator().manual_seed(7))
+    teacher[1] = -math.inf
+    top = distill.top_logits_reference(teacher, 5)
+    assert top.lse[1] == -math.inf
+    y = torch.tensor([3, 4, 5])
+    for ce, targets in ((0.0, None), (0.3, y)):
+        zz = z.clone().requires_grad_(True)
+        rows = distill.distillation_loss_reference(zz, top.ids, top.values, top.lse, targets, ce_weight=ce, reduction="none")
+        (g,) = torch.autograd.grad(rows.sum(), zz)
+        assert torch.isfinite(rows).all() and torch.isfinite(g).all()
+        want = -ce * torch.log_softmax(z, 1)[1, 4]
+        torch.testing.assert_close(rows[1], want)
+        others = distill.distillation_loss_reference(z[::2], top.ids[::2], top.values[::2], top.lse[::2],
+                                                     None if targets is None else targets[::2], ce_weight=ce, reduction="none")
+        torch.testing.assert_close(rows[::2].detach(), others)

@@ -721,3 +721,27 @@ def test_columns_named_many_times_give_the_same_bits(n, dtype, v, offset):
         got = rows.detach(), torch.autograd.grad(rows.sum(), zz)[0]
         once = once or got
         assert torch.equal(got[0], once[0]) and torch.equal(got[1], once[1])
+
+
+@pytest.mark.parametrize("n", [700, 7])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_teacher_rows_without_any_logit(n, dtype):
+    teacher = _logits(n, 30011, dtype, 39)
+    teacher[::5] = float("-inf")
+    top = _ops().top_logits(teacher, 12, temperature=2.0)
+    assert (top.lse[::5] == float("-inf")).all()
+    z = _logits(n, 30011, dtype, 40)
+    y = _targets(n, 30011, top.ids, 41)
+    there = top.ids.clone()
+    there[::5] = -1  # the same teacher, its empty rows without entries
+    lse = top.lse.clone()
+    lse[::5] = 0.0
+    for ce, targets in ((0.0, None), (0.5, y)):
+        def both(ids, lse):
+            zz = z.detach().requires_grad_(True)
+            rows = _ops().distillation_loss(zz, ids, top.values, lse, targets, 2.0, 1.0, ce, reduction="none")
+            return rows.detach(), torch.autograd.grad(rows.sum(), zz)[0]
+        got, want = both(top.ids, top.lse), both(there, lse)
+        assert torch.isfinite(got[0]).all()
+        torch.testing.assert_close(got[0], want[0], rtol=64 * U, atol=64 * U)
+        torch.testing.assert_close(got[1].float(), want[1].float(), rtol=2 * HALF_ULP[dtype] + 64 * U * 20, atol=1e-9)
