@@ -398,8 +398,8 @@ std::vector<Tensor> top_logits(const Tensor& z, int64_t k, double tau) {
   return {values, ids, lse};
 }
 
-// (loss [N] fp32, dz or an undefined tensor).  dz is given (its columns past V are zeroed) or not wanted.  factor: one number
-// or one per row that multiplies loss and gradient besides; a single 1 leaves dz as it is and the loss unset.
+// loss [N] fp32.  dz is given (its columns past V are zeroed) or not wanted.  factor, with an fp16 dz of fp16 logits: one number or
+// one per row that multiplies loss and gradient besides; a single 1 leaves dz as it is and the loss unset.
 Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c10::optional<Tensor>& teacher_lse,
                     const c10::optional<Tensor>& targets, double tau, double kd, double ce,
                     const c10::optional<Tensor>& scale, const c10::optional<Tensor>& dz,

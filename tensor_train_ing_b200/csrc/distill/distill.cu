@@ -20,7 +20,8 @@
 //
 // Few rows, and rows shorter than the persistent kernel's.  Bound by what a row waits for: its copy, the list, and the three
 // barriers between maximum, sums and gradient, filled only by the SM's other CTAs.  8288 rows of 16384 bf16 logits, 64 listed:
-// 100 us for the loss (42 us for the bytes), 154 us with the gradient (83 us).
+// 95 us for the loss (42 us for the bytes), 136 us with the gradient (83 us).  Six CTAs of 256 threads share an SM there, so
+// the registers are held to 40: 57 leave four of them and cost a quarter of the time.
 #include "../common/host.h"
 #include "distill_common.cuh"
 
@@ -30,10 +31,7 @@ namespace {
 using distill::first_of_column;
 using distill::get_mark;
 using distill::Params;
-using distill::nothing_to_do;
 using distill::put_mark;
-using distill::scale_of;
-using distill::scale_of_all;
 using distill::teacher_logit;
 using distill::zero_row;
 
@@ -58,6 +56,7 @@ struct Shared {
   float red_max[rows::kMaxThreads / 32];
   float target_logit;
   float mass, rest;  // P and m
+  float scale;
   // the row's scalars for the gradient: q_j = 2^(z_j c - top) inv_sum; the passes over the slice use ref
   rows::Ref ref, ref1, top, top1;
   float A, B, inv_sum, inv_sum1, all_mass;
@@ -72,14 +71,14 @@ struct Entry {
   int owner;    // whether this entry stands for its column here (the first CTA-local entry with this column)
 };
 
-template <typename TZ, typename TG, bool GRAD, int POW>
-__global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __restrict__ z,
-                                                                   TG* __restrict__ dz,
-                                                                   const __grid_constant__ Params p) {
+template <typename TZ, typename TG, int FORM, int POW>
+__global__ void __launch_bounds__(rows::kMaxThreads, 3) distill_kernel(const TZ* __restrict__ z, TG* __restrict__ dz,
+                                                                      const __grid_constant__ Params p) {
   constexpr int E = Slice<TZ>::kVec;
+  constexpr bool GRAD = FORM != distill::kLoss;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
-  if (nothing_to_do(p)) return;  // the same for the whole grid
+  if (distill::nothing_to_do<FORM>(p)) return;  // the same for the whole grid
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = p.parts, rank = parts > 1 ? cluster.block_rank() : 0;
   const long long row = blockIdx.x / parts;
@@ -122,6 +121,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
       has_target |= c >= 0 && c == target;
     }
     const float target_logit = p.ce != 0.f ? to_f32(zrow[target]) : 0.f;
+    const float scale = distill::scale_of<FORM>(p, distill::scale_of_all(p), row);
     present = __reduce_add_sync(0xffffffffu, present);
     has_target = __any_sync(0xffffffffu, has_target);
     top = warp_max(top);
@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     if (lane == 0) {
       const float rest = p.teacher_lse != nullptr && present > 0 && !empty ? 1.f - mass : 0.f;
       sh.mass = mass;
+      sh.scale = scale;
       sh.rest = rest > kDistillLeastRest ? rest : 0.f;
       sh.target_logit = target_logit;
       sh.target_listed = has_target;
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   const rows::Ref ref(mx, c), ref1 = rows::ref_at_one<POW>(ref);
 
   // Take the listed logits out of the slice.  Entries that share a column agree on one: the slot holds the number
-  // of its last writer until that one puts -inf there (no number has -inf's bits).  Where any do, the first stands for the column.
+  // of its last writer until that one puts -inf there (no number has -inf's bits).
   for (int i = tid; i < p.k; i += blockDim.x)
     if (list[i].col >= 0 && s.holds(list[i].col)) put_mark(s.sm + (list[i].col - s.first), i);
   __syncthreads();
@@ -180,10 +181,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     if (owner && p.k >= p.vocab) atomicAdd(&sh.listed, 1);  // only such a list can name every column
   }
   __syncthreads();
-  if (sh.repeats) {
-    for (int i = tid; i < p.k; i += blockDim.x)
-      if (list[i].col >= 0 && s.holds(list[i].col)) list[i].owner = first_of_column(list, i);
-  }
+  const bool repeats = sh.repeats;
   if (parts > 1) cluster.barrier_wait();
 
   // sums over the slice and its listed columns, relative to the slice's largest logit
@@ -207,6 +205,10 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     });
     float sum[4] = {(acc[0].x + acc[0].y) + (acc[1].x + acc[1].y), (acc1[0].x + acc1[0].y) + (acc1[1].x + acc1[1].y),
                     0.f, 0.f};
+    if (repeats) {  // the first entry stands for a column, in every run
+      for (int i = tid; i < p.k; i += blockDim.x)
+        if (list[i].col >= 0 && s.holds(list[i].col)) list[i].owner = first_of_column(list, i);
+    }
     for (int i = tid; i < p.k; i += blockDim.x) {
       if (list[i].owner) {
         sum[2] += exp2f(ref.log2_of(list[i].z, c));
@@ -236,16 +238,17 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   // The row's scalars, by the first warp of every CTA, the parts in the same order.
   rows::Ref top(0.f, c), top1 = rows::ref_at_one<POW>(top);
   float S = 0.f, total = 0.f, total1 = 0.f, m = 0.f;
-  // What the gradient needs, and the loss, from the rest's sum relative to `at` and the logarithm of the rest's probability.
-  auto finish = [&](const rows::Ref& at, float rest_sum, float log_rest) {
-    const float scale = scale_of(p, scale_of_all(p), row);
+  // What the gradient needs, and the loss, from the rest's sum relative to `at`, which is f (at temperature 1: f1) times the row's
+  // reference, and the logarithm of the rest's probability.
+  auto finish = [&](const rows::Ref& at, float f, float f1, float rest_sum, float log_rest) {
+    const float scale = sh.scale;
     const float mass = sh.mass + m;
     const rows::Ref at1 = rows::ref_at_one<POW>(at);
     if (lane == 0) {
-      float A = mass != 0.f ? mass * exp2f(top.log2_of(at, c)) / total : 0.f;
+      float A = mass != 0.f ? mass * f / total : 0.f;
       if (m > 0.f && rest_sum > 0.f) A -= m / rest_sum;
       A *= scale * p.kd * p.tau;
-      float B = p.ce != 0.f ? scale * p.ce * exp2f(top1.log2_of(at1, c1)) / total1 : 0.f;
+      float B = p.ce != 0.f ? scale * p.ce * f1 / total1 : 0.f;
       if (POW == 0) {  // one exponential serves both terms
         A += B;
         B = 0.f;
@@ -291,11 +294,11 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     for (int q = 0; q < parts; ++q) {
       const Part& w = sh.part[q];
       if (w.rest == 0.f && w.list == 0.f) continue;
-      const float f = q == best ? 1.f : exp2f(top.log2_of(w.ref, c));
+      const float step = top.log2_of(w.ref, c), f = q == best ? 1.f : exp2f(step);
       S += w.rest * f;
       L += w.list * f;
       if (POW != 0) {
-        const float f1 = q == best ? 1.f : exp2f(top1.log2_of(w.ref1, c1));
+        const float f1 = q == best ? 1.f : exp2f(rows::log2_at_one<POW>(step, top1, w.ref1));
         S1 += w.rest1 * f1;
         L1 += w.list1 * f1;
       }
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
     m = p.k >= p.vocab && all_listed >= p.vocab ? 0.f : sh.rest;
     const bool again = m > 0.f && S < kLeastRestSum;
     if (lane == 0) sh.again = again;
-    if (!again) finish(top, S, logf(S / total));
+    if (!again) finish(top, 1.f, 1.f, S, logf(S / total));
   }
   __syncthreads();
   if (sh.again) {  // the same for the whole cluster: the rest's sum, relative to the rest's own largest logit
@@ -349,7 +352,9 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
       S = 0.f;
       for (int q = 0; q < parts; ++q)
         if (sh.again_part[q].rest != 0.f) S += sh.again_part[q].rest * exp2f(own.log2_of(sh.again_part[q].ref, c));
-      finish(own, S, logf(S) + top.log_of(own, c, p.inv_tau) - logf(total));
+      const float step = top.log2_of(own, c);
+      finish(own, exp2f(step), exp2f(POW > 0 ? rows::log2_at_one<POW>(step, top1, rows::ref_at_one<POW>(own)) : step), S,
+             logf(S) + top.log_of(own, c, p.inv_tau) - logf(total));
     }
     __syncthreads();
   }
@@ -396,7 +401,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads) distill_kernel(const TZ* __
   if (rank == parts - 1)
     for (int i = p.vocab + tid; i < p.dz_cols; i += blockDim.x) drow[i] = from_f32<TG>(0.f);
   __syncthreads();
-  const float scale = scale_of(p, scale_of_all(p), row);
+  const float scale = sh.scale;
   const float kd = scale * p.kd * p.tau, ce = scale * p.ce;
   for (int i = tid; i < p.k; i += blockDim.x) {
     if (!list[i].owner) continue;
@@ -443,6 +448,8 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
   TTB_CHECK(a.dz == nullptr || a.dz_type == a.z_type ||
                 (a.z_type == ScalarType::kF32 && a.dz_type == ScalarType::kBF16),
             "distillation: the gradient has the logits' type, or bf16 for fp32 logits");
+  TTB_CHECK(a.factor == nullptr || (a.dz != nullptr && a.z_type == ScalarType::kF16 && a.dz_type == a.z_type),
+            "distillation: factors multiply an fp16 gradient");
   if (a.rows == 0) return;
   const rows::Plan plan = rows::plan_rows(a.rows, a.vocab, scalar_bytes(a.z_type));
   TTB_CHECK(a.rows * plan.parts <= 0x7FFFFFFFLL, "distillation: too many rows");
@@ -492,10 +499,7 @@ void distill_loss(const DistillArgs& a, cudaStream_t stream) {
     using TG = std::remove_pointer_t<decltype(dz)>;
     distill::with_pow(pow, [&](auto w) {
       constexpr int POW = decltype(w)::value;
-      if (dz == nullptr)
-        launch(distill_kernel<TZ, TG, false, POW>, z, dz);
-      else
-        launch(distill_kernel<TZ, TG, true, POW>, z, dz);
+      distill::with_form<TZ, TG>(a, [&](auto form) { launch(distill_kernel<TZ, TG, decltype(form)::value, POW>, z, dz); });
     });
   });
 }

@@ -58,8 +58,8 @@ struct DistillArgs {
   const long long* targets;   // [rows] or null; a negative target leaves its row out
   float tau, kd, ce;
   const float* scale;  // device scalar or null (1)
-  // What multiplies row r besides: factor[r * factor_step], or null (1).  A single factor (step 0) of 1 leaves loss and dz as
-  // they are: they hold the answer already.
+  // With an fp16 gradient of fp16 logits: what multiplies row r besides, factor[r * factor_step], or null (1).  A single factor
+  // (step 0) of 1 leaves loss and dz as they are: dz holds the answer already.
   const float* factor;
   int factor_step;
   float* loss;         // [rows]

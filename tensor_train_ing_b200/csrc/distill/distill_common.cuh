@@ -31,13 +31,19 @@ __device__ __forceinline__ float teacher_logit(const Params& p, long long i) {
   return to_f32(static_cast<const __half*>(p.t)[i]);
 }
 
+// What a kernel forms: the loss, its gradient too, or both once more with a factor (DistillArgs::factor; kernels of their own,
+// so that the others carry no code for it).
+constexpr int kLoss = 0, kGradient = 1, kAgain = 2;
+
+template <int FORM>
 __device__ __forceinline__ bool nothing_to_do(const Params& p) {
-  return p.factor != nullptr && p.factor_step == 0 && *p.factor == 1.f;
+  return FORM == kAgain && p.factor_step == 0 && *p.factor == 1.f;
 }
 // What multiplies a row's loss and gradient, `scale` being what multiplies all rows'.
 __device__ __forceinline__ float scale_of_all(const Params& p) { return p.scale != nullptr ? *p.scale : 1.f; }
+template <int FORM>
 __device__ __forceinline__ float scale_of(const Params& p, float scale, long long row) {
-  return p.factor != nullptr ? scale * p.factor[row * p.factor_step] : scale;
+  return FORM == kAgain ? scale * p.factor[row * p.factor_step] : scale;
 }
 
 // The smem element a listed column's slot holds while entries compete for it, as bits of a finite value.
@@ -55,7 +61,7 @@ __device__ __forceinline__ int get_mark(const T* p) {
 // Whether no entry before i names entry i's column.  Which of several entries stands for a column decides where its exponential
 // is added; the competition for its slot has some winner, this one has the same in every run.
 template <typename E>
-__device__ __forceinline__ bool first_of_column(const E* list, int i) {
+__device__ __noinline__ bool first_of_column(const E* list, int i) {
   for (int j = 0; j < i; ++j)
     if (list[j].col == list[i].col) return false;
   return true;
@@ -91,6 +97,15 @@ void with_pow(int pow, F&& f) {
     case 2: return f(std::integral_constant<int, 2>{});
     default: return f(std::integral_constant<int, 4>{});
   }
+}
+
+// f(std::integral_constant<int, FORM>) for these types.
+template <typename TZ, typename TG, typename F>
+void with_form(const DistillArgs& a, F&& f) {
+  if (a.dz == nullptr) return f(std::integral_constant<int, kLoss>{});
+  if (a.factor == nullptr) return f(std::integral_constant<int, kGradient>{});
+  if constexpr (std::is_same_v<TZ, __half> && std::is_same_v<TG, __half>)
+    f(std::integral_constant<int, kAgain>{});
 }
 
 // The kernel for many long rows (distill_ring.cu); false where it does not apply.

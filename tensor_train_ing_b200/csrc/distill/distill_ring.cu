@@ -254,10 +254,11 @@ __device__ __forceinline__ void patch_stages(TZ* sm, Listed* lists, Shared& sh, 
   }
 }
 
-template <typename TZ, typename TG, bool GRAD, int POW>
+template <typename TZ, typename TG, int FORM, int POW>
 __device__ __forceinline__ void consume(const TZ* z, TG* dz, const TZ* sm, const Listed* lists, Shared& sh,
                                         const Params& p, const Place& at, float c) {
   constexpr int E = Span<TZ>::kVec;
+  constexpr bool GRAD = FORM != kLoss;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int turn = 0;
   unsigned on_side = 0;  // bit s: the parity of the live rows side s has had
@@ -393,9 +394,10 @@ __device__ __forceinline__ float2 relative_sums(float& top, float sum, float sum
   return warp_sum2(make_float2(sum, sum1));
 }
 
-template <typename TG, bool GRAD, int POW>
+template <typename TG, int FORM, int POW>
 __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, const Params& p, const Place& at, float c,
                                             float c1) {
+  constexpr bool GRAD = FORM != kLoss;
   const int lane = threadIdx.x & 31;
   const float all_scale = scale_of_all(p);
   int turn = 0;
@@ -439,7 +441,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
       warp_arrives(&sh.side_free[side]);
       continue;
     }
-    const float scale = scale_of(p, all_scale, r.row);
+    const float scale = scale_of<FORM>(p, all_scale, r.row);
     // The unlisted columns' sums, relative to one reference: of this CTA, then of the row.  The consumers wait for what
     // follows, so independent sums go through the lanes together and quotients are the hardware's (2 ulp).
     const rows::WarpSum w = lane < kRingWarps ? sh.sums[side][lane] : rows::WarpSum{-CUDART_INF_F, 0.f, 0.f};
@@ -536,14 +538,14 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
   }
 }
 
-template <typename TZ, typename TG, bool GRAD, int POW>
+template <typename TZ, typename TG, int FORM, int POW>
 __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __restrict__ z, TG* __restrict__ dz,
                                                                   const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
   TZ* sm = reinterpret_cast<TZ*>(smem);
   auto* lists = reinterpret_cast<Listed*>(smem + static_cast<size_t>(p.per) * 16);
-  if (nothing_to_do(p)) return;  // the same for the whole grid
+  if (nothing_to_do<FORM>(p)) return;  // the same for the whole grid
   if (threadIdx.x == 0) {
     for (int g = 0; g < kStages; ++g) {
       mbar_init(&sh.full[g], 1);
@@ -570,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
   const float c = p.inv_tau * CUDART_L2E_F, c1 = POW == 1 ? CUDART_L2E_F : (POW > 1 ? POW : 1) * c;
   const int warp = threadIdx.x >> 5;
   if (warp < kRingWarps) {
-    consume<TZ, TG, GRAD, POW>(z, dz, sm, lists, sh, p, at, c);
+    consume<TZ, TG, FORM, POW>(z, dz, sm, lists, sh, p, at, c);
   } else if (warp == kProducer) {
     if ((threadIdx.x & 31) == 0) produce(z, sm, sh, p, at);
   } else if (warp == kLister) {
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_ring_kernel(const TZ* __r
   } else if (warp == kPatcher) {
     patch_stages(sm, lists, sh, p);
   } else {
-    finish_rows<TG, GRAD, POW>(dz, lists, sh, p, at, c, c1);
+    finish_rows<TG, FORM, POW>(dz, lists, sh, p, at, c, c1);
   }
   if (p.parts > 1) {  // no CTA leaves while another may still write to it
     __syncwarp();
@@ -604,8 +606,8 @@ int active_clusters(const void* kernel, const cudaLaunchConfig_t& cfg, int parts
 }  // namespace
 
 bool loss_by_ring(const DistillArgs& a, const Params& params, int pow, cudaStream_t stream) {
-  // Shorter rows go a CTA each, several to an SM.  Measured with 8288 rows, 64 listed: 32 KB (16384 bf16) 135 us here and
-  // 100 us there, with gradient 193 and 154; 64 KB (32768 bf16) 157 and 197, 249 and 282; (16384 fp32) 131 and 199, 229 and 264.
+  // Shorter rows go a CTA each, several to an SM.  Measured with 8288 rows, 64 listed: 32 KB (16384 bf16) 129 us here and
+  // 95 us there, with gradient 176 and 136; 64 KB (32768 bf16) 149 and 195, 232 and 261; (16384 fp32) 127 and 179, 211 and 248.
   constexpr size_t kLeastSlice = 48 * 1024;
   constexpr size_t kMostBytes = 113 * 1024;  // two CTAs on an SM
   const int E = 16 / scalar_bytes(a.z_type);
@@ -644,10 +646,7 @@ bool loss_by_ring(const DistillArgs& a, const Params& params, int pow, cudaStrea
     using TG = std::remove_pointer_t<decltype(dz)>;
     with_pow(pow, [&](auto w) {
       constexpr int POW = decltype(w)::value;
-      if (dz == nullptr)
-        launch(distill_ring_kernel<TZ, TG, false, POW>, z, dz);
-      else
-        launch(distill_ring_kernel<TZ, TG, true, POW>, z, dz);
+      with_form<TZ, TG>(a, [&](auto form) { launch(distill_ring_kernel<TZ, TG, decltype(form)::value, POW>, z, dz); });
     });
   });
   return true;

@@ -169,12 +169,6 @@ __device__ __forceinline__ float max_of(const uint4& u) {
   }
 }
 
-// log2 of o1 over ref1, references at temperature 1, where `step` is that of the references at tau that they go with.
-template <int POW>
-__device__ __forceinline__ float log2_at_one(float step, const Ref& ref1, const Ref& o1) {
-  return POW == 1 ? ref1.log2_of(o1, CUDART_L2E_F) : POW * step;
-}
-
 // A thread's running sums of exp((z - ref) / tau) and, for POW > 0, exp(z - ref), over whatever it has seen.  The
 // reference is the largest logit of its first vector that has one.  While `see` is called before every vector it moves when
 // one exceeds it by more than 2^40, at the temperature or at 1, so that no element adds more to either sum.  Vectors added

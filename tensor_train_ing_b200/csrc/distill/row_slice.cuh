@@ -215,6 +215,12 @@ __device__ __forceinline__ Ref ref_at_one(const Ref& ref) {
   if constexpr (POW > 1) r.r = POW * ref.r;
   return r;
 }
+// log2 of o1 over ref1, references at temperature 1, where `step` is that of the references at tau that they go with.
+template <int POW>
+__device__ __forceinline__ float log2_at_one(float step, const Ref& ref1, const Ref& o1) {
+  return POW == 1 ? ref1.log2_of(o1, CUDART_L2E_F) : POW * step;
+}
+
 // exp(z - reference) of a pair of logits, from e = exp((z - reference) / tau) where POW says so.
 template <int POW, bool FAR>
 __device__ __forceinline__ float2 at_one(float2 e, float2 z, const Ref& ref1) {

@@ -12,7 +12,7 @@
 //
 // Few rows, and rows shorter than the persistent kernel's.  Latency bounds it: the copy, the maxima, the bound and the ranking
 // follow one another, and only the other CTAs of the SM fill the gaps.  4 rows of 50257 fp32 logits, the top 32: 12 us with the
-// launch; 8288 rows of 32768 bf16, the top 8: 151 us (83 us for the bytes).
+// launch; 8288 rows of 32768 bf16, the top 8: 149 us (83 us for the bytes).
 #include "../common/host.h"
 #include "top_common.cuh"
 

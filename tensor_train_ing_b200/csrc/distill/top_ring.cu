@@ -372,8 +372,8 @@ bool top_logits_by_ring(const TopLogitsArgs& a, cudaStream_t stream) {
   const long long bytes = static_cast<long long>(a.vocab) * scalar_bytes(a.type);
   if (bytes / 16 / kRingThreads > 0xFFFF) return false;  // a vector's number is kept in 16 bits
   // A collector's time per row grows with k, a consumer's with the row's length.  Measured with 8288 bf16 rows, here and
-  // with a row per CTA: 32768 columns, top 8 158 and 151 us, top 64 220 and 188; 40960 columns 176 and 212, 231 and 251,
-  // top 128 351 and 324.  4144 fp32 rows of 32768 columns: top 8 107 and 196 us, top 128 177 and 269.
+  // with a row per CTA: 32768 columns, top 8 150 and 149 us, top 64 216 and 182; 40960 columns 165 and 210, 220 and 247,
+  // top 128 349 and 317.  4144 fp32 rows of 32768 columns: top 8 100 and 192 us, top 128 173 and 259.
   if (bytes < 80 * 1024 || a.k * 1024LL > bytes) return false;
   if (a.rows < 4LL * num_sms()) return false;  // few rows leave CTAs without any
   const size_t smem = kSlots * kChunkVectors * 16 + sizeof(Shared);

@@ -745,3 +745,19 @@ def test_teacher_rows_without_any_logit(n, dtype):
         assert torch.isfinite(got[0]).all()
         torch.testing.assert_close(got[0], want[0], rtol=64 * U, atol=64 * U)
         torch.testing.assert_close(got[1].float(), want[1].float(), rtol=2 * HALF_ULP[dtype] + 64 * U * 20, atol=1e-9)
+
+
+def test_factors_are_refused_where_they_have_no_kernel():
+    from tensor_train_ing_b200.ops._ext import lib
+    one = torch.ones(1, device="cuda")
+    ids, t = torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.zeros(4, 2, device="cuda")
+    for dtype in (F32, BF16, F16):
+        z = _logits(4, 50, dtype, 42)
+        for dz in (None, torch.empty_like(z)):
+            if dtype == F16 and dz is not None:
+                continue
+            with pytest.raises((RuntimeError, ValueError), match="factors"):
+                lib().distill_loss(z, ids, t, None, None, 1.0, 1.0, 0.0, None, dz, one)
+    with pytest.raises((RuntimeError, ValueError), match="factor"):
+        z = _logits(4, 50, F16, 42)
+        lib().distill_loss(z, ids, t, None, None, 1.0, 1.0, 0.0, None, torch.empty_like(z), torch.ones(3, device="cuda"))
