@@ -10,9 +10,10 @@
 // What they hand over is kept for several rows; every hand-over is an mbarrier with bounded waits, and a wait that runs
 // out ends all roles.  The arithmetic is that of distill.cu, of which this is the form for long rows: 4096 rows of 50257
 // bf16 logits, the loss alone, took 142 us there, with two CTAs of an SM each waiting through about 6 us of latencies per
-// row, and 93 us here (63 us for the bytes); loss and gradient of 8192 rows at tau 2 took 422 us and 335 us (252 us).  4096 rows
-// of 131072 fp32 logits, in clusters: 904 us (658 us).  The consumers bound it: special-function unit and issue slots are
-// half busy, with twelve warps of a CTA each in a chain of one vector's load, exponentials and sums.
+// row, and 92 us here (63 us for the bytes); loss and gradient of 8192 rows at tau 2 took 422 us and 333 us (252 us).  4096 rows
+// of 131072 fp32 logits, in clusters: 903 us (658 us).  8192 rows of 50257 fp32 logits with a bf16 gradient: 471 us (378 us).  No
+// unit is full (special functions and issue slots 50 to 57 %, DRAM 48 to 55 %): the twelve consumer warps of a CTA are each in a
+// chain of one vector's load, exponentials and sums.
 #include <map>
 #include <mutex>
 #include <tuple>

@@ -57,7 +57,9 @@ def factor_of(scale, count, reduction: str):
     if reduction == "sum":
         return scale
     inverse = count.clamp_min(1).double().reciprocal()
-    return inverse if scale is None else inverse * scale.detach().reshape(())
+    if scale is None:
+        return inverse
+    return inverse * (scale.detach().reshape(()) if isinstance(scale, torch.Tensor) else float(scale))
 
 
 def _rows(logits: torch.Tensor, what: str) -> torch.Tensor:
