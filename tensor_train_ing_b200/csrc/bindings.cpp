@@ -398,14 +398,12 @@ std::vector<Tensor> top_logits(const Tensor& z, int64_t k, double tau) {
   return {values, ids, lse};
 }
 
-// loss [N] fp32.  dz is given (its columns past V are zeroed) or not wanted.  factor, with an fp16 dz of fp16 logits: one number or
-// one per row that multiplies loss and gradient besides; a single 1 leaves dz as it is and the loss unset.
-Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c10::optional<Tensor>& teacher_lse,
-                    const c10::optional<Tensor>& targets, double tau, double kd, double ce,
-                    const c10::optional<Tensor>& scale, const c10::optional<Tensor>& dz,
-                    const c10::optional<Tensor>& factor = c10::nullopt) {
+// The checked arguments of the loss kernels, without the place of the loss.  dz is given (its columns past V are zeroed) or not wanted.
+ttb::DistillArgs distill_args(const Tensor& z, const Tensor& ids, const Tensor& t,
+                              const c10::optional<Tensor>& teacher_lse, const c10::optional<Tensor>& targets,
+                              double tau, double kd, double ce, const c10::optional<Tensor>& scale,
+                              const c10::optional<Tensor>& dz) {
   check_rows(z, "logits", z);
-  const c10::cuda::CUDAGuard guard(z.device());
   const int64_t N = z.size(0), V = z.size(1), K = ids.size(-1);
   TORCH_CHECK(V >= 1 && V < (1LL << 31), "the logits have no columns");
   for (const Tensor* q : {&ids, &t}) {
@@ -423,8 +421,6 @@ Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c
                 "targets must be dense int64 [rows] on the logits' device");
   TORCH_CHECK(ce == 0.0 || targets.has_value(), "the cross-entropy term needs targets");
   if (scale.has_value()) check_f32_vector(*scale, "scale", 1, z);
-  if (factor.has_value()) check_f32_vector(*factor, "factor", factor->numel() == 1 ? 1 : N, z);
-  auto loss = torch::empty({N}, z.options().dtype(torch::kFloat32));
   ttb::DistillArgs a{};
   a.z = z.data_ptr();
   a.ldz = z.stride(0);
@@ -442,9 +438,6 @@ Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c
   a.kd = static_cast<float>(kd);
   a.ce = static_cast<float>(ce);
   a.scale = scale.has_value() ? scale->data_ptr<float>() : nullptr;
-  a.factor = factor.has_value() ? factor->data_ptr<float>() : nullptr;
-  a.factor_step = factor.has_value() && factor->numel() > 1 ? 1 : 0;
-  a.loss = loss.data_ptr<float>();
   if (dz.has_value()) {
     check_rows(*dz, "dz", z);
     TORCH_CHECK(dz->size(0) == N && dz->size(1) >= V, "dz must have the logits' rows and at least their columns");
@@ -454,8 +447,35 @@ Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c
     a.dz_type = scalar_type(*dz, "dz");
   }
   a.status = ttb::status_ptr();
+  return a;
+}
+
+Tensor distill_loss_of(ttb::DistillArgs& a, const Tensor& z) {
+  Tensor loss = torch::empty({z.size(0)}, z.options().dtype(torch::kFloat32));
+  a.loss = loss.data_ptr<float>();
   ttb::distill_loss(a, cur_stream());
   return loss;
+}
+
+void set_factor(ttb::DistillArgs& a, const Tensor& factor) {
+  check_f32_vector(factor, "factor", factor.numel() == 1 ? 1 : a.rows, factor);
+  a.factor = factor.data_ptr<float>();
+  a.factor_step = factor.numel() > 1 ? 1 : 0;
+}
+
+// loss [N] fp32.  With an fp16 dz of fp16 logits, a factor (one number or one per row) multiplies the gradient besides; a single 1
+// leaves dz as it is, and the loss is not set.
+Tensor distill_loss(const Tensor& z, const Tensor& ids, const Tensor& t, const c10::optional<Tensor>& teacher_lse,
+                    const c10::optional<Tensor>& targets, double tau, double kd, double ce,
+                    const c10::optional<Tensor>& scale, const c10::optional<Tensor>& dz,
+                    const c10::optional<Tensor>& factor) {
+  const c10::cuda::CUDAGuard guard(z.device());
+  auto a = distill_args(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, dz);
+  if (factor.has_value()) {
+    TORCH_CHECK(factor->device() == z.device(), "factor must be on the logits' device");
+    set_factor(a, *factor);
+  }
+  return distill_loss_of(a, z);
 }
 
 // Rows of dz times g (one factor, or one per row), in place; a factor of 1 leaves its row untouched.
@@ -475,6 +495,31 @@ Tensor gradient_like(const Tensor& z) {
   return at::empty_strided({n, v}, {ld >= v && ld < v + 64 ? ld : v, 1}, z.options());
 }
 
+// The gradient of fp16 logits, formed again with the factor that the backward brings.
+struct FormAgain : torch::CustomClassHolder {
+  ttb::DistillArgs args;
+  std::vector<Tensor> inputs;  // what args point to besides z, which the node saves
+  std::vector<int64_t> versions;
+
+  FormAgain(const ttb::DistillArgs& a, std::initializer_list<c10::optional<Tensor>> tensors) : args(a) {
+    for (const auto& t : tensors)
+      if (t.has_value()) {
+        inputs.push_back(*t);
+        versions.push_back(version_of(*t));
+      }
+  }
+  static int64_t version_of(const Tensor& t) { return t.is_inference() ? 0 : static_cast<int64_t>(t._version()); }
+  void operator()(const Tensor& factor) {
+    for (size_t i = 0; i < inputs.size(); ++i)
+      TORCH_CHECK(version_of(inputs[i]) == versions[i],
+                  "distillation_loss: a list, target or scale was changed in place before the backward");
+    const c10::cuda::CUDAGuard guard(factor.device());
+    set_factor(args, factor);
+    args.loss = nullptr;
+    ttb::distill_loss(args, cur_stream());
+  }
+};
+
 // distill_loss with its gradient formed in the same pass over the logits and kept instead of them; the backward
 // multiplies it by the incoming factor in place, so it can run once.  A factor other than 1 then rounds bf16 a second time (another
 // 2^-9 of the value), which costs less than keeping the logits.  fp16 has no exponents for that: a loss scaler's factor
@@ -486,20 +531,20 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
                         double kd, double ce, const c10::optional<Tensor>& scale, bool total) {
     at::AutoDispatchBelowADInplaceOrView guard;
     Tensor dz = gradient_like(z);
-    Tensor loss = distill_loss(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, dz);
+    const c10::cuda::CUDAGuard device(z.device());
+    auto args = distill_args(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, dz);
+    Tensor loss = distill_loss_of(args, z);
     ctx->saved_data["dz"] = dz;
     if (z.scalar_type() == torch::kFloat16) {
-      ctx->save_for_backward({z, ids, t, teacher_lse.value_or(Tensor()), targets.value_or(Tensor()),
-                              scale.value_or(Tensor())});
-      ctx->saved_data["tau"] = tau;
-      ctx->saved_data["kd"] = kd;
-      ctx->saved_data["ce"] = ce;
+      ctx->save_for_backward({z});
+      ctx->saved_data["again"] = c10::IValue::make_capsule(c10::make_intrusive<FormAgain>(
+          args, std::initializer_list<c10::optional<Tensor>>{ids, t, teacher_lse, targets, scale}));
     }
     return total ? loss.sum() : loss;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    const auto saved = ctx->get_saved_variables();
+    const auto saved = ctx->get_saved_variables();  // fp16: the logits, unchanged
     at::AutoDispatchBelowADInplaceOrView guard;
     auto& kept = ctx->saved_data["dz"];
     TORCH_CHECK(kept.isTensor(), "distillation_loss: the gradient was handed out by an earlier backward");
@@ -509,9 +554,9 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
     if (saved.empty()) {
       scale_rows_(dz, factor);
     } else {
-      const auto given = [](const Tensor& q) { return q.defined() ? c10::optional<Tensor>(q) : c10::nullopt; };
-      distill_loss(saved[0], saved[1], saved[2], given(saved[3]), given(saved[4]), ctx->saved_data["tau"].toDouble(),
-                   ctx->saved_data["kd"].toDouble(), ctx->saved_data["ce"].toDouble(), given(saved[5]), dz, factor);
+      auto& again = ctx->saved_data["again"];
+      (*c10::static_intrusive_pointer_cast<FormAgain>(again.toCapsule()))(factor);
+      again = c10::IValue();
     }
     if (dz.size(0) > 0) autograd_launches += 1;
     torch::autograd::variable_list out(10);
@@ -528,7 +573,7 @@ Tensor distillation(const Tensor& z, const Tensor& ids, const Tensor& t, const c
   refuse_tangent("distillation_loss", z);
   if (at::GradMode::is_enabled() && z.requires_grad())
     return DistillNode::apply(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, total);
-  const Tensor loss = distill_loss(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, c10::nullopt);
+  const Tensor loss = distill_loss(z, ids, t, teacher_lse, targets, tau, kd, ce, scale, c10::nullopt, c10::nullopt);
   return total ? loss.sum() : loss;
 }
 
@@ -1062,8 +1107,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("z"), py::arg("k"), py::arg("tau"));
   m.def("distill_loss", &distill_loss, "distillation loss of each row and, into dz, its gradient", py::arg("z"),
         py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),
-        py::arg("ce"), py::arg("scale"), py::arg("dz"),
-        py::arg("factor") = py::none());
+        py::arg("ce"), py::arg("scale"), py::arg("dz"), py::arg("factor") = py::none());
   m.def("scale_rows_", &scale_rows_, "rows of dz times their factor, in place", py::arg("dz"), py::arg("g"));
   m.def("distillation", &distillation, "distillation loss of rows or their sum, differentiable", py::arg("z"),
         py::arg("ids"), py::arg("t"), py::arg("teacher_lse"), py::arg("targets"), py::arg("tau"), py::arg("kd"),

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads, 3) distill_kernel(const TZ*
     target = p.targets[row];
     if (target >= p.vocab && rank == 0 && tid == 0) record_error(p.status, kErrBadIndex);
     if (target < 0 || target >= p.vocab) {  // the same for the whole cluster
-      if (rank == 0 && tid == 0) p.loss[row] = 0.f;
+      if (FORM != distill::kAgain && rank == 0 && tid == 0) p.loss[row] = 0.f;
       if (GRAD) zero_row(drow, p.dz_cols, rank * blockDim.x + tid, parts * blockDim.x);
       return;
     }
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(rows::kMaxThreads, 3) distill_kernel(const TZ*
       sh.inv_sum1 = 1.f / total1;
       sh.all_mass = mass;
     }
-    if (rank == 0) {
+    if (FORM != distill::kAgain && rank == 0) {
       const float log2_total = log2f(total);
       float kl = 0.f;
       for (int i = lane; i < p.k; i += 32) {

@@ -59,10 +59,10 @@ struct DistillArgs {
   float tau, kd, ce;
   const float* scale;  // device scalar or null (1)
   // With an fp16 gradient of fp16 logits: what multiplies row r besides, factor[r * factor_step], or null (1).  A single factor
-  // (step 0) of 1 leaves loss and dz as they are: dz holds the answer already.
+  // (step 0) of 1 leaves dz as it is: it holds the answer already.  The loss is not written then.
   const float* factor;
   int factor_step;
-  float* loss;         // [rows]
+  float* loss;         // [rows]; with a factor unused
   void* dz;            // null: no gradient.  [rows, dz_cols], rows lddz apart; columns past vocab are written as zeros
   long long lddz;
   int dz_cols;

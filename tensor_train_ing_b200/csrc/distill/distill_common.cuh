@@ -31,8 +31,8 @@ __device__ __forceinline__ float teacher_logit(const Params& p, long long i) {
   return to_f32(static_cast<const __half*>(p.t)[i]);
 }
 
-// What a kernel forms: the loss, its gradient too, or both once more with a factor (DistillArgs::factor; kernels of their own,
-// so that the others carry no code for it).
+// What a kernel forms: the loss, its gradient too, or the gradient once more with a factor (DistillArgs::factor; kernels of
+// their own, so that the others carry no code for it).
 constexpr int kLoss = 0, kGradient = 1, kAgain = 2;
 
 template <int FORM>

@@ -438,7 +438,7 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     }
     if (GRAD && !warp_waits(&sh.sums_ready[side], (n / kSides) & 1, &sh.stop, p.status)) return;
     if (!r.live) {
-      if (lane == 0 && at.rank == 0) p.loss[r.row] = 0.f;
+      if (FORM != kAgain && lane == 0 && at.rank == 0) p.loss[r.row] = 0.f;
       warp_arrives(&sh.side_free[side]);
       continue;
     }
@@ -496,14 +496,14 @@ __device__ __forceinline__ void finish_rows(TG* dz, Listed* lists, Shared& sh, c
     }
     const float log2_total = log2f(total);
     float kl = 0.f;
-    if (at.rank == 0) {
+    if (FORM != kAgain && at.rank == 0) {
       for (int i = lane; i < p.k; i += 32) {
         const float logq = (ref.log2_of(list[i].z, c) - log2_total) * CUDART_LN2_F;
         if (list[i].p != 0.f) kl += list[i].p * (list[i].logp - logq);
       }
       kl = warp_sum(kl);
     }
-    if (lane == 0 && at.rank == 0) {
+    if (FORM != kAgain && lane == 0 && at.rank == 0) {
       // log q_rest from its parts: the probability itself may leave fp32's range
       if (m > 0.f) kl += m * ((log2f(m) - log2f(S) + log2_total) * CUDART_LN2_F - ref.log_of(own, c, p.inv_tau));
       float loss = p.kd != 0.f ? p.kd * p.tau * p.tau * kl : 0.f;

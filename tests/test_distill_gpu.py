@@ -761,3 +761,33 @@ def test_factors_are_refused_where_they_have_no_kernel():
     with pytest.raises((RuntimeError, ValueError), match="factor"):
         z = _logits(4, 50, F16, 42)
         lib().distill_loss(z, ids, t, None, None, 1.0, 1.0, 0.0, None, torch.empty_like(z), torch.ones(3, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_lists_from_inference_mode(dtype):
+    teacher = _logits(6, 900, dtype, 43)
+    with torch.inference_mode():
+        top = _ops().top_logits(teacher, 8, temperature=2.0)
+        y = _targets(6, 900, top.ids, 44)
+        scale = torch.full((1,), 0.5, device="cuda")
+    z = _logits(6, 900, dtype, 45).requires_grad_(True)
+    loss = lambda *a: _ops().distillation_loss(z, *a, temperature=2.0, ce_weight=0.5, scale=0.5)  # noqa: E731
+    (want,) = torch.autograd.grad(4.0 * loss(top.ids.clone(), top.values.clone(), top.lse.clone(), y.clone()), z)
+    (got,) = torch.autograd.grad(4.0 * _ops().distillation_loss(z, top.ids, top.values, top.lse, y, temperature=2.0,
+                                                              ce_weight=0.5, scale=scale), z)
+    assert torch.equal(got, want) and got.any()
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_fp16_inputs_changed_before_the_backward_are_reported(which):
+    z = _logits(6, 900, F16, 46)
+    ids, t, lse = _teacher(z, 6, F32, 47, True, 1.0)
+    y, scale = _targets(6, 900, ids, 48), torch.ones(1, device="cuda")
+    zz = z.clone().requires_grad_(True)
+    logits = zz * 1
+    inputs = [logits, ids, t, lse, y, scale]
+    loss = _ops().distillation_loss(logits, ids, t, lse, y, ce_weight=0.5, scale=scale)
+    with torch.no_grad():
+        inputs[which].add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation|changed in place"):
+        torch.autograd.grad(8.0 * loss, zz)
