@@ -430,14 +430,17 @@ class LinearDistillFn(torch.autograd.Function):
             total += lib().distill_loss(z[: e - s, :V], ids[s:e], t[s:e], lse[s:e] if lse is not None else None,
                                         targets[s:e], tau, kd, ce, scale, dz[s:e] if keep else None).sum()
         if grad:
-            ctx.save_for_backward(x, targets, ids, t, lse, scale)
+            # lists made in inference mode cannot be saved as such
+            ctx.made = [q if q is not None and q.is_inference() else None for q in (targets, ids, t, lse, scale)]
+            ctx.save_for_backward(x, *(q if m is None else None for q, m in zip((targets, ids, t, lse, scale), ctx.made)))
         ctx.group, ctx.dz, ctx.args = group, dz, (V, alpha, chunk, tau, kd, ce)
         return total
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, targets, ids, t, lse, scale = ctx.saved_tensors
+        x, *saved = ctx.saved_tensors
+        targets, ids, t, lse, scale = (q if m is None else m for q, m in zip(saved, ctx.made))
         V, alpha, chunk, tau, kd, ce = ctx.args
         group, dz = ctx.group, ctx.dz
         ctx.dz = None

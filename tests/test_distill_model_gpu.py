@@ -161,3 +161,18 @@ def test_the_mean_is_the_sum_with_its_factor_inside(fused):
             assert torch.equal(p.grad, want[name]), name
     _, none = model(idx, targets=torch.full_like(y, -100), teacher=teacher)
     assert none == 0
+
+
+@pytest.mark.parametrize("keep", [8 << 30, 0])
+def test_lists_from_inference_mode_train_the_fused_path(keep, monkeypatch):
+    from tensor_train_ing_b200.ops.fused import LinearDistillFn
+    monkeypatch.setattr(LinearDistillFn, "KEEP_BYTES", keep)
+    model = _model()
+    idx, y, teacher = _batch()
+    loss, grads = _run(model, idx, y, teacher)
+    with torch.inference_mode():
+        made = teacher._replace(ids=teacher.ids.clone(), values=teacher.values.clone(), lse=teacher.lse.clone())
+    again, ref = _run(model, idx, y, made)
+    assert torch.equal(loss, again)
+    for name, g in grads.items():
+        assert torch.equal(g, ref[name]), name
