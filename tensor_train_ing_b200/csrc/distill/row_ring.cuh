@@ -192,7 +192,7 @@ struct Sums {
   // to this logit, `above` the reference by so many powers of two
   __device__ __forceinline__ void move(float logit, float above, float c) {
     const Ref next(logit, c), next1 = ref_at_one<POW>(next);
-    if (set && sum() < CUDART_INF_F) {  // an infinite sum stays one (times a factor that underflows it would be NaN)
+    if (set && !overflowed()) {  // sums past kSafeSum stay so: a factor that underflows would hide what they lose
       const float step = next.excess(c) - above;
       const float2 f = both(fast_exp2(step));
       acc[0] = mul2(acc[0], f);

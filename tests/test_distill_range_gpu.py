@@ -148,3 +148,23 @@ def test_a_rest_far_below_the_list(n):
     t = torch.tensor([[1.0, 0.5, 0.0]], device="cuda").repeat(n, 1)
     lse = torch.logsumexp(t, 1) + 0.3
     _compare(z, z, ids, t, lse, None, 1.0, 1.0, 0.0)
+
+
+# Rows off 16 bytes: their first and last columns are added one by one, after the others.
+@pytest.mark.parametrize("n", [700, 91])
+@pytest.mark.parametrize("dtype,v,offset", [(F32, 36226, 1), (BF16, 36226, 3), (BF16, 50257, 5)])
+@pytest.mark.parametrize("tau,ce", [(1.0, 0.0), (1.3, 0.5), (2.0, 0.5), (4.0, 0.5), (6.0, 0.5)])
+def test_finite_masks_and_the_rows_ends(n, dtype, v, offset, tau, ce):
+    z = _logits(n, v, dtype, 83, ld=v, offset=offset, spread=0.3)
+    lows = (-70.0, -80.0, -86.0, -87.0, -87.5, -88.0, -88.5, -90.0)
+    places = (1, 9, 1001, 15003, 32507, v - 601, v - 9, v - 3, v - 1)
+    for r in range(n):
+        at, low = places[r // len(lows) % len(places)], lows[r % len(lows)]
+        if r % 2:
+            z[r, :at] = low
+        else:  # the last columns alone lie below, or the first
+            z[r, -at:] = low if r % 4 else z[r, -at:]
+            z[r, -1] = 0.5
+    ids, t, lse = _teacher(z, 5, F32, 84, True, tau)
+    _check_loss(z, ids, t, lse, _targets(n, v, ids, 85), tau, 0.8, ce, 0.5)
+    _check_top(z, 8, tau)
